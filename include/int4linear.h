@@ -184,6 +184,81 @@ int int4linear_linear_fp6_converted(const void *x_conv_d, const void *w_conv_d, 
                                     const float *row_scale_d, const float *col_scale_d, void *y_d,
                                     int out_type, int m, int n, int k, void *stream);
 
+/*
+ * MXFP4: 4-bit floats with block scales, which gfx950's matrix cores multiply as they are.
+ * (The reference has no counterpart; its operands carry no scales.)
+ *
+ * A rows x k matrix is two device arrays, both row-major and 16-byte aligned:
+ *   codes   two E2M1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) per byte, even k
+ *           in the low nibble as in the packed s4 layout; a row takes 128 bytes per 256 k
+ *           begun, what is behind k being zeros;
+ *   scales  one E8M0 byte s per 32 k: 2^(s - 127), 255 a NaN; a row takes 16 bytes per 512 k
+ *           begun, zeros behind k.
+ * int4linear_mxfp4_code_bytes and _scale_bytes are the arrays' sizes (0 for a negative size).
+ * Any k >= 0 is accepted; sizes beyond 2^30 are refused with INT4LINEAR_ERR_UNSUPPORTED.
+ *
+ * All calls are asynchronous on `stream`, allocate nothing, take no locks and do not touch the
+ * library's workspace: they may be captured into a graph once the device is set up.  Types are
+ * INT4LINEAR_OUT_F32, _F16 or _BF16.  Sums are held in float.
+ */
+size_t int4linear_mxfp4_code_bytes(int rows, int k);
+size_t int4linear_mxfp4_scale_bytes(int rows, int k);
+
+/* x_d (rows x k of `type`, `ld` >= k elements between rows, aligned to its element) -> MXFP4.  A
+ * block's scale is 2^e with e = max(-127, floor(log2(max |x|)) - 2); x 2^-e goes to the nearest
+ * E2M1 value, ties to the even code, beyond 6 to 6.  A block with an infinity or a NaN becomes NaN
+ * (scale 255).  The padding of codes and scales is written too. */
+int int4linear_mxfp4_quantize(const void *x_d, int type, size_t ld, void *codes_d, void *scales_d,
+                              int rows, int k, void *stream);
+/* The way back: y_d (rows x k of `type`, `ld` >= k elements between rows). */
+int int4linear_mxfp4_dequantize(const void *codes_d, const void *scales_d, void *y_d, int type,
+                                size_t ld, int rows, int k, void *stream);
+
+/* Y[m x n] = X[m x k] W[n x k]^T + bias, rounded once to out_type; y_d contiguous, 16-byte
+ * aligned.  bias_d: n floats or NULL.  k == 0 gives the bias. */
+int int4linear_mxfp4_linear(const void *x_codes_d, const void *x_scales_d, const void *w_codes_d,
+                            const void *w_scales_d, const float *bias_d, void *y_d, int out_type,
+                            int m, int n, int k, void *stream);
+
+/* The gated feed-forward block's first half in one kernel: H[m x n] = act(X Wg^T) * (X Wu^T).
+ * SILU: g / (1 + e^-g).  GELU: g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2. */
+enum {
+    INT4LINEAR_ACT_SILU = 0,
+    INT4LINEAR_ACT_GELU = 1
+};
+int int4linear_mxfp4_gated(const void *x_codes_d, const void *x_scales_d, const void *wg_codes_d,
+                           const void *wg_scales_d, const void *wu_codes_d, const void *wu_scales_d,
+                           int activation, void *h_d, int out_type, int m, int n, int k, void *stream);
+/* The same with H in MXFP4 (m x n, quantised from the float product): the down projection's operand. */
+int int4linear_mxfp4_gated_quantized(const void *x_codes_d, const void *x_scales_d, const void *wg_codes_d,
+                                     const void *wg_scales_d, const void *wu_codes_d,
+                                     const void *wu_scales_d, int activation, void *h_codes_d,
+                                     void *h_scales_d, int m, int n, int k, void *stream);
+
+/* Gradients of int4linear_mxfp4_linear at the values that X and W stand for (a training step hands
+ * them on to what was quantised as they are):
+ *   dx (m x k, bfloat16) = dy W,  dw (n x k, dw_type) = dy^T X,  dbias (n floats) = column sums of dy.
+ * dy_d is m x n bfloat16, contiguous, 16-byte aligned like dx_d and dw_d; dx_d, dw_d and dbias_d may
+ * each be NULL (not wanted).  dw_type: INT4LINEAR_OUT_BF16 or _F32.  work_d: a 256-byte aligned device
+ * buffer of at least int4linear_mxfp4_linear_backward_bytes(m, n, k) bytes, else INT4LINEAR_ERR_SCRATCH. */
+size_t int4linear_mxfp4_linear_backward_bytes(int m, int n, int k);
+int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, const void *x_scales_d,
+                                     const void *w_codes_d, const void *w_scales_d, void *dx_d, void *dw_d,
+                                     int dw_type, float *dbias_d, void *work_d, size_t work_bytes,
+                                     int m, int n, int k, void *stream);
+
+/* Gradients of int4linear_mxfp4_gated from dh_d (m x n bfloat16), likewise.  The projections are computed
+ * again from the operands, so the forward pass has nothing to keep:
+ *   dg = dh u act'(g), du = dh act(g) (each rounded to bfloat16 for the products that follow),
+ *   dx = dg Wg + du Wu,  dwg = dg^T X,  dwu = du^T X.
+ * dx_d may be NULL, and so may dwg_d and dwu_d together. */
+size_t int4linear_mxfp4_gated_backward_bytes(int m, int n, int k);
+int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, const void *x_scales_d,
+                                    const void *wg_codes_d, const void *wg_scales_d,
+                                    const void *wu_codes_d, const void *wu_scales_d, int activation,
+                                    void *dx_d, void *dwg_d, void *dwu_d, int dw_type, void *work_d,
+                                    size_t work_bytes, int m, int n, int k, void *stream);
+
 /* Bytes of internal workspace INT4LINEAR_KERNEL_AUTO would use for a shape on the current
  * device (0 when the chosen kernel needs none).  Sets the device up if that has not
  * happened yet, so the answer does not depend on what was called before.  It is that of the kernel

@@ -24,6 +24,17 @@ from .api import (  # noqa: F401
     linear_v11_launch,
     linear_v20_launch,
     linear_v21_launch,
+    mxfp4_code_bytes,
+    mxfp4_dequantize,
+    mxfp4_gated,
+    mxfp4_gated_backward,
+    mxfp4_gated_backward_bytes,
+    mxfp4_gated_quantized,
+    mxfp4_linear,
+    mxfp4_linear_backward,
+    mxfp4_linear_backward_bytes,
+    mxfp4_quantize,
+    mxfp4_scale_bytes,
     pack,
     pack_device,
     pack_rows,

@@ -35,6 +35,19 @@ C_ABI = [
     ("int4linear_gemm_fp6_converted", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     ("int4linear_linear_fp6_converted", c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                                 c_int, c_int, c_int, c_void_p]),
+    ("int4linear_mxfp4_code_bytes", c_size_t, [c_int, c_int]),
+    ("int4linear_mxfp4_scale_bytes", c_size_t, [c_int, c_int]),
+    ("int4linear_mxfp4_quantize", c_int, [c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    ("int4linear_mxfp4_dequantize", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_int, c_int, c_void_p]),
+    ("int4linear_mxfp4_linear", c_int, [c_void_p] * 6 + [c_int] * 4 + [c_void_p]),
+    ("int4linear_mxfp4_gated", c_int, [c_void_p] * 6 + [c_int, c_void_p] + [c_int] * 4 + [c_void_p]),
+    ("int4linear_mxfp4_gated_quantized", c_int, [c_void_p] * 6 + [c_int, c_void_p, c_void_p] + [c_int] * 3 + [c_void_p]),
+    ("int4linear_mxfp4_linear_backward_bytes", c_size_t, [c_int, c_int, c_int]),
+    ("int4linear_mxfp4_linear_backward", c_int,
+     [c_void_p] * 7 + [c_int, c_void_p, c_void_p, c_size_t] + [c_int] * 3 + [c_void_p]),
+    ("int4linear_mxfp4_gated_backward_bytes", c_size_t, [c_int, c_int, c_int]),
+    ("int4linear_mxfp4_gated_backward", c_int,
+     [c_void_p] * 7 + [c_int] + [c_void_p] * 3 + [c_int, c_void_p, c_size_t] + [c_int] * 3 + [c_void_p]),
     ("int4linear_workspace_bytes", c_size_t, [c_int, c_int, c_int]),
     ("int4linear_set_workspace_limit", None, [c_size_t]),
     ("int4linear_release_workspace", c_int, []),

@@ -151,6 +151,116 @@ def linear_fp6_converted(x_conv_d, w_conv_d, bias_d, row_scale_d, col_scale_d, y
                                                    stream))
 
 
+ACTIVATIONS = {"silu": 0, "gelu": 1}  # INT4LINEAR_ACT_*
+
+
+def mxfp4_code_bytes(rows: int, k: int) -> int:
+    """Bytes of a rows x k matrix's codes in MXFP4 (a row: 128 per 256 k begun)."""
+    return int(_lib.load().int4linear_mxfp4_code_bytes(rows, k))
+
+
+def mxfp4_scale_bytes(rows: int, k: int) -> int:
+    """Bytes of a rows x k matrix's scales in MXFP4 (a row: 16 per 512 k begun)."""
+    return int(_lib.load().int4linear_mxfp4_scale_bytes(rows, k))
+
+
+def mxfp4_quantize(x_d, codes_d, scales_d, rows: int, k: int, *, in_type: str = "bf16", ld: int | None = None,
+                   stream: int | None = None) -> None:
+    """x_d (rows x k of in_type "f32", "f16" or "bf16", ld elements between rows, k if None) -> MXFP4."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_mxfp4_quantize(_ptr(x_d), OUT_TYPES[in_type], k if ld is None else ld, _ptr(codes_d),
+                                             _ptr(scales_d), rows, k, stream))
+
+
+def mxfp4_dequantize(codes_d, scales_d, y_d, rows: int, k: int, *, out_type: str = "bf16", ld: int | None = None,
+                     stream: int | None = None) -> None:
+    """MXFP4 -> y_d (rows x k of out_type, ld elements between rows, k if None)."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_mxfp4_dequantize(_ptr(codes_d), _ptr(scales_d), _ptr(y_d), OUT_TYPES[out_type],
+                                               k if ld is None else ld, rows, k, stream))
+
+
+def mxfp4_linear(x_codes_d, x_scales_d, w_codes_d, w_scales_d, bias_d, y_d, out_type: str, m: int, n: int, k: int, *,
+                 stream: int | None = None) -> None:
+    """Y (m x n of out_type) = X * W^T + bias for MXFP4 operands; bias_d (n float32) may be None."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_mxfp4_linear(_ptr(x_codes_d), _ptr(x_scales_d), _ptr(w_codes_d), _ptr(w_scales_d),
+                                           _ptr(bias_d), _ptr(y_d), OUT_TYPES[out_type], m, n, k, stream))
+
+
+def mxfp4_gated(x_codes_d, x_scales_d, wg_codes_d, wg_scales_d, wu_codes_d, wu_scales_d, h_d, out_type: str, m: int,
+                n: int, k: int, *, activation: str = "silu", stream: int | None = None) -> None:
+    """H (m x n of out_type) = act(X * Wg^T) * (X * Wu^T) in one kernel; activation "silu" or "gelu"."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_mxfp4_gated(_ptr(x_codes_d), _ptr(x_scales_d), _ptr(wg_codes_d), _ptr(wg_scales_d),
+                                          _ptr(wu_codes_d), _ptr(wu_scales_d), ACTIVATIONS[activation], _ptr(h_d),
+                                          OUT_TYPES[out_type], m, n, k, stream))
+
+
+def mxfp4_gated_quantized(x_codes_d, x_scales_d, wg_codes_d, wg_scales_d, wu_codes_d, wu_scales_d, h_codes_d,
+                          h_scales_d, m: int, n: int, k: int, *, activation: str = "silu",
+                          stream: int | None = None) -> None:
+    """mxfp4_gated with H in MXFP4, the form the down projection takes."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_mxfp4_gated_quantized(_ptr(x_codes_d), _ptr(x_scales_d), _ptr(wg_codes_d),
+                                                    _ptr(wg_scales_d), _ptr(wu_codes_d), _ptr(wu_scales_d),
+                                                    ACTIVATIONS[activation], _ptr(h_codes_d), _ptr(h_scales_d), m, n, k,
+                                                    stream))
+
+
+def _work(work_d) -> tuple[int, int]:
+    """Address and bytes of a workspace: a tensor, or None."""
+    return (0, 0) if work_d is None else (work_d.data_ptr(), work_d.numel() * work_d.element_size())
+
+
+def mxfp4_linear_backward_bytes(m: int, n: int, k: int) -> int:
+    """Bytes of workspace mxfp4_linear_backward needs."""
+    return int(_lib.load().int4linear_mxfp4_linear_backward_bytes(m, n, k))
+
+
+def mxfp4_linear_backward(dy_d, x_codes_d, x_scales_d, w_codes_d, w_scales_d, dx_d, dw_d, dw_type: str, dbias_d, work_d,
+                          m: int, n: int, k: int, *, stream: int | None = None) -> None:
+    """dx (bfloat16) = dy W, dw (dw_type "bf16" or "f32") = dy^T X, dbias (float32) = column sums of dy
+    (bfloat16); dx_d, dw_d and dbias_d may each be None.  work_d: a tensor of at least
+    mxfp4_linear_backward_bytes(m, n, k) bytes."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_mxfp4_linear_backward(_ptr(dy_d), _ptr(x_codes_d), _ptr(x_scales_d), _ptr(w_codes_d),
+                                                    _ptr(w_scales_d), _ptr(dx_d), _ptr(dw_d), OUT_TYPES[dw_type],
+                                                    _ptr(dbias_d), *_work(work_d), m, n, k, stream))
+
+
+def mxfp4_gated_backward_bytes(m: int, n: int, k: int) -> int:
+    """Bytes of workspace mxfp4_gated_backward needs."""
+    return int(_lib.load().int4linear_mxfp4_gated_backward_bytes(m, n, k))
+
+
+def mxfp4_gated_backward(dh_d, x_codes_d, x_scales_d, wg_codes_d, wg_scales_d, wu_codes_d, wu_scales_d, dx_d, dwg_d,
+                         dwu_d, dw_type: str, work_d, m: int, n: int, k: int, *, activation: str = "silu",
+                         stream: int | None = None) -> None:
+    """Gradients of mxfp4_gated from dh (bfloat16): dx (bfloat16), dwg and dwu (dw_type "bf16" or "f32");
+    dx_d, or dwg_d and dwu_d together, may be None.  work_d: a tensor of at least
+    mxfp4_gated_backward_bytes(m, n, k) bytes."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_mxfp4_gated_backward(_ptr(dh_d), _ptr(x_codes_d), _ptr(x_scales_d), _ptr(wg_codes_d),
+                                                   _ptr(wg_scales_d), _ptr(wu_codes_d), _ptr(wu_scales_d),
+                                                   ACTIVATIONS[activation], _ptr(dx_d), _ptr(dwg_d), _ptr(dwu_d),
+                                                   OUT_TYPES[dw_type], *_work(work_d), m, n, k, stream))
+
+
 def workspace_bytes(m: int, n: int, k: int) -> int:
     """Internal workspace the automatic dispatch would use for this shape."""
     return int(_lib.load().int4linear_workspace_bytes(m, n, k))

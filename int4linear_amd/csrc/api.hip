@@ -1,6 +1,7 @@
 // C ABI of libint4linear.so, shape dispatch, and the reference's C++-linkage shims.
 #include "../../include/int4linear.h"
 #include "kernels.h"
+#include "mxfp4.h"
 
 #include <atomic>
 #include <cstdint>
@@ -84,6 +85,8 @@ hipError_t set_up_device(PerDevice &pd, int dev)
         err = fp6_init(pd.info);
     if (err == hipSuccess)
         err = skinny_init(pd.info);
+    if (err == hipSuccess)
+        err = line_gemm_init(pd.info);
     if (err == hipSuccess)  // `dev` is current here: the addresses are this device's copies
         err = hipGetSymbolAddress((void **)&pd.scratch, HIP_SYMBOL(scratch));
     if (err == hipSuccess)
@@ -773,3 +776,19 @@ void linear_v21_launch(void *x, void *w, void *y, int m, int n, int k)
 {
     launch_version("linear_v21_launch", 21, x, w, y, m, n, k);
 }
+
+// What the other file of the C ABI (api_mxfp4.hip) shares with this one.
+namespace int4linear {
+
+int api_begin(hipStream_t stream, DeviceInfo *info)
+{
+    PerDevice *pd = nullptr;
+    const int st = ensure_init(&pd, true, stream);
+    if (st == INT4LINEAR_OK)
+        *info = pd->info;
+    return st;
+}
+
+int api_status(hipError_t e) { return e == hipSuccess ? INT4LINEAR_OK : fail_hip(e); }
+
+}  // namespace int4linear

@@ -1,0 +1,75 @@
+// MXFP4 matrices: the format, and the launchers between api_mxfp4.hip and the kernel files.
+//
+// A row is cut into blocks of 32 values along k.  A block has one scale, 2^(s - 127) with s in 8
+// bits (E8M0; s = 255: the block is NaN), and 32 values of 4 bits (E2M1: sign, two exponent bits, one
+// mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two per byte, even k in the low nibble as in the packed
+// s4 layout.  Codes and scales are two arrays, row-major, both padded at the end of each row with
+// zeros: codes to 128 bytes (256 k, one line of the caches and one stage of the GEMM), scales to 16
+// (512 k, one load of a lane for two stages).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace int4linear {
+
+constexpr int kMxBlock = 32;      // values that share a scale
+constexpr int kLineBytes = 128;   // codes of 256 k
+constexpr int kLineFp4 = 256;     // k in a line of 4-bit values
+constexpr int kLineBf16 = 64;     // k in a line of bfloat16
+
+inline size_t mx_code_stride(int k) { return ((size_t)k + 255) / 256 * 128; }
+inline size_t mx_scale_stride(int k) { return ((size_t)k + 511) / 512 * 16; }
+
+// A matrix in MXFP4 whose rows are `rows` x k values.
+struct MxMatrix {
+    const uint8_t *codes;
+    const uint8_t *scales;
+    int rows;
+};
+
+// act(g) * u; the gelu is its tanh form.
+enum Activation : int { kSilu = 0, kGelu = 1 };
+
+// x (rows x k of `type`, an OutKind other than kOutS32; ld elements between rows) -> codes, scales.
+hipError_t launch_mx_quantize(const void *x, int type, size_t ld, uint8_t *codes, uint8_t *scales, int rows, int k,
+                              hipStream_t stream);
+// The way back: y = what codes and scales stand for.
+hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld, int k, hipStream_t stream);
+// dst[c * ld + r] = q[r][c] in bfloat16 for c < k; r goes on to the next multiple of 64 with zeros.
+hipError_t launch_mx_dequantize_transposed(const MxMatrix &q, uint16_t *dst, size_t ld, int k, hipStream_t stream);
+// src (rows x cols bfloat16, contiguous) -> transposed (cols x ld_t, zeros behind the rows); where they are
+// not null, padded (rows x ld_p, zeros behind the columns) and sums (cols floats: each column's sum, by way of
+// partial: ceil(rows / 64) x cols floats).
+hipError_t launch_bf16_transpose(const uint16_t *src, int rows, int cols, uint16_t *transposed, size_t ld_t, uint16_t *padded,
+                                 size_t ld_p, float *sums, float *partial, hipStream_t stream);
+
+hipError_t line_gemm_init(const DeviceInfo &dev);
+
+// y = x w^T + bias.  bias: n floats or null; out: an OutKind other than kOutS32.
+hipError_t launch_mx_linear(const MxMatrix &x, const MxMatrix &w, const float *bias, void *y, int out, int k, const DeviceInfo &dev,
+                            hipStream_t stream);
+// h = act(x wg^T) * (x wu^T), as an array of `out` ...
+hipError_t launch_mx_gated(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, void *h, int out, int k,
+                           const DeviceInfo &dev, hipStream_t stream);
+// ... or in MXFP4.
+hipError_t launch_mx_gated_quantized(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, uint8_t *codes,
+                                     uint8_t *scales, int k, const DeviceInfo &dev, hipStream_t stream);
+// Gradients of the two projections from dh (m x n bfloat16): d is m x 2 * ld_n, dg in columns 0 .. ld_n - 1 and du
+// behind them, dt is 2 * n x ld_m, the transposes of both; bfloat16, padding written as zeros.
+hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
+                                     uint16_t *d, size_t ld_n, uint16_t *dt, size_t ld_m, int k, const DeviceInfo &dev,
+                                     hipStream_t stream);
+// y[z] = a[z] b^T for bfloat16 operands whose rows are `k` values, padded with zeros to a multiple of 64 (`ld`
+// elements between rows, a multiple of 64).  a is `batch` (1 or 2) matrices of m rows back to back.
+hipError_t launch_bf16_gemm(const uint16_t *a, size_t ld_a, int m, const uint16_t *b, size_t ld_b, int n, int k, void *y0, void *y1,
+                            int batch, int out, const DeviceInfo &dev, hipStream_t stream);
+
+// Between the files of the C ABI (api.hip): the current device's record, set up for work on `stream`, and a
+// HIP error as the status of a call.  Both return an INT4LINEAR_* status.
+int api_begin(hipStream_t stream, DeviceInfo *info);
+int api_status(hipError_t e);
+
+}  // namespace int4linear
