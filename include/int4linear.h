@@ -195,7 +195,8 @@ int int4linear_linear_fp6_converted(const void *x_conv_d, const void *w_conv_d, 
  *   scales  one E8M0 byte s per 32 k: 2^(s - 127), 255 a NaN; a row takes 16 bytes per 512 k
  *           begun, zeros behind k.
  * int4linear_mxfp4_code_bytes and _scale_bytes are the arrays' sizes (0 for a negative size).
- * Any k >= 0 is accepted; sizes beyond 2^30 are refused with INT4LINEAR_ERR_UNSUPPORTED.
+ * Any k >= 0 is accepted.  Rows beyond 2^30, a product's k beyond 2^22 and a gradient's sizes beyond
+ * 2^22 - 64 are refused with INT4LINEAR_ERR_UNSUPPORTED.
  *
  * All calls are asynchronous on `stream`, allocate nothing, take no locks and do not touch the
  * library's workspace: they may be captured into a graph once the device is set up.  Types are

@@ -11,7 +11,9 @@ using namespace int4linear;
 
 // Row and column numbers are 32-bit in the kernels, rounded up to tiles; offsets are 64-bit.
 constexpr int kMostRows = 1 << 30;
-constexpr int kMostTransposed = 65535 * 64;  // the transposes' grid
+// A tile's loads are a base and 32 bits of offset over at most 256 rows, and the transposes have 65535 rows of
+// tiles of 64: k of a product, and every size of a gradient, which is some product's k.
+constexpr int kMostK = 1 << 22;
 
 bool aligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 bool is_type(int type) { return type == INT4LINEAR_OUT_F32 || type == INT4LINEAR_OUT_F16 || type == INT4LINEAR_OUT_BF16; }
@@ -145,7 +147,7 @@ int int4linear_mxfp4_linear(const void *x_codes_d, const void *x_scales_d, const
                             const float *bias_d, void *y_d, int out_type, int m, int n, int k, void *stream)
 {
     Checks ok;
-    ok.sizes(m, n, k).that(is_type(out_type), INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(m, n, k).that(k <= kMostK && is_type(out_type), INT4LINEAR_ERR_UNSUPPORTED);
     if (!ok || m == 0 || n == 0)
         return ok.status;
     ok.array(y_d, 16, true).optional(bias_d, 4).matrix(x_codes_d, x_scales_d, m, k).matrix(w_codes_d, w_scales_d, n, k);
@@ -164,7 +166,7 @@ int int4linear_mxfp4_gated(const void *x_codes_d, const void *x_scales_d, const 
                            int k, void *stream)
 {
     Checks ok;
-    ok.sizes(m, n, k).that(is_type(out_type) && is_activation(activation), INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(m, n, k).that(k <= kMostK && is_type(out_type) && is_activation(activation), INT4LINEAR_ERR_UNSUPPORTED);
     if (!ok || m == 0 || n == 0)
         return ok.status;
     ok.array(h_d, 16, true).matrix(x_codes_d, x_scales_d, m, k);
@@ -185,7 +187,7 @@ int int4linear_mxfp4_gated_quantized(const void *x_codes_d, const void *x_scales
                                      void *h_scales_d, int m, int n, int k, void *stream)
 {
     Checks ok;
-    ok.sizes(m, n, k).that(is_activation(activation), INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(m, n, k).that(k <= kMostK && is_activation(activation), INT4LINEAR_ERR_UNSUPPORTED);
     if (!ok || m == 0 || n == 0)
         return ok.status;
     ok.matrix(h_codes_d, h_scales_d, m, n).matrix(x_codes_d, x_scales_d, m, k);
@@ -211,7 +213,7 @@ int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, co
                                      size_t work_bytes, int m, int n, int k, void *stream_v)
 {
     Checks ok;
-    ok.sizes(m, n, k).that(n <= kMostTransposed && k <= kMostTransposed, INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(m, n, k).that(m <= kMostK - 64 && n <= kMostK - 64 && k <= kMostK - 64, INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(!dw_d || dw_type == INT4LINEAR_OUT_F32 || dw_type == INT4LINEAR_OUT_BF16, INT4LINEAR_ERR_UNSUPPORTED);
     const bool want_dx = dx_d && m > 0 && k > 0, want_dw = dw_d && n > 0 && k > 0, want_sums = dbias_d && n > 0;
     if (!ok || (!want_dx && !want_dw && !want_sums))
@@ -258,7 +260,7 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
                                     int k, void *stream_v)
 {
     Checks ok;
-    ok.sizes(m, n, k).that(n <= kMostTransposed && k <= kMostTransposed, INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(m, n, k).that(m <= kMostK - 64 && n <= kMostK - 64 && k <= kMostK - 64, INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(is_activation(activation), INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(!dwg_d || dw_type == INT4LINEAR_OUT_F32 || dw_type == INT4LINEAR_OUT_BF16, INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(!dwg_d == !dwu_d, INT4LINEAR_ERR_NULL);

@@ -8,8 +8,6 @@
 // alike, which is all that a sum over k asks for.  With 4-bit operands a chunk is one block of 32, and the
 // scales of the four chunks that a lane sees in a stage are the four bytes of one aligned dword.
 //
-// b's rows are the instruction's first operand: a lane then holds, for one row of a, four consecutive
-// columns of y in each group of eight, and stores are wide.
 #include "mxfp4.h"
 
 #include <type_traits>
@@ -40,70 +38,108 @@ struct LineRows {
 
 // ---- what happens to a tile's sums ------------------------------------------------------------
 // An epilogue is called once per wave as ep(acc, row, col, lane): acc[j][i] is the 32 x 32 block at rows
-// row + 32 j of a and columns col + 32 i of the product; element t of a lane is at row + 32 j + lane % 32
-// and column col + 32 i + 8 (t / 4) + 4 (lane / 32) + t % 4.  kPair: two operands b share the
-// tile, blocks i even of the first, odd of the second, each pair over the same 32 columns.
+// row + 32 j of a and columns col + 32 i of the product.  Which operand the matrix instruction takes first decides
+// what a lane holds of it:
+//   kColumns = false: row lane % 32; element t is column 8 (t / 4) + 4 (lane / 32) + t % 4;
+//   kColumns = true:  column lane % 32; element t is row 8 (t / 4) + 4 (lane / 32) + t % 4.
+// 16-bit outputs whose rows are multiples of 16 bytes take the first: two lanes swap halves and each stores 16
+// bytes.  All others take the second: a store covers 32 neighbouring elements of two rows, wherever they begin.
+// kPair: two operands b share the tile, blocks i even of the first, odd of the second, each pair over the same
+// 32 columns.
 
 template <int OUT>
-__device__ __forceinline__ void store4(void *y, size_t at, const float (&v)[4], int valid, bool vec)
+using OutElement = std::conditional_t<OUT == kOutF32, float, std::conditional_t<OUT == kOutF16, _Float16, __bf16>>;
+
+// A lane's 16 columns of a row (kColumns = false), rounded to 16 bits -> 8 columns from 8 * (lane / 32) on
+// in out[0], from 16 + 8 * (lane / 32) on in out[1].
+template <int OUT>
+__device__ __forceinline__ void gather_row(const float (&v)[16], v4i (&out)[2])
 {
-    if constexpr (OUT == kOutF32) {
-        float *dst = (float *)y + at;
-        if (vec && valid == 4) {
-            *(v4f *)dst = (v4f){v[0], v[1], v[2], v[3]};
-            return;
-        }
+    using T = OutElement<OUT>;
+    typedef T v2t __attribute__((ext_vector_type(2)));
+    int p[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (q < valid)
-                dst[q] = v[q];
+    for (int e = 0; e < 8; ++e)
+        p[e] = __builtin_bit_cast(int, (v2t){(T)v[2 * e], (T)v[2 * e + 1]});
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const auto x = __builtin_amdgcn_permlane32_swap(p[4 * half], p[4 * half + 2], false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(p[4 * half + 1], p[4 * half + 3], false, false);
+        out[half] = (v4i){(int)x[0], (int)y[0], (int)x[1], (int)y[1]};
+    }
+}
+
+// The 16 results v of a lane's part of a block of y (ld elements between rows) at (row, col).
+template <int OUT, bool COLUMNS>
+__device__ __forceinline__ void store_block(void *y, size_t ld, int m, int n, int row, int col, int lane, const float (&v)[16])
+{
+    using T = OutElement<OUT>;
+    T *dst = (T *)y;
+    if constexpr (COLUMNS) {
+        const int c = col + (lane & 31), r0 = row + 4 * (lane >> 5);
+        dst += (size_t)r0 * ld + c;
+        if (c < n) {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                const int dr = 8 * (t / 4) + t % 4;
+                if (r0 + dr < m)
+                    dst[(size_t)dr * ld] = (T)v[t];
+            }
+        }
     } else {
-        using T = std::conditional_t<OUT == kOutF16, _Float16, __bf16>;
-        typedef T v4t __attribute__((ext_vector_type(4)));
-        T *dst = (T *)y + at;
-        if (vec && valid == 4) {
-            *(v4t *)dst = (v4t){(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-            return;
+        v4i out[2];
+        gather_row<OUT>(v, out);
+        const int r = row + (lane & 31), c = col + 8 * (lane >> 5);
+        dst += (size_t)r * ld + c;
+        if (r < m) {  // (n is a multiple of 8)
+            if (c < n)
+                *(v4i *)dst = out[0];
+            if (c + 16 < n)
+                *(v4i *)(dst + 16) = out[1];
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (q < valid)
-                dst[q] = (T)v[q];
     }
 }
 
 // y = sums + bias, rounded once to OUT.
-template <int OUT>
+template <int OUT, bool COLUMNS>
 struct PlainEpilogue {
-    static constexpr bool kPair = false;
-    void *y[2];  // by blockIdx.z
+    static constexpr bool kPair = false, kColumns = COLUMNS;
+    void *y0, *y1;  // by blockIdx.z
     const float *bias;
     size_t ld;
     int m, n;
-    bool vec;  // four columns from a multiple of four on are aligned
 
     template <int FM, int FN>
-    __device__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
+    __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
-        void *dst = y[blockIdx.z];
+        void *dst = blockIdx.z ? y1 : y0;
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int r = row + kFrag * j + (lane & 31);
-            if (r >= m)
-                continue;
+        for (int i = 0; i < FN; ++i) {
+            const int c = col + kFrag * i;
+            float add[16];
 #pragma unroll
-            for (int i = 0; i < FN; ++i)
+            for (int t = 0; t < 16; ++t)
+                add[t] = 0.0f;
+            if (bias) {
+                if constexpr (COLUMNS) {
+                    const float b = bias[min(c + (lane & 31), n - 1)];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int c = col + kFrag * i + 8 * q + 4 * (lane >> 5);
-                    if (c >= n)
-                        continue;
-                    float v[4];
+                    for (int t = 0; t < 16; ++t)
+                        add[t] = b;
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        v[e] = acc[j][i][4 * q + e] + (bias ? bias[min(c + e, n - 1)] : 0.0f);
-                    store4<OUT>(dst, (size_t)r * ld + c, v, min(n - c, 4), vec);
+                    for (int t = 0; t < 16; ++t)
+                        add[t] = bias[min(c + 8 * (t / 4) + 4 * (lane >> 5) + t % 4, n - 1)];
                 }
+            }
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                float v[16];
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+                    v[t] = acc[j][i][t] + add[t];
+                store_block<OUT, COLUMNS>(dst, ld, m, n, row + kFrag * j, c, lane, v);
+            }
         }
     }
 };
@@ -116,67 +152,49 @@ __device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(
 
 __device__ __forceinline__ float activate(int act, float g)
 {
-    if (act == kSilu)
-        return g * logistic(g);
-    return g * logistic(kGeluScale * (g + kGeluCubic * g * g * g));
+    return g * logistic(act == kSilu ? g : kGeluScale * (g + kGeluCubic * g * g * g));
 }
 
 __device__ __forceinline__ void activate_with_slope(int act, float g, float &value, float &slope)
 {
-    if (act == kSilu) {
-        const float s = logistic(g);
-        value = g * s;
-        slope = s * (1.0f + g * (1.0f - s));
-    } else {
-        const float s = logistic(kGeluScale * (g + kGeluCubic * g * g * g));
-        value = g * s;
-        slope = s + g * s * (1.0f - s) * kGeluScale * (1.0f + 3.0f * kGeluCubic * g * g);
-    }
+    const float s = logistic(act == kSilu ? g : kGeluScale * (g + kGeluCubic * g * g * g));
+    value = g * s;
+    slope = s + g * s * (1.0f - s) * (act == kSilu ? 1.0f : kGeluScale * (1.0f + 3.0f * kGeluCubic * g * g));
 }
 
 // h = act(g) * u, rounded once to OUT.
-template <int OUT>
+template <int OUT, bool COLUMNS>
 struct GatedEpilogue {
-    static constexpr bool kPair = true;
+    static constexpr bool kPair = true, kColumns = COLUMNS;
     void *h;
     size_t ld;
     int m, n, act;
-    bool vec;
 
     template <int FM, int FN>
-    __device__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
+    __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int r = row + kFrag * j + (lane & 31);
-            if (r >= m)
-                continue;
+        for (int j = 0; j < FM; ++j)
 #pragma unroll
-            for (int i = 0; i < FN; i += 2)
+            for (int i = 0; i < FN; i += 2) {
+                float v[16];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int c = col + kFrag * (i / 2) + 8 * q + 4 * (lane >> 5);
-                    if (c >= n)
-                        continue;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        v[e] = activate(act, acc[j][i][4 * q + e]) * acc[j][i + 1][4 * q + e];
-                    store4<OUT>(h, (size_t)r * ld + c, v, min(n - c, 4), vec);
-                }
-        }
+                for (int t = 0; t < 16; ++t)
+                    v[t] = activate(act, acc[j][i][t]) * acc[j][i + 1][t];
+                store_block<OUT, COLUMNS>(h, ld, m, n, row + kFrag * j, col + kFrag * (i / 2), lane, v);
+            }
     }
 };
 
 // The same in MXFP4: a block of 32 columns of a row sits in lanes l and l + 32.
 struct GatedMxEpilogue {
-    static constexpr bool kPair = true;
+    static constexpr bool kPair = true, kColumns = false;
     uint8_t *codes, *scales;
     size_t code_stride, scale_stride;
     int m, n, act;
 
     template <int FM, int FN>
-    __device__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
+    __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
@@ -192,29 +210,37 @@ struct GatedMxEpilogue {
                     v[t] = c < n ? activate(act, acc[j][i][t]) * acc[j][i + 1][t] : 0.0f;
                     big = max(big, __builtin_bit_cast(unsigned, v[t]) & 0x7FFFFFFFu);
                 }
-                big = max(big, (unsigned)__shfl_xor((int)big, 32));
+                const auto both = __builtin_amdgcn_permlane32_swap(big, big, false, false);
+                big = max(both[0], both[1]);
                 const int field = (int)(big >> 23);
                 const int code = field == 255 ? 255 : max(field - 2, 0);
-                const float inverse = field == 255 ? 0.0f : __builtin_bit_cast(float, code == 254 ? 0x00400000 : (254 - code) << 23);
-                if (r >= m || (size_t)c0 >= code_stride * 2)
-                    continue;
-                unsigned short *dst = (unsigned short *)(codes + (size_t)r * code_stride + c0 / 2) + (lane >> 5);
+                const float inverse = __builtin_bit_cast(float, code >= 254 ? 0x00400000 : (254 - code) << 23);
+                unsigned bits[2];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float s[4];
+                for (int h = 0; h < 2; ++h) {
+                    float s[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[e] = field == 255 ? 0.0f : v[4 * q + e] * inverse;
-                    unsigned bits = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, s[0], s[1], 1.0f, 0);
-                    bits = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(bits, s[2], s[3], 1.0f, 1);
-                    dst[2 * q] = (unsigned short)bits;
+                    for (int e = 0; e < 8; ++e)
+                        s[e] = field == 255 ? 0.0f : v[8 * h + e] * inverse;
+                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, s[0], s[1], 1.0f, 0);
+                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(bits[h], s[2], s[3], 1.0f, 1);
+                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(bits[h], s[4], s[5], 1.0f, 2);
+                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(bits[h], s[6], s[7], 1.0f, 3);
                 }
-                if (lane < 32) {
-                    uint8_t *to = scales + (size_t)r * scale_stride + c0 / kMxBlock;
-                    *to = (uint8_t)code;
-                    // the row's last line of codes; its scales go on for one more where they are not 16 yet
-                    if ((size_t)c0 + kMxBlock == code_stride * 2 && code_stride % (2 * kLineBytes))
-                        *(unsigned long long *)(to + 1) = 0;
+                // bits[h]: 16 bits for columns 16 h + 4 (lane / 32) .., 16 for those 8 further on.  The lane pair's four words
+                // make dwords 2 h and 2 h + 1 of the block; the lower lane takes h = 0, the upper h = 1.
+                const auto x = __builtin_amdgcn_permlane32_swap(bits[0], bits[1], false, false);
+                const unsigned lo = (x[0] & 0xFFFFu) | (x[1] << 16), hi = (x[0] >> 16) | (x[1] & 0xFFFF0000u);
+                if (r < m && (size_t)c0 < code_stride * 2) {
+                    *(unsigned long long *)(codes + (size_t)r * code_stride + c0 / 2 + 8 * (lane >> 5)) =
+                        lo | ((unsigned long long)hi << 32);
+                    if (lane < 32) {
+                        uint8_t *to = scales + (size_t)r * scale_stride + c0 / kMxBlock;
+                        *to = (uint8_t)code;
+                        // the row's last line of codes; its scales go on for one more where they are not 16 yet
+                        if ((size_t)c0 + kMxBlock == code_stride * 2 && code_stride % (2 * kLineBytes))
+                            *(unsigned long long *)(to + 1) = 0;
+                    }
                 }
             }
         }
@@ -225,29 +251,32 @@ struct GatedMxEpilogue {
 // on matrix cores that take 16 bits; the roundings of the terms (2^-8 at most, of random sign) add up to as much as
 // the rounding of the result itself.
 struct GradientEpilogue {
-    static constexpr bool kPair = true;
+    static constexpr bool kPair = true, kColumns = false;
     const __bf16 *dh;
     __bf16 *d, *dt;
     size_t ld_n, ld_m;
     int m, n, act;
-    bool vec;
+    bool vec;  // dh's rows are multiples of 8 bytes
 
     template <int FM, int FN>
-    __device__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
+    __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
             const int r = row + kFrag * j + (lane & 31);
 #pragma unroll
-            for (int i = 0; i < FN; i += 2)
+            for (int i = 0; i < FN; i += 2) {
+                const int c0 = col + kFrag * (i / 2);
+                float dg[16], du[16];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int c = col + kFrag * (i / 2) + 8 * q + 4 * (lane >> 5);
+                    const int c = c0 + 8 * q + 4 * (lane >> 5);
                     v4bf in = {};
-                    if (r < m && c < n) {
+                    if (r < m) {
                         const __bf16 *src = dh + (size_t)r * n + c;
-                        if (vec && c + 4 <= n) {
-                            in = *(const v4bf *)src;
+                        if (vec) {
+                            if (c < n)
+                                in = *(const v4bf *)src;
                         } else {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
@@ -255,45 +284,51 @@ struct GradientEpilogue {
                                     in[e] = src[e];
                         }
                     }
-                    v4bf dg = {}, du = {};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if (r >= m || c + e >= n)
-                            continue;  // padding: exact zeros, whatever the clamped rows gave
+                        const int t = 4 * q + e;
                         float value, slope;
-                        activate_with_slope(act, acc[j][i][4 * q + e], value, slope);
-                        const float up = acc[j][i + 1][4 * q + e], g = (float)in[e];
-                        dg[e] = (__bf16)(g * up * slope);
-                        du[e] = (__bf16)(g * value);
-                    }
-                    if (r < m && (size_t)c < ld_n) {
-                        *(v4bf *)(d + (size_t)r * 2 * ld_n + c) = dg;
-                        *(v4bf *)(d + (size_t)r * 2 * ld_n + ld_n + c) = du;
-                    }
-                    if ((size_t)r < ld_m) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (c + e < n) {
-                                dt[(size_t)(c + e) * ld_m + r] = dg[e];
-                                dt[((size_t)n + c + e) * ld_m + r] = du[e];
-                            }
+                        activate_with_slope(act, acc[j][i][t], value, slope);
+                        // padding: exact zeros, whatever the clamped rows gave
+                        const bool there = r < m && c + e < n;
+                        const float g = (float)in[e];
+                        dg[t] = there ? g * acc[j][i + 1][t] * slope : 0.0f;
+                        du[t] = there ? g * value : 0.0f;
                     }
                 }
+                store_block<kOutBF16, false>(d, 2 * ld_n, m, (int)ld_n, row + kFrag * j, c0, lane, dg);
+                store_block<kOutBF16, false>(d + ld_n, 2 * ld_n, m, (int)ld_n, row + kFrag * j, c0, lane, du);
+                // the transposes: 32 neighbouring rows a store
+                if ((size_t)r < ld_m) {
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) {
+                        const int c = c0 + 8 * (t / 4) + 4 * (lane >> 5) + t % 4;
+                        if (c < n) {
+                            dt[(size_t)c * ld_m + r] = (__bf16)dg[t];
+                            dt[((size_t)n + c) * ld_m + r] = (__bf16)du[t];
+                        }
+                    }
+                }
+            }
         }
     }
 };
 
 // ---- the kernel -------------------------------------------------------------------------------
 
-template <int WAVES_M_, int WAVES_N_, int FM_, int FN_>
+// WAVES_M x WAVES_N wavefronts, each FM x FN blocks of 32 x 32; OCC waves per SIMD.
+template <int WAVES_M_, int WAVES_N_, int FM_, int FN_, int OCC_>
 struct LineTile {
-    static constexpr int WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, FM = FM_, FN = FN_;
+    static constexpr int WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, FM = FM_, FN = FN_, OCC = OCC_;
     static constexpr int NWAVES = WAVES_M * WAVES_N, THREADS = NWAVES * 64;
     static constexpr int BM = WAVES_M * FM * kFrag, BN = WAVES_N * FN * kFrag;
     static constexpr int STAGE = (BM + BN) * kLineBytes;
-    static constexpr int LDS = 2 * STAGE;
-    static constexpr int CHUNKS = STAGE / 1024 / NWAVES;  // 1-KiB loads per wave and stage
-    static_assert(STAGE % (1024 * NWAVES) == 0);
+    static constexpr int SCALES = (BM + BN) * 16;       // scales of two stages
+    static constexpr int LDS = 2 * STAGE + 2 * SCALES;  // two of each
+    static constexpr int CHUNK_ROWS = 8;                // rows of a 1-KiB load
+    static constexpr int A_CH = BM / CHUNK_ROWS / NWAVES, B_CH = BN / CHUNK_ROWS / NWAVES;  // loads per wave and stage
+    static constexpr int SLOTS = FM * FN;               // matrix instructions per step
+    static_assert(BM % (CHUNK_ROWS * NWAVES) == 0 && BN % (CHUNK_ROWS * NWAVES) == 0 && BM % 64 == 0 && BN % 64 == 0);
 };
 
 // Order of tiles: workgroup ids go round-robin over the 8 XCDs; ids congruent mod 8 get consecutive
@@ -315,210 +350,423 @@ __device__ __forceinline__ void tile_coords(int v, int total, int tiles_m, int t
 }
 
 #define I4L_LDS(p) ((__attribute__((address_space(3))) void *)(p))
-#define I4L_GLOBAL(p) ((const __attribute__((address_space(1))) void *)(p))
 
+// 16 bytes per lane from base + offset straight into LDS at to + 16 * lane.
+__device__ __forceinline__ void dma16(const void *base, unsigned offset, unsigned to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory");
+}
+__device__ __forceinline__ void dma16(const void *lane_address, unsigned to)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(lane_address), "s"(to) : "memory");
+}
+
+// Marks a value as used at this point of the program without generating code.
+__device__ __forceinline__ void pin(const v16f &v) { asm volatile("" ::"v"(v)); }
+
+// Sums without a single term: y = bias.
+template <int OUT>
+__global__ __launch_bounds__(256) void fill_rows_kernel(void *y, const float *bias, size_t count, size_t n)
+{
+    for (size_t at = (size_t)blockIdx.x * 256 + threadIdx.x; at < count; at += (size_t)gridDim.x * 256) {
+        ((OutElement<OUT> *)y)[at] = (OutElement<OUT>)(bias ? bias[at % n] : 0.0f);
+    }
+}
+
+template <int OUT>
+hipError_t fill_rows(void *y, const float *bias, size_t m, size_t n, hipStream_t stream)
+{
+    const size_t groups = (m * n + 255) / 256;
+    fill_rows_kernel<OUT><<<(unsigned)(groups < 4096 ? groups : 4096), 256, 0, stream>>>(y, bias, m * n, n);
+    return hipGetLastError();
+}
+
+// Persistent: a workgroup walks tiles blockIdx.x, + gridDim.x, ... and its loads run ahead of the
+// arithmetic across the ends of tiles.  Two stages of lines ring in LDS.  A stage is four steps of FM x FN
+// matrix instructions; while a step's instructions run, the next step's operands are read from LDS into the other
+// register set.  Before a stage's last step every read of the stage has been made: there the waves meet, the
+// next stage must have landed, and the stage's buffer is given to the loads of the one after that.
 template <bool FP4, class C, class Ep>
-__global__ __launch_bounds__(C::THREADS) void line_gemm_kernel(LineRows a, LineRows b0, LineRows b1, size_t a_batch, int stages,
-                                                               int tiles_m, int tiles_n, Ep ep)
+__global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows a, LineRows b0, LineRows b1, size_t a_batch, int stages,
+                                                                       int tiles_m, int tiles_n, Ep ep)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / C::WAVES_N, wn = wave % C::WAVES_N;
-    int tm, tn;
-    tile_coords(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
-    const int m0 = tm * C::BM;
-    const int n0 = tn * (Ep::kPair ? C::BN / 2 : C::BN);  // column of y
-
-    // Row of an LDS row of b's part of the tile, and its matrix.
-    auto b_row = [&](int r, bool &second) {
-        second = Ep::kPair && ((r / kFrag) & 1);
-        const int c = n0 + (Ep::kPair ? r / (2 * kFrag) * kFrag + r % kFrag : r);
-        return min(c, b0.rows - 1);
-    };
-
-    // Load c of a wave fills LDS rows 8 (c * NWAVES + wave) .. + 7 of a stage, lane l the 16 bytes at place l.
-    // The chunk that lies at place p of row r is p ^ (r / 2 % 8): the 16 lanes that an LDS read serves together
-    // then touch every bank once.
-    const uint8_t *src[C::CHUNKS];
-#pragma unroll
-    for (int c = 0; c < C::CHUNKS; ++c) {
-        const int r = (c * C::NWAVES + wave) * 8 + (lane >> 3);
-        const int chunk = (lane & 7) ^ ((r >> 1) & 7);
-        bool second = false;
-        if (r < C::BM) {
-            src[c] = a.data + blockIdx.z * a_batch + (size_t)min(m0 + r, a.rows - 1) * a.stride + chunk * 16;
-        } else {
-            const int br = b_row(r - C::BM, second);
-            src[c] = (second ? b1.data : b0.data) + (size_t)br * b0.stride + chunk * 16;
-        }
-    }
-    auto load_stage = [&](int s) {
-#pragma unroll
-        for (int c = 0; c < C::CHUNKS; ++c) {
-            uint8_t *dst = lds + (s & 1) * C::STAGE + (c * C::NWAVES + wave) * 1024;
-            __builtin_amdgcn_global_load_lds(I4L_GLOBAL(src[c] + (size_t)s * kLineBytes), I4L_LDS(dst), 16, 0, 0);
-        }
-    };
-
-    // Scales: this lane's row of every fragment, the dword of its lane group.
-    const uint8_t *a_scale[C::FM], *b_scale[C::FN];
-    if constexpr (FP4) {
-#pragma unroll
-        for (int j = 0; j < C::FM; ++j)
-            a_scale[j] = a.scales + (size_t)min(m0 + (wm * C::FM + j) * kFrag + (lane & 31), a.rows - 1) * a.scale_stride + 4 * (lane >> 5);
-#pragma unroll
-        for (int i = 0; i < C::FN; ++i) {
-            bool second;
-            const int r = b_row((wn * C::FN + i) * kFrag + (lane & 31), second);
-            b_scale[i] = (second ? b1.scales : b0.scales) + (size_t)r * b0.scale_stride + 4 * (lane >> 5);
-        }
-    }
+    const int total = tiles_m * tiles_n;
+    const int my_tiles = (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    const uint8_t *a_data = a.data + blockIdx.z * a_batch;
+    constexpr int kTileN = Ep::kPair ? C::BN / 2 : C::BN;  // columns of y
 
     v16f acc[C::FM][C::FN];
+    auto clear = [&] {
 #pragma unroll
-    for (int j = 0; j < C::FM; ++j)
+        for (int j = 0; j < C::FM; ++j)
 #pragma unroll
-        for (int i = 0; i < C::FN; ++i)
-            acc[j][i] = (v16f)0.0f;
+            for (int i = 0; i < C::FN; ++i)
+                acc[j][i] = (v16f)0.0f;
+    };
+    auto finish = [&](int it) {
+        int tm, tn;
+        tile_coords(blockIdx.x + it * gridDim.x, total, tiles_m, tiles_n, tm, tn);
+        ep(acc, tm * C::BM + wm * C::FM * kFrag, tn * kTileN + wn * C::FN * kFrag / (Ep::kPair ? 2 : 1), lane);
+        clear();
+    };
+    clear();
 
-    const int swz = ((lane & 31) >> 1) & 7;
-    const uint8_t *a_rd = lds + (wm * C::FM * kFrag + (lane & 31)) * kLineBytes;
-    const uint8_t *b_rd = lds + (C::BM + wn * C::FN * kFrag + (lane & 31)) * kLineBytes;
+    // ---- loads.  Load c of a wave fills LDS rows 8 (c * NWAVES + wave) .. + 7 of its operand's part of a
+    // stage, lane l the 16 bytes at place l % 8 of row l / 8.  The chunk that lies at place p of row r is
+    // p ^ (r / 2 % 8): the 16 lanes that an LDS read serves together then touch every bank once.
+    const unsigned lds_base = (unsigned)(size_t)I4L_LDS(lds);
+    const int ld_row = wave * C::CHUNK_ROWS + (lane >> 3);
+    const unsigned ld_chunk = (unsigned)(((lane & 7) ^ ((ld_row >> 1) & 7)) * 16);
+    static_assert(C::NWAVES * C::CHUNK_ROWS % 16 == 0 || C::A_CH + C::B_CH == 2, "the same swizzle for all loads of a lane");
+    const uint8_t *a_base = nullptr, *b_base[2] = {};  // this tile's rows, this stage's line
+    unsigned a_off[C::A_CH], b_off[C::B_CH];
+    const uint8_t *scale_at = nullptr;  // FP4: this lane's row of scales (wave w moves those of LDS rows 64 w ..)
+    constexpr bool kScaleWavesAll = (C::BM + C::BN) / 64 >= C::NWAVES;
+    static_assert((C::BM + C::BN) / 64 <= C::NWAVES);
+    int ld_it = 0, ld_s = 0;
+    unsigned ld_buffer = 0, ld_slot = 0;
 
-    if (stages > 0)
-        load_stage(0);
-    for (int s = 0; s < stages; ++s) {
-        int sa[C::FM], sb[C::FN];
+    // Matrix and row (of the tile) of LDS row r of b's part.
+    auto b_row = [](int r) { return Ep::kPair ? r / (2 * kFrag) * kFrag + r % kFrag : r; };
+    auto b_second = [](int r) { return Ep::kPair && (r / kFrag) % 2 != 0; };
+
+    auto ld_tile = [&](int it) {
+        int tm, tn;
+        tile_coords(blockIdx.x + it * gridDim.x, total, tiles_m, tiles_n, tm, tn);
+        const int m0 = tm * C::BM, n0 = tn * kTileN;
+        a_base = a_data + (size_t)m0 * a.stride;
+        // rows behind the matrix: the last one again
+        const int last_a = a.rows - 1 - m0, last_b = b0.rows - 1 - n0;
+#pragma unroll
+        for (int c = 0; c < C::A_CH; ++c)
+            a_off[c] = (unsigned)min(c * C::NWAVES * C::CHUNK_ROWS + ld_row, last_a) * (unsigned)a.stride + ld_chunk;
+        // (last_b is negative where h's padding alone is in the tile: then the matrix's last row)
+        const int nb = min(n0, b0.rows - 1);
+        b_base[0] = b0.data + (size_t)nb * b0.stride;
+        b_base[1] = b1.data + (size_t)nb * b0.stride;
+#pragma unroll
+        for (int c = 0; c < C::B_CH; ++c)
+            b_off[c] = (unsigned)max(min(b_row(c * C::NWAVES * C::CHUNK_ROWS + ld_row), last_b), 0) * (unsigned)b0.stride + ld_chunk;
+        if constexpr (FP4) {
+            const int r = wave * 64 + lane;
+            if (r < C::BM) {
+                scale_at = a.scales + (size_t)(m0 + min(r, last_a)) * a.scale_stride;
+            } else {
+                const int br = r - C::BM;
+                scale_at = (b_second(br) ? b1.scales : b0.scales) + (size_t)(nb + max(min(b_row(br), last_b), 0)) * b0.scale_stride;
+            }
+        }
+    };
+    constexpr int kLoads = C::A_CH + C::B_CH;
+    auto load = [&](int c) {
+        const unsigned to = lds_base + ld_buffer + (unsigned)wave * 1024u;
+        if (c < C::A_CH)
+            dma16(a_base, a_off[c], to + (unsigned)(c * C::NWAVES) * 1024u);
+        else
+            dma16(b_base[b_second(((c - C::A_CH) * C::NWAVES + wave) * C::CHUNK_ROWS)], b_off[c - C::A_CH], to + (unsigned)(C::BM * kLineBytes) + (unsigned)((c - C::A_CH) * C::NWAVES) * 1024u);
+    };
+    // After a stage's loads: its scales, if they are not there already, and on to the next stage.  Behind the
+    // last stage the cursor stays: it is loaded again, into a buffer that nobody reads.
+    auto load_rest = [&] {
+        if constexpr (FP4) {
+            if ((ld_s & 1) == 0 && (kScaleWavesAll || wave < (C::BM + C::BN) / 64))
+                dma16(scale_at, lds_base + 2 * C::STAGE + ld_slot + (unsigned)wave * 1024u);
+        }
+        ld_buffer ^= (unsigned)C::STAGE;
+        if (ld_s + 1 < stages) {
+            ++ld_s;
+            a_base += kLineBytes;
+            b_base[0] += kLineBytes;
+            b_base[1] += kLineBytes;
+            if ((ld_s & 1) == 0) {
+                scale_at += 16;
+                ld_slot ^= (unsigned)C::SCALES;
+            }
+        } else if (ld_it + 1 < my_tiles) {
+            ld_s = 0;
+            ld_slot ^= (unsigned)C::SCALES;
+            ld_tile(++ld_it);
+        }
+    };
+    static_assert((C::STAGE & (C::STAGE - 1)) == 0 && (C::SCALES & (C::SCALES - 1)) == 0);
+
+    ld_tile(0);
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c)
+        load(c);
+    load_rest();
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c)
+        load(c);
+    load_rest();
+
+    // ---- arithmetic
+    const int fr = lane & 31, fg = lane >> 5;
+    unsigned chunk_at[4];
+#pragma unroll
+    for (int J = 0; J < 4; ++J)
+        chunk_at[J] = (unsigned)(((4 * fg + J) ^ ((fr >> 1) & 7)) * 16 + fr * kLineBytes);
+    const unsigned a_rd = (unsigned)(wm * C::FM * kFrag * kLineBytes);
+    const unsigned b_rd = (unsigned)((C::BM + wn * C::FN * kFrag) * kLineBytes);
+    const unsigned as_rd = (unsigned)(2 * C::STAGE + (wm * C::FM * kFrag + fr) * 16 + 4 * fg);
+    const unsigned bs_rd = (unsigned)(2 * C::STAGE + (C::BM + wn * C::FN * kFrag + fr) * 16 + 4 * fg);
+    v4i fa[2][C::FM], fb[2][C::FN];
+    int sa[2][C::FM] = {}, sb[2][C::FN] = {};
+
+    // Operand r of step J of the stage in `buffer`, into register set p.
+    constexpr int kReads = C::FM + C::FN;
+    auto read = [&](unsigned buffer, int J, int p, int r) {
+        const uint8_t *at = lds + (buffer + chunk_at[J]);
+        if (r < C::FM)
+            fa[p][r] = *(const v4i *)(at + a_rd + r * kFrag * kLineBytes);
+        else
+            fb[p][r - C::FM] = *(const v4i *)(at + b_rd + (r - C::FM) * kFrag * kLineBytes);
+    };
+    auto read_scales = [&](unsigned slot, int s, int p) {
+        if constexpr (FP4) {
+            const uint8_t *at = lds + (slot + 8 * (s & 1));
+#pragma unroll
+            for (int j = 0; j < C::FM; ++j)
+                sa[p][j] = *(const int *)(at + as_rd + j * kFrag * 16);
+#pragma unroll
+            for (int i = 0; i < C::FN; ++i)
+                sb[p][i] = *(const int *)(at + bs_rd + i * kFrag * 16);
+        }
+    };
+    // The matrix instructions of step J, `behind` called after each with its number.
+    auto step = [&](auto j_tag, auto &&behind) {
+        constexpr int J = decltype(j_tag)::value, p = J & 1;
+        [&]<int... SLOT>(std::integer_sequence<int, SLOT...>) {
+            ([&] {
+                constexpr int j = SLOT / C::FN, i = SLOT % C::FN;
+                if constexpr (FP4) {
+                    const v8i wide_a = {fa[p][j][0], fa[p][j][1], fa[p][j][2], fa[p][j][3], 0, 0, 0, 0};
+                    const v8i wide_b = {fb[p][i][0], fb[p][i][1], fb[p][i][2], fb[p][i][3], 0, 0, 0, 0};
+                    if constexpr (Ep::kColumns)
+                        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_a, wide_b, acc[j][i], 4, 4, J, sa[0][j], J, sb[0][i]);
+                    else
+                        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_b, wide_a, acc[j][i], 4, 4, J, sb[0][i], J, sa[0][j]);
+                } else {
+                    const v8bf wide_a = __builtin_bit_cast(v8bf, fa[p][j]), wide_b = __builtin_bit_cast(v8bf, fb[p][i]);
+                    if constexpr (Ep::kColumns)
+                        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wide_a, wide_b, acc[j][i], 0, 0, 0);
+                    else
+                        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wide_b, wide_a, acc[j][i], 0, 0, 0);
+                }
+                pin(acc[j][i]);
+                __builtin_amdgcn_sched_barrier(0);
+                behind(std::integral_constant<int, SLOT>{});
+                __builtin_amdgcn_sched_barrier(0);
+            }(), ...);
+        }(std::make_integer_sequence<int, C::SLOTS>{});
+    };
+    constexpr int kReadsPerSlot = (kReads + C::SLOTS - 1) / C::SLOTS;
+    constexpr int kLoadsPerSlot = (kLoads + C::SLOTS - 1) / C::SLOTS;
+
+    // Lines have landed and every wave is here.
+    auto meet = [&] {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    meet();
+#pragma unroll
+    for (int r = 0; r < kReads; ++r)
+        read(0, 0, 0, r);
+    read_scales(0, 0, 0);
+
+    unsigned buffer = 0, slot = 0;
+    int it = 0, s = 0;
+    while (true) {
+        [&]<int... J>(std::integer_sequence<int, J...>) {
+            (step(std::integral_constant<int, J>{},
+                  [&](auto slot_tag) {
+                      constexpr int at = decltype(slot_tag)::value * kReadsPerSlot;
+#pragma unroll
+                      for (int r = at; r < at + kReadsPerSlot && r < kReads; ++r)
+                          read(buffer, J + 1, (J + 1) & 1, r);
+                  }),
+             ...);
+        }(std::make_integer_sequence<int, 3>{});
+        meet();
+        const bool last = s + 1 == stages;
+        const int next_s = last ? 0 : s + 1;
+        if ((next_s & 1) == 0)
+            slot ^= (unsigned)C::SCALES;
+        read_scales(slot, next_s, 1);
+        step(std::integral_constant<int, 3>{}, [&](auto slot_tag) {
+            constexpr int at = decltype(slot_tag)::value * kReadsPerSlot, load_at = decltype(slot_tag)::value * kLoadsPerSlot;
+#pragma unroll
+            for (int r = at; r < at + kReadsPerSlot && r < kReads; ++r)
+                read(buffer ^ (unsigned)C::STAGE, 0, 0, r);
+#pragma unroll
+            for (int c = load_at; c < load_at + kLoadsPerSlot && c < kLoads; ++c)
+                load(c);
+        });
+        load_rest();
         if constexpr (FP4) {
 #pragma unroll
             for (int j = 0; j < C::FM; ++j)
-                sa[j] = *(const int *)(a_scale[j] + 8 * (size_t)s);
+                sa[0][j] = sa[1][j];
 #pragma unroll
             for (int i = 0; i < C::FN; ++i)
-                sb[i] = *(const int *)(b_scale[i] + 8 * (size_t)s);
+                sb[0][i] = sb[1][i];
         }
-        __syncthreads();  // stage s has landed (the barrier waits for loads), stage s - 1 has been read
-        if (s + 1 < stages)
-            load_stage(s + 1);
-        const int buffer = (s & 1) * C::STAGE;
-        [&]<int... J>(std::integer_sequence<int, J...>) {
-            ([&] {
-                const int at = buffer + ((4 * (lane >> 5) + J) ^ swz) * 16;
-                v4i fa[C::FM], fb[C::FN];
-#pragma unroll
-                for (int j = 0; j < C::FM; ++j)
-                    fa[j] = *(const v4i *)(a_rd + at + j * kFrag * kLineBytes);
-#pragma unroll
-                for (int i = 0; i < C::FN; ++i)
-                    fb[i] = *(const v4i *)(b_rd + at + i * kFrag * kLineBytes);
-#pragma unroll
-                for (int j = 0; j < C::FM; ++j)
-#pragma unroll
-                    for (int i = 0; i < C::FN; ++i) {
-                        if constexpr (FP4) {
-                            const v8i wide_a = {fa[j][0], fa[j][1], fa[j][2], fa[j][3], 0, 0, 0, 0};
-                            const v8i wide_b = {fb[i][0], fb[i][1], fb[i][2], fb[i][3], 0, 0, 0, 0};
-                            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_b, wide_a, acc[j][i], 4, 4, J, sb[i], J, sa[j]);
-                        } else {
-                            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, fb[i]),
-                                                                               __builtin_bit_cast(v8bf, fa[j]), acc[j][i], 0, 0, 0);
-                        }
-                    }
-            }(), ...);
-        }(std::make_integer_sequence<int, 4>{});
+        buffer ^= (unsigned)C::STAGE;
+        s = next_s;
+        if (last) {
+            finish(it);
+            if (++it == my_tiles)
+                break;
+        }
     }
-    ep(acc, m0 + wm * C::FM * kFrag, n0 + wn * C::FN * kFrag / (Ep::kPair ? 2 : 1), lane);
+    // (loads into buffers that nobody reads may be in flight: they end before the workgroup's LDS is given away)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-using Tile128 = LineTile<2, 2, 2, 2>;
+using Tile128 = LineTile<2, 2, 2, 2, 2>;
+using Tile256 = LineTile<4, 2, 2, 4, 2>;
 
 template <bool FP4, class C, class Ep>
-hipError_t launch(const LineRows &a, const LineRows &b0, const LineRows &b1, size_t a_batch, int batch, int stages, int n, const Ep &ep,
-                  hipStream_t stream)
+hipError_t launch_tile(const LineRows &a, const LineRows &b0, const LineRows &b1, size_t a_batch, int batch, int stages, int n, const Ep &ep,
+                       const DeviceInfo &dev, hipStream_t stream)
 {
     const int bn = Ep::kPair ? C::BN / 2 : C::BN;
     const int tiles_m = (a.rows + C::BM - 1) / C::BM, tiles_n = (n + bn - 1) / bn;
-    line_gemm_kernel<FP4, C, Ep><<<dim3((unsigned)(tiles_m * tiles_n), 1, (unsigned)batch), C::THREADS, C::LDS, stream>>>(
-        a, b0, b1, a_batch, stages, tiles_m, tiles_n, ep);
+    const int per_cu = C::NWAVES >= 8 ? 1 : 2;
+    const int groups = min(tiles_m * tiles_n, max(1, dev.cu_count * per_cu / batch));
+    line_gemm_kernel<FP4, C, Ep><<<dim3((unsigned)groups, 1, (unsigned)batch), C::THREADS, C::LDS, stream>>>(a, b0, b1, a_batch, stages, tiles_m, tiles_n, ep);
     return hipGetLastError();
+}
+
+template <bool FP4, class Ep>
+hipError_t launch(const LineRows &a, const LineRows &b0, const LineRows &b1, size_t a_batch, int batch, int stages, int n, const Ep &ep,
+                  const DeviceInfo &dev, hipStream_t stream)
+{
+    const long tiles256 = (long)((a.rows + 255) / 256) * ((n + (Ep::kPair ? 127 : 255)) / (Ep::kPair ? 128 : 256)) * batch;
+    if (tiles256 >= 128)
+        return launch_tile<FP4, Tile256>(a, b0, b1, a_batch, batch, stages, n, ep, dev, stream);
+    return launch_tile<FP4, Tile128>(a, b0, b1, a_batch, batch, stages, n, ep, dev, stream);
 }
 
 LineRows rows_of(const MxMatrix &q, int k) { return {q.codes, q.scales, mx_code_stride(k), mx_scale_stride(k), q.rows}; }
 
-bool aligned(const void *p, size_t ld, int out)
-{
-    const size_t bytes = out == kOutF32 ? 16 : 8;
-    return (uintptr_t)p % bytes == 0 && ld % 4 == 0;
-}
-
-// f(std::integral_constant<int, out>) for the output type of a call.
+// f(type, columns) with the output type of a call and the epilogue's form for rows of n elements.
 template <class F>
-hipError_t by_type(int out, F &&f)
+hipError_t by_type(int out, int n, F &&f)
 {
-    switch (out) {
-    case kOutF32:
-        return f(std::integral_constant<int, kOutF32>{});
-    case kOutF16:
-        return f(std::integral_constant<int, kOutF16>{});
-    default:
-        return f(std::integral_constant<int, kOutBF16>{});
-    }
+    if (out == kOutF32)
+        return f(std::integral_constant<int, kOutF32>{}, std::true_type{});
+    if (out == kOutF16)
+        return n % 8 ? f(std::integral_constant<int, kOutF16>{}, std::true_type{}) : f(std::integral_constant<int, kOutF16>{}, std::false_type{});
+    return n % 8 ? f(std::integral_constant<int, kOutBF16>{}, std::true_type{}) : f(std::integral_constant<int, kOutBF16>{}, std::false_type{});
 }
 
 }  // namespace
 
-hipError_t line_gemm_init(const DeviceInfo &) { return hipSuccess; }
+// Lets the kernels of an epilogue have their LDS.
+template <bool FP4, class Ep>
+static hipError_t allow_lds()
+{
+    hipError_t e = hipSuccess;
+    auto allow = [&](auto tile) {
+        using C = decltype(tile);
+        if (e == hipSuccess)
+            e = hipFuncSetAttribute((const void *)line_gemm_kernel<FP4, C, Ep>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+    };
+    allow(Tile128{});
+    allow(Tile256{});
+    return e;
+}
 
-hipError_t launch_mx_linear(const MxMatrix &x, const MxMatrix &w, const float *bias, void *y, int out, int k, const DeviceInfo &,
+hipError_t line_gemm_init(const DeviceInfo &)
+{
+    hipError_t e = hipSuccess;
+    for (auto allow : {allow_lds<true, PlainEpilogue<kOutF32, true>>, allow_lds<true, PlainEpilogue<kOutF16, true>>,
+                       allow_lds<true, PlainEpilogue<kOutF16, false>>, allow_lds<true, PlainEpilogue<kOutBF16, true>>,
+                       allow_lds<true, PlainEpilogue<kOutBF16, false>>, allow_lds<true, GatedEpilogue<kOutF32, true>>,
+                       allow_lds<true, GatedEpilogue<kOutF16, true>>, allow_lds<true, GatedEpilogue<kOutF16, false>>,
+                       allow_lds<true, GatedEpilogue<kOutBF16, true>>, allow_lds<true, GatedEpilogue<kOutBF16, false>>,
+                       allow_lds<true, GatedMxEpilogue>, allow_lds<true, GradientEpilogue>,
+                       allow_lds<false, PlainEpilogue<kOutF32, true>>, allow_lds<false, PlainEpilogue<kOutBF16, true>>,
+                       allow_lds<false, PlainEpilogue<kOutBF16, false>>})
+        if (e == hipSuccess)
+            e = allow();
+    return e;
+}
+
+hipError_t launch_mx_linear(const MxMatrix &x, const MxMatrix &w, const float *bias, void *y, int out, int k, const DeviceInfo &dev,
                             hipStream_t stream)
 {
     const int stages = (k + kLineFp4 - 1) / kLineFp4;
-    return by_type(out, [&](auto type) {
-        const PlainEpilogue<decltype(type)::value> ep{{y, nullptr}, bias, (size_t)w.rows, x.rows, w.rows, aligned(y, w.rows, out)};
-        return launch<true, Tile128>(rows_of(x, k), rows_of(w, k), rows_of(w, k), 0, 1, stages, w.rows, ep, stream);
+    return by_type(out, w.rows, [&](auto type, auto columns) {
+        constexpr int OUT = decltype(type)::value;
+        if (stages == 0)
+            return fill_rows<OUT>(y, bias, (size_t)x.rows, (size_t)w.rows, stream);
+        const PlainEpilogue<OUT, decltype(columns)::value> ep{y, nullptr, bias, (size_t)w.rows, x.rows, w.rows};
+        return launch<true>(rows_of(x, k), rows_of(w, k), rows_of(w, k), 0, 1, stages, w.rows, ep, dev, stream);
     });
 }
 
 hipError_t launch_mx_gated(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, void *h, int out, int k,
-                           const DeviceInfo &, hipStream_t stream)
+                           const DeviceInfo &dev, hipStream_t stream)
 {
     const int stages = (k + kLineFp4 - 1) / kLineFp4;
-    return by_type(out, [&](auto type) {
-        const GatedEpilogue<decltype(type)::value> ep{h, (size_t)wg.rows, x.rows, wg.rows, act, aligned(h, wg.rows, out)};
-        return launch<true, Tile128>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, wg.rows, ep, stream);
+    return by_type(out, wg.rows, [&](auto type, auto columns) {
+        constexpr int OUT = decltype(type)::value;
+        if (stages == 0)
+            return fill_rows<OUT>(h, nullptr, (size_t)x.rows, (size_t)wg.rows, stream);
+        const GatedEpilogue<OUT, decltype(columns)::value> ep{h, (size_t)wg.rows, x.rows, wg.rows, act};
+        return launch<true>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, wg.rows, ep, dev, stream);
     });
 }
 
 hipError_t launch_mx_gated_quantized(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, uint8_t *codes,
-                                     uint8_t *scales, int k, const DeviceInfo &, hipStream_t stream)
+                                     uint8_t *scales, int k, const DeviceInfo &dev, hipStream_t stream)
 {
     const int stages = (k + kLineFp4 - 1) / kLineFp4;
     const int n = wg.rows;
+    if (stages == 0) {
+        hipError_t e = fill_rows<kOutF32>(codes, nullptr, (size_t)x.rows, mx_code_stride(n) / 4, stream);
+        return e == hipSuccess ? fill_rows<kOutF32>(scales, nullptr, (size_t)x.rows, mx_scale_stride(n) / 4, stream) : e;
+    }
     const GatedMxEpilogue ep{codes, scales, mx_code_stride(n), mx_scale_stride(n), x.rows, n, act};
     // (the grid covers the padding at the end of h's rows)
-    return launch<true, Tile128>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, (int)(mx_code_stride(n) * 2), ep, stream);
+    return launch<true>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, (int)(mx_code_stride(n) * 2), ep, dev, stream);
 }
 
 hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
-                                     uint16_t *d, size_t ld_n, uint16_t *dt, size_t ld_m, int k, const DeviceInfo &,
+                                     uint16_t *d, size_t ld_n, uint16_t *dt, size_t ld_m, int k, const DeviceInfo &dev,
                                      hipStream_t stream)
 {
     const int stages = (k + kLineFp4 - 1) / kLineFp4;
-    const GradientEpilogue ep{(const __bf16 *)dh, (__bf16 *)d, (__bf16 *)dt, ld_n, ld_m, x.rows, wg.rows, act,
-                              aligned(dh, wg.rows, kOutBF16)};
-    return launch<true, Tile128>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, wg.rows, ep, stream);
+    const GradientEpilogue ep{(const __bf16 *)dh, (__bf16 *)d, (__bf16 *)dt, ld_n, ld_m, x.rows, wg.rows, act, wg.rows % 4 == 0};
+    return launch<true>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, wg.rows, ep, dev, stream);
 }
 
 hipError_t launch_bf16_gemm(const uint16_t *a, size_t ld_a, int m, const uint16_t *b, size_t ld_b, int n, int k, void *y0, void *y1,
-                            int batch, int out, const DeviceInfo &, hipStream_t stream)
+                            int batch, int out, const DeviceInfo &dev, hipStream_t stream)
 {
     const int stages = (k + kLineBf16 - 1) / kLineBf16;
     const LineRows ra{(const uint8_t *)a, nullptr, ld_a * 2, 0, m}, rb{(const uint8_t *)b, nullptr, ld_b * 2, 0, n};
-    return by_type(out, [&](auto type) {
-        const PlainEpilogue<decltype(type)::value> ep{{y0, y1}, nullptr, (size_t)n, m, n, aligned(y0, n, out) && (batch == 1 || aligned(y1, n, out))};
-        return launch<false, Tile128>(ra, rb, rb, (size_t)m * ld_a * 2, batch, stages, n, ep, stream);
-    });
+    auto run = [&](auto type, auto columns) {
+        constexpr int OUT = decltype(type)::value;
+        if (stages == 0) {
+            hipError_t e = hipSuccess;
+            for (int z = 0; z < batch && e == hipSuccess; ++z)
+                e = fill_rows<OUT>(z ? y1 : y0, nullptr, (size_t)m, (size_t)n, stream);
+            return e;
+        }
+        const PlainEpilogue<OUT, decltype(columns)::value> ep{y0, y1, nullptr, (size_t)n, m, n};
+        return launch<false>(ra, rb, rb, (size_t)m * ld_a * 2, batch, stages, n, ep, dev, stream);
+    };
+    if (out == kOutF32)
+        return run(std::integral_constant<int, kOutF32>{}, std::true_type{});
+    return n % 8 ? run(std::integral_constant<int, kOutBF16>{}, std::true_type{}) : run(std::integral_constant<int, kOutBF16>{}, std::false_type{});
 }
 
 }  // namespace int4linear

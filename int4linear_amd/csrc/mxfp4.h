@@ -57,7 +57,7 @@ hipError_t launch_mx_gated(const MxMatrix &x, const MxMatrix &wg, const MxMatrix
 // ... or in MXFP4.
 hipError_t launch_mx_gated_quantized(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, uint8_t *codes,
                                      uint8_t *scales, int k, const DeviceInfo &dev, hipStream_t stream);
-// Gradients of the two projections from dh (m x n bfloat16): d is m x 2 * ld_n, dg in columns 0 .. ld_n - 1 and du
+// Gradients of the two projections (k > 0) from dh (m x n bfloat16): d is m x 2 * ld_n, dg in columns 0 .. ld_n - 1 and du
 // behind them, dt is 2 * n x ld_m, the transposes of both; bfloat16, padding written as zeros.
 hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
                                      uint16_t *d, size_t ld_n, uint16_t *dt, size_t ld_m, int k, const DeviceInfo &dev,
