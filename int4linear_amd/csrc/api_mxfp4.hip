@@ -241,11 +241,11 @@ int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, co
     if (e == hipSuccess && want_dw && m > 0)
         e = launch_mx_dequantize_transposed(matrix(x_codes_d, x_scales_d, m), p.x_t, p.ld_m, k, stream);
     if (e == hipSuccess && want_dw)
-        e = launch_bf16_gemm(p.dy_t, p.ld_m, n, p.x_t, p.ld_m, k, m, dw_d, dw_d, 1, dw_type, info, stream);
+        e = launch_bf16_gemm(p.dy_t, n, p.x_t, k, p.ld_m, m, dw_d, dw_d, 1, dw_type, info, stream);
     if (e == hipSuccess && want_dx && n > 0)
         e = launch_mx_dequantize_transposed(matrix(w_codes_d, w_scales_d, n), p.w_t, p.ld_n, k, stream);
     if (e == hipSuccess && want_dx)
-        e = launch_bf16_gemm(ragged ? p.dy_padded : dy, p.ld_n, m, p.w_t, p.ld_n, k, n, dx_d, dx_d, 1, kOutBF16, info, stream);
+        e = launch_bf16_gemm(ragged ? p.dy_padded : dy, m, p.w_t, k, p.ld_n, n, dx_d, dx_d, 1, kOutBF16, info, stream);
     return api_status(e);
 }
 
@@ -287,14 +287,14 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
     if (e == hipSuccess && want_dw && m > 0)
         e = launch_mx_dequantize_transposed(x, p.x_t, p.ld_m, k, stream);
     if (e == hipSuccess && want_dw)
-        e = launch_bf16_gemm(p.d_t, p.ld_m, n, p.x_t, p.ld_m, k, m, dwg_d, dwu_d, 2, dw_type, info, stream);
+        e = launch_bf16_gemm(p.d_t, n, p.x_t, k, p.ld_m, m, dwg_d, dwu_d, 2, dw_type, info, stream);
     // wg and wu side by side: row c of w_t is column c of wg, then column c of wu
     if (e == hipSuccess && want_dx && n > 0)
         e = launch_mx_dequantize_transposed(wg, p.w_t, 2 * p.ld_n, k, stream);
     if (e == hipSuccess && want_dx && n > 0)
         e = launch_mx_dequantize_transposed(wu, p.w_t + p.ld_n, 2 * p.ld_n, k, stream);
     if (e == hipSuccess && want_dx)
-        e = launch_bf16_gemm(p.d, 2 * p.ld_n, m, p.w_t, 2 * p.ld_n, k, (int)(n > 0 ? 2 * p.ld_n : 0), dx_d, dx_d, 1, kOutBF16, info,
+        e = launch_bf16_gemm(p.d, m, p.w_t, k, 2 * p.ld_n, (int)(n > 0 ? 2 * p.ld_n : 0), dx_d, dx_d, 1, kOutBF16, info,
                              stream);
     return api_status(e);
 }

@@ -7,8 +7,8 @@
 // group lane / 32 takes chunk (16 bytes) 4 * (lane / 32) + j of its rows in step j = 0 .. 3, for a and b
 // alike, which is all that a sum over k asks for.  With 4-bit operands a chunk is one block of 32, and the
 // scales of the four chunks that a lane sees in a stage are the four bytes of one aligned dword.
-//
 #include "mxfp4.h"
+#include "mxfp4_epilogue.h"
 
 #include <type_traits>
 #include <utility>
@@ -27,13 +27,14 @@ typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 constexpr int kFrag = 32;
 
-// Rows of an operand.  data[row * stride] starts a row of `stages` lines; scales likewise (4-bit only).
-struct LineRows {
-    const uint8_t *data;
-    const uint8_t *scales;
-    size_t stride;
-    size_t scale_stride;
-    int rows;
+// The operands.  A row is `stages` lines, `stride` bytes from the next, and with 4-bit values its scales, scale_stride
+// bytes from the next, for a and b alike.  The gated block's two matrices b have as many rows each.
+struct LineOperands {
+    const uint8_t *a, *b0, *b1;
+    const uint8_t *a_scales, *b0_scales, *b1_scales;
+    size_t a_batch;  // bytes from the matrix a of blockIdx.z to the next
+    unsigned stride, scale_stride;
+    int a_rows, b_rows, stages;
 };
 
 // ---- what happens to a tile's sums ------------------------------------------------------------
@@ -46,9 +47,6 @@ struct LineRows {
 // bytes.  All others take the second: a store covers 32 neighbouring elements of two rows, wherever they begin.
 // kPair: two operands b share the tile, blocks i even of the first, odd of the second, each pair over the same
 // 32 columns.
-
-template <int OUT>
-using OutElement = std::conditional_t<OUT == kOutF32, float, std::conditional_t<OUT == kOutF16, _Float16, __bf16>>;
 
 // A lane's 16 columns of a row (kColumns = false), rounded to 16 bits -> 8 columns from 8 * (lane / 32) on
 // in out[0], from 16 + 8 * (lane / 32) on in out[1].
@@ -144,24 +142,6 @@ struct PlainEpilogue {
     }
 };
 
-// act(g) and its slope.  The gelu's (1 + tanh z) / 2 is the logistic function of 2 z.
-constexpr float kGeluScale = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-constexpr float kGeluCubic = 0.044715f;
-
-__device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
-
-__device__ __forceinline__ float activate(int act, float g)
-{
-    return g * logistic(act == kSilu ? g : kGeluScale * (g + kGeluCubic * g * g * g));
-}
-
-__device__ __forceinline__ void activate_with_slope(int act, float g, float &value, float &slope)
-{
-    const float s = logistic(act == kSilu ? g : kGeluScale * (g + kGeluCubic * g * g * g));
-    value = g * s;
-    slope = s + g * s * (1.0f - s) * (act == kSilu ? 1.0f : kGeluScale * (1.0f + 3.0f * kGeluCubic * g * g));
-}
-
 // h = act(g) * u, rounded once to OUT.
 template <int OUT, bool COLUMNS>
 struct GatedEpilogue {
@@ -212,21 +192,9 @@ struct GatedMxEpilogue {
                 }
                 const auto both = __builtin_amdgcn_permlane32_swap(big, big, false, false);
                 big = max(both[0], both[1]);
-                const int field = (int)(big >> 23);
-                const int code = field == 255 ? 255 : max(field - 2, 0);
-                const float inverse = __builtin_bit_cast(float, code >= 254 ? 0x00400000 : (254 - code) << 23);
-                unsigned bits[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float s[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        s[e] = field == 255 ? 0.0f : v[8 * h + e] * inverse;
-                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, s[0], s[1], 1.0f, 0);
-                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(bits[h], s[2], s[3], 1.0f, 1);
-                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(bits[h], s[4], s[5], 1.0f, 2);
-                    bits[h] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(bits[h], s[6], s[7], 1.0f, 3);
-                }
+                unsigned code, bits[2];
+                bits[0] = encode_block_part({v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}, big, code);
+                bits[1] = encode_block_part({v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]}, big, code);
                 // bits[h]: 16 bits for columns 16 h + 4 (lane / 32) .., 16 for those 8 further on.  The lane pair's four words
                 // make dwords 2 h and 2 h + 1 of the block; the lower lane takes h = 0, the upper h = 1.
                 const auto x = __builtin_amdgcn_permlane32_swap(bits[0], bits[1], false, false);
@@ -234,13 +202,8 @@ struct GatedMxEpilogue {
                 if (r < m && (size_t)c0 < code_stride * 2) {
                     *(unsigned long long *)(codes + (size_t)r * code_stride + c0 / 2 + 8 * (lane >> 5)) =
                         lo | ((unsigned long long)hi << 32);
-                    if (lane < 32) {
-                        uint8_t *to = scales + (size_t)r * scale_stride + c0 / kMxBlock;
-                        *to = (uint8_t)code;
-                        // the row's last line of codes; its scales go on for one more where they are not 16 yet
-                        if ((size_t)c0 + kMxBlock == code_stride * 2 && code_stride % (2 * kLineBytes))
-                            *(unsigned long long *)(to + 1) = 0;
-                    }
+                    if (lane < 32)
+                        store_block_scale(scales + (size_t)r * scale_stride, c0, code_stride, code);
                 }
             }
         }
@@ -316,19 +279,23 @@ struct GradientEpilogue {
 
 // ---- the kernel -------------------------------------------------------------------------------
 
-// WAVES_M x WAVES_N wavefronts, each FM x FN blocks of 32 x 32; OCC waves per SIMD.
-template <int WAVES_M_, int WAVES_N_, int FM_, int FN_, int OCC_>
+constexpr int kChunkRows = 8;    // rows of a 1-KiB load
+constexpr int kScaleStages = 2;  // stages whose scales are 16 bytes of a row
+constexpr int kSteps = 4;        // steps of a stage
+
+// WAVES_M x WAVES_N wavefronts, each FM x FN blocks of 32 x 32; STAGES stages in LDS; OCC waves per SIMD.
+template <int WAVES_M_, int WAVES_N_, int FM_, int FN_, int STAGES_, int OCC_>
 struct LineTile {
-    static constexpr int WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, FM = FM_, FN = FN_, OCC = OCC_;
+    static constexpr int WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, FM = FM_, FN = FN_, STAGES = STAGES_, OCC = OCC_;
     static constexpr int NWAVES = WAVES_M * WAVES_N, THREADS = NWAVES * 64;
     static constexpr int BM = WAVES_M * FM * kFrag, BN = WAVES_N * FN * kFrag;
     static constexpr int STAGE = (BM + BN) * kLineBytes;
-    static constexpr int SCALES = (BM + BN) * 16;       // scales of two stages
-    static constexpr int LDS = 2 * STAGE + 2 * SCALES;  // two of each
-    static constexpr int CHUNK_ROWS = 8;                // rows of a 1-KiB load
-    static constexpr int A_CH = BM / CHUNK_ROWS / NWAVES, B_CH = BN / CHUNK_ROWS / NWAVES;  // loads per wave and stage
-    static constexpr int SLOTS = FM * FN;               // matrix instructions per step
-    static_assert(BM % (CHUNK_ROWS * NWAVES) == 0 && BN % (CHUNK_ROWS * NWAVES) == 0 && BM % 64 == 0 && BN % 64 == 0);
+    static constexpr int SCALES = (BM + BN) * 16;                 // scales of two stages
+    template <bool FP4>
+    static constexpr int LDS = STAGES * (STAGE + (FP4 ? SCALES : 0));
+    static constexpr int A_CH = BM / kChunkRows / NWAVES, B_CH = BN / kChunkRows / NWAVES;  // loads per wave and stage
+    static constexpr int SLOTS = FM * FN;                         // matrix instructions per step
+    static_assert(BM % (kChunkRows * NWAVES) == 0 && BN % (kChunkRows * NWAVES) == 0 && BM % 64 == 0 && BN % 64 == 0);
 };
 
 // Order of tiles: workgroup ids go round-robin over the 8 XCDs; ids congruent mod 8 get consecutive
@@ -351,16 +318,6 @@ __device__ __forceinline__ void tile_coords(int v, int total, int tiles_m, int t
 
 #define I4L_LDS(p) ((__attribute__((address_space(3))) void *)(p))
 
-// 16 bytes per lane from base + offset straight into LDS at to + 16 * lane.
-__device__ __forceinline__ void dma16(const void *base, unsigned offset, unsigned to)
-{
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory");
-}
-__device__ __forceinline__ void dma16(const void *lane_address, unsigned to)
-{
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(lane_address), "s"(to) : "memory");
-}
-
 // Marks a value as used at this point of the program without generating code.
 __device__ __forceinline__ void pin(const v16f &v) { asm volatile("" ::"v"(v)); }
 
@@ -382,13 +339,12 @@ hipError_t fill_rows(void *y, const float *bias, size_t m, size_t n, hipStream_t
 }
 
 // Persistent: a workgroup walks tiles blockIdx.x, + gridDim.x, ... and its loads run ahead of the
-// arithmetic across the ends of tiles.  Two stages of lines ring in LDS.  A stage is four steps of FM x FN
-// matrix instructions; while a step's instructions run, the next step's operands are read from LDS into the other
-// register set.  Before a stage's last step every read of the stage has been made: there the waves meet, the
-// next stage must have landed, and the stage's buffer is given to the loads of the one after that.
+// arithmetic across the ends of tiles.  STAGES stages ring in LDS.  A stage is four steps of FM x FN matrix
+// instructions; while a step's instructions run, the next step's operands are read from LDS into the other register
+// set.  Before a stage's last step every read of the stage has been made: there the waves meet, the next stage must
+// have landed (younger ones stay in flight), and the stage's buffer is given to the loads of the stage STAGES further on.
 template <bool FP4, class C, class Ep>
-__global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows a, LineRows b0, LineRows b1, size_t a_batch, int stages,
-                                                                       int tiles_m, int tiles_n, Ep ep)
+__global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOperands o, int tiles_m, int tiles_n, Ep ep)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
@@ -396,7 +352,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
     const int wm = wave / C::WAVES_N, wn = wave % C::WAVES_N;
     const int total = tiles_m * tiles_n;
     const int my_tiles = (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
-    const uint8_t *a_data = a.data + blockIdx.z * a_batch;
+    const uint8_t *a_data = o.a + blockIdx.z * o.a_batch;
+    const int stages = o.stages;
     constexpr int kTileN = Ep::kPair ? C::BN / 2 : C::BN;  // columns of y
 
     v16f acc[C::FM][C::FN];
@@ -419,13 +376,11 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
     // stage, lane l the 16 bytes at place l % 8 of row l / 8.  The chunk that lies at place p of row r is
     // p ^ (r / 2 % 8): the 16 lanes that an LDS read serves together then touch every bank once.
     const unsigned lds_base = (unsigned)(size_t)I4L_LDS(lds);
-    const int ld_row = wave * C::CHUNK_ROWS + (lane >> 3);
+    const int ld_row = wave * kChunkRows + (lane >> 3);
     const unsigned ld_chunk = (unsigned)(((lane & 7) ^ ((ld_row >> 1) & 7)) * 16);
-    static_assert(C::NWAVES * C::CHUNK_ROWS % 16 == 0 || C::A_CH + C::B_CH == 2, "the same swizzle for all loads of a lane");
-    const uint8_t *a_base = nullptr, *b_base[2] = {};  // this tile's rows, this stage's line
+    const uint8_t *a_base = nullptr, *b_base[2] = {};  // this tile's rows, this stage's bytes
     unsigned a_off[C::A_CH], b_off[C::B_CH];
     const uint8_t *scale_at = nullptr;  // FP4: this lane's row of scales (wave w moves those of LDS rows 64 w ..)
-    constexpr bool kScaleWavesAll = (C::BM + C::BN) / 64 >= C::NWAVES;
     static_assert((C::BM + C::BN) / 64 <= C::NWAVES);
     int ld_it = 0, ld_s = 0;
     unsigned ld_buffer = 0, ld_slot = 0;
@@ -438,26 +393,26 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
         int tm, tn;
         tile_coords(blockIdx.x + it * gridDim.x, total, tiles_m, tiles_n, tm, tn);
         const int m0 = tm * C::BM, n0 = tn * kTileN;
-        a_base = a_data + (size_t)m0 * a.stride;
+        a_base = uniform(a_data + (size_t)m0 * o.stride);
         // rows behind the matrix: the last one again
-        const int last_a = a.rows - 1 - m0, last_b = b0.rows - 1 - n0;
+        const int last_a = o.a_rows - 1 - m0, last_b = o.b_rows - 1 - n0;
 #pragma unroll
         for (int c = 0; c < C::A_CH; ++c)
-            a_off[c] = (unsigned)min(c * C::NWAVES * C::CHUNK_ROWS + ld_row, last_a) * (unsigned)a.stride + ld_chunk;
+            a_off[c] = (unsigned)min(c * C::NWAVES * kChunkRows + ld_row, last_a) * o.stride + ld_chunk;
         // (last_b is negative where h's padding alone is in the tile: then the matrix's last row)
-        const int nb = min(n0, b0.rows - 1);
-        b_base[0] = b0.data + (size_t)nb * b0.stride;
-        b_base[1] = b1.data + (size_t)nb * b0.stride;
+        const int nb = min(n0, o.b_rows - 1);
+        b_base[0] = uniform(o.b0 + (size_t)nb * o.stride);
+        b_base[1] = uniform(o.b1 + (size_t)nb * o.stride);
 #pragma unroll
         for (int c = 0; c < C::B_CH; ++c)
-            b_off[c] = (unsigned)max(min(b_row(c * C::NWAVES * C::CHUNK_ROWS + ld_row), last_b), 0) * (unsigned)b0.stride + ld_chunk;
+            b_off[c] = (unsigned)max(min(b_row(c * C::NWAVES * kChunkRows + ld_row), last_b), 0) * o.stride + ld_chunk;
         if constexpr (FP4) {
             const int r = wave * 64 + lane;
             if (r < C::BM) {
-                scale_at = a.scales + (size_t)(m0 + min(r, last_a)) * a.scale_stride;
+                scale_at = o.a_scales + (size_t)(m0 + min(r, last_a)) * o.scale_stride;
             } else {
                 const int br = r - C::BM;
-                scale_at = (b_second(br) ? b1.scales : b0.scales) + (size_t)(nb + max(min(b_row(br), last_b), 0)) * b0.scale_stride;
+                scale_at = (b_second(br) ? o.b1_scales : o.b0_scales) + (size_t)(nb + max(min(b_row(br), last_b), 0)) * o.scale_stride;
             }
         }
     };
@@ -467,53 +422,53 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
         if (c < C::A_CH)
             dma16(a_base, a_off[c], to + (unsigned)(c * C::NWAVES) * 1024u);
         else
-            dma16(b_base[b_second(((c - C::A_CH) * C::NWAVES + wave) * C::CHUNK_ROWS)], b_off[c - C::A_CH], to + (unsigned)(C::BM * kLineBytes) + (unsigned)((c - C::A_CH) * C::NWAVES) * 1024u);
+            dma16(b_base[b_second(((c - C::A_CH) * C::NWAVES + wave) * kChunkRows)], b_off[c - C::A_CH],
+                  to + (unsigned)(C::BM * kLineBytes) + (unsigned)((c - C::A_CH) * C::NWAVES) * 1024u);
     };
+    auto next_in_ring = [](unsigned at, unsigned step) { return at == (C::STAGES - 1) * step ? 0u : at + step; };
     // After a stage's loads: its scales, if they are not there already, and on to the next stage.  Behind the
-    // last stage the cursor stays: it is loaded again, into a buffer that nobody reads.
+    // last stage the cursor stays: it is loaded again, into buffers that nobody reads.
     auto load_rest = [&] {
         if constexpr (FP4) {
-            if ((ld_s & 1) == 0 && (kScaleWavesAll || wave < (C::BM + C::BN) / 64))
-                dma16(scale_at, lds_base + 2 * C::STAGE + ld_slot + (unsigned)wave * 1024u);
+            if (ld_s % kScaleStages == 0 && ((C::BM + C::BN) / 64 == C::NWAVES || wave < (C::BM + C::BN) / 64))
+                dma16(scale_at, lds_base + C::STAGES * C::STAGE + ld_slot + (unsigned)wave * 1024u);
         }
-        ld_buffer ^= (unsigned)C::STAGE;
+        ld_buffer = next_in_ring(ld_buffer, C::STAGE);
         if (ld_s + 1 < stages) {
             ++ld_s;
             a_base += kLineBytes;
             b_base[0] += kLineBytes;
             b_base[1] += kLineBytes;
-            if ((ld_s & 1) == 0) {
+            if (FP4 && ld_s % kScaleStages == 0) {
                 scale_at += 16;
-                ld_slot ^= (unsigned)C::SCALES;
+                ld_slot = next_in_ring(ld_slot, C::SCALES);
             }
         } else if (ld_it + 1 < my_tiles) {
             ld_s = 0;
-            ld_slot ^= (unsigned)C::SCALES;
+            ld_slot = next_in_ring(ld_slot, C::SCALES);
             ld_tile(++ld_it);
         }
     };
-    static_assert((C::STAGE & (C::STAGE - 1)) == 0 && (C::SCALES & (C::SCALES - 1)) == 0);
 
     ld_tile(0);
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c)
-        load(c);
-    load_rest();
+    for (int st = 0; st < C::STAGES; ++st) {
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c)
-        load(c);
-    load_rest();
+        for (int c = 0; c < kLoads; ++c)
+            load(c);
+        load_rest();
+    }
 
     // ---- arithmetic
     const int fr = lane & 31, fg = lane >> 5;
-    unsigned chunk_at[4];
+    unsigned chunk_at[kSteps];
 #pragma unroll
-    for (int J = 0; J < 4; ++J)
-        chunk_at[J] = (unsigned)(((4 * fg + J) ^ ((fr >> 1) & 7)) * 16 + fr * kLineBytes);
+    for (int J = 0; J < kSteps; ++J)
+        chunk_at[J] = (unsigned)(((kSteps * fg + J) ^ ((fr >> 1) & 7)) * 16 + fr * kLineBytes);
     const unsigned a_rd = (unsigned)(wm * C::FM * kFrag * kLineBytes);
     const unsigned b_rd = (unsigned)((C::BM + wn * C::FN * kFrag) * kLineBytes);
-    const unsigned as_rd = (unsigned)(2 * C::STAGE + (wm * C::FM * kFrag + fr) * 16 + 4 * fg);
-    const unsigned bs_rd = (unsigned)(2 * C::STAGE + (C::BM + wn * C::FN * kFrag + fr) * 16 + 4 * fg);
+    const unsigned as_rd = (unsigned)(C::STAGES * C::STAGE + (wm * C::FM * kFrag + fr) * 16 + 4 * fg);
+    const unsigned bs_rd = (unsigned)(C::STAGES * C::STAGE + (C::BM + wn * C::FN * kFrag + fr) * 16 + 4 * fg);
     v4i fa[2][C::FM], fb[2][C::FN];
     int sa[2][C::FM] = {}, sb[2][C::FN] = {};
 
@@ -528,7 +483,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
     };
     auto read_scales = [&](unsigned slot, int s, int p) {
         if constexpr (FP4) {
-            const uint8_t *at = lds + (slot + 8 * (s & 1));
+            const uint8_t *at = lds + (slot + 8 * (s % kScaleStages));
 #pragma unroll
             for (int j = 0; j < C::FM; ++j)
                 sa[p][j] = *(const int *)(at + as_rd + j * kFrag * 16);
@@ -567,21 +522,31 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
     constexpr int kReadsPerSlot = (kReads + C::SLOTS - 1) / C::SLOTS;
     constexpr int kLoadsPerSlot = (kLoads + C::SLOTS - 1) / C::SLOTS;
 
-    // Lines have landed and every wave is here.
-    auto meet = [&] {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // All but the youngest IN_FLIGHT stages have landed, this wave's reads are done, and every wave is here.  (Loads
+    // complete in order; scales and stores in between only make the wait a little longer.)
+    auto meet = [&](auto in_flight) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(decltype(in_flight)::value * kLoads) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    meet();
+    static_assert((C::STAGES - 1) * kLoads <= 63);
+    meet(std::integral_constant<int, C::STAGES - 1>{});
 #pragma unroll
     for (int r = 0; r < kReads; ++r)
         read(0, 0, 0, r);
-    read_scales(0, 0, 0);
+    read_scales(0, 0, 1);
 
     unsigned buffer = 0, slot = 0;
     int it = 0, s = 0;
     while (true) {
+        if constexpr (FP4) {
+#pragma unroll
+            for (int j = 0; j < C::FM; ++j)
+                sa[0][j] = sa[1][j];
+#pragma unroll
+            for (int i = 0; i < C::FN; ++i)
+                sb[0][i] = sb[1][i];
+        }
         [&]<int... J>(std::integer_sequence<int, J...>) {
             (step(std::integral_constant<int, J>{},
                   [&](auto slot_tag) {
@@ -591,32 +556,25 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
                           read(buffer, J + 1, (J + 1) & 1, r);
                   }),
              ...);
-        }(std::make_integer_sequence<int, 3>{});
-        meet();
+        }(std::make_integer_sequence<int, kSteps - 1>{});
+        meet(std::integral_constant<int, C::STAGES - 2>{});
         const bool last = s + 1 == stages;
         const int next_s = last ? 0 : s + 1;
-        if ((next_s & 1) == 0)
-            slot ^= (unsigned)C::SCALES;
+        if (FP4 && next_s % kScaleStages == 0)
+            slot = next_in_ring(slot, C::SCALES);
+        const unsigned next_buffer = next_in_ring(buffer, C::STAGE);
         read_scales(slot, next_s, 1);
-        step(std::integral_constant<int, 3>{}, [&](auto slot_tag) {
+        step(std::integral_constant<int, kSteps - 1>{}, [&](auto slot_tag) {
             constexpr int at = decltype(slot_tag)::value * kReadsPerSlot, load_at = decltype(slot_tag)::value * kLoadsPerSlot;
 #pragma unroll
             for (int r = at; r < at + kReadsPerSlot && r < kReads; ++r)
-                read(buffer ^ (unsigned)C::STAGE, 0, 0, r);
+                read(next_buffer, 0, 0, r);
 #pragma unroll
             for (int c = load_at; c < load_at + kLoadsPerSlot && c < kLoads; ++c)
                 load(c);
         });
         load_rest();
-        if constexpr (FP4) {
-#pragma unroll
-            for (int j = 0; j < C::FM; ++j)
-                sa[0][j] = sa[1][j];
-#pragma unroll
-            for (int i = 0; i < C::FN; ++i)
-                sb[0][i] = sb[1][i];
-        }
-        buffer ^= (unsigned)C::STAGE;
+        buffer = next_buffer;
         s = next_s;
         if (last) {
             finish(it);
@@ -628,32 +586,41 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineRows 
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-using Tile128 = LineTile<2, 2, 2, 2, 2>;
-using Tile256 = LineTile<4, 2, 2, 4, 2>;
+using Tile256 = LineTile<4, 2, 2, 4, 2, 2>;
+using Tile128 = LineTile<2, 2, 2, 2, 2, 2>;
+using TileWide = LineTile<2, 2, 1, 2, 3, 2>;  // 64 x 128
+
+// Workgroups of a tile that a CU's LDS holds.
+template <class C, bool FP4>
+constexpr int per_cu = 160 * 1024 / C::template LDS<FP4>;
 
 template <bool FP4, class C, class Ep>
-hipError_t launch_tile(const LineRows &a, const LineRows &b0, const LineRows &b1, size_t a_batch, int batch, int stages, int n, const Ep &ep,
-                       const DeviceInfo &dev, hipStream_t stream)
+hipError_t launch_tile(const LineOperands &o, int batch, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
     const int bn = Ep::kPair ? C::BN / 2 : C::BN;
-    const int tiles_m = (a.rows + C::BM - 1) / C::BM, tiles_n = (n + bn - 1) / bn;
-    const int per_cu = C::NWAVES >= 8 ? 1 : 2;
-    const int groups = min(tiles_m * tiles_n, max(1, dev.cu_count * per_cu / batch));
-    line_gemm_kernel<FP4, C, Ep><<<dim3((unsigned)groups, 1, (unsigned)batch), C::THREADS, C::LDS, stream>>>(a, b0, b1, a_batch, stages, tiles_m, tiles_n, ep);
+    const int tiles_m = (o.a_rows + C::BM - 1) / C::BM, tiles_n = (n + bn - 1) / bn;
+    const int groups = min(tiles_m * tiles_n, max(1, dev.cu_count * per_cu<C, FP4> / batch));
+    line_gemm_kernel<FP4, C, Ep><<<dim3((unsigned)groups, 1, (unsigned)batch), C::THREADS, C::template LDS<FP4>, stream>>>(o, tiles_m, tiles_n, ep);
     return hipGetLastError();
 }
 
+// n: columns of the product that have to be covered.
 template <bool FP4, class Ep>
-hipError_t launch(const LineRows &a, const LineRows &b0, const LineRows &b1, size_t a_batch, int batch, int stages, int n, const Ep &ep,
-                  const DeviceInfo &dev, hipStream_t stream)
+hipError_t launch(const LineOperands &o, int batch, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
-    const long tiles256 = (long)((a.rows + 255) / 256) * ((n + (Ep::kPair ? 127 : 255)) / (Ep::kPair ? 128 : 256)) * batch;
+    const long tiles256 = (long)((o.a_rows + 255) / 256) * ((n + (Ep::kPair ? 127 : 255)) / (Ep::kPair ? 128 : 256)) * batch;
     if (tiles256 >= 128)
-        return launch_tile<FP4, Tile256>(a, b0, b1, a_batch, batch, stages, n, ep, dev, stream);
-    return launch_tile<FP4, Tile128>(a, b0, b1, a_batch, batch, stages, n, ep, dev, stream);
+        return launch_tile<FP4, Tile256>(o, batch, n, ep, dev, stream);
+    return launch_tile<FP4, Tile128>(o, batch, n, ep, dev, stream);
 }
 
-LineRows rows_of(const MxMatrix &q, int k) { return {q.codes, q.scales, mx_code_stride(k), mx_scale_stride(k), q.rows}; }
+LineOperands operands(const MxMatrix &x, const MxMatrix &w0, const MxMatrix &w1, int k)
+{
+    return {x.codes, w0.codes, w1.codes, x.scales, w0.scales, w1.scales, 0, (unsigned)mx_code_stride(k), (unsigned)mx_scale_stride(k),
+            x.rows, w0.rows, (k + kLineFp4 - 1) / kLineFp4};
+}
+
+constexpr int kSkinnyRows = 32;  // up to here the weight-streaming kernel
 
 // f(type, columns) with the output type of a call and the epilogue's form for rows of n elements.
 template <class F>
@@ -676,7 +643,7 @@ static hipError_t allow_lds()
     auto allow = [&](auto tile) {
         using C = decltype(tile);
         if (e == hipSuccess)
-            e = hipFuncSetAttribute((const void *)line_gemm_kernel<FP4, C, Ep>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+            e = hipFuncSetAttribute((const void *)line_gemm_kernel<FP4, C, Ep>, hipFuncAttributeMaxDynamicSharedMemorySize, C::template LDS<FP4>);
     };
     allow(Tile128{});
     allow(Tile256{});
@@ -702,67 +669,69 @@ hipError_t line_gemm_init(const DeviceInfo &)
 hipError_t launch_mx_linear(const MxMatrix &x, const MxMatrix &w, const float *bias, void *y, int out, int k, const DeviceInfo &dev,
                             hipStream_t stream)
 {
-    const int stages = (k + kLineFp4 - 1) / kLineFp4;
+    if (k > 0 && x.rows <= kSkinnyRows)
+        return launch_mx_linear_skinny(x, w, bias, y, out, k, stream);
     return by_type(out, w.rows, [&](auto type, auto columns) {
         constexpr int OUT = decltype(type)::value;
-        if (stages == 0)
+        if (k == 0)
             return fill_rows<OUT>(y, bias, (size_t)x.rows, (size_t)w.rows, stream);
         const PlainEpilogue<OUT, decltype(columns)::value> ep{y, nullptr, bias, (size_t)w.rows, x.rows, w.rows};
-        return launch<true>(rows_of(x, k), rows_of(w, k), rows_of(w, k), 0, 1, stages, w.rows, ep, dev, stream);
+        return launch<true>(operands(x, w, w, k), 1, w.rows, ep, dev, stream);
     });
 }
 
 hipError_t launch_mx_gated(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, void *h, int out, int k,
                            const DeviceInfo &dev, hipStream_t stream)
 {
-    const int stages = (k + kLineFp4 - 1) / kLineFp4;
+    if (k > 0 && x.rows <= kSkinnyRows)
+        return launch_mx_gated_skinny(x, wg, wu, act, h, out, k, stream);
     return by_type(out, wg.rows, [&](auto type, auto columns) {
         constexpr int OUT = decltype(type)::value;
-        if (stages == 0)
+        if (k == 0)
             return fill_rows<OUT>(h, nullptr, (size_t)x.rows, (size_t)wg.rows, stream);
         const GatedEpilogue<OUT, decltype(columns)::value> ep{h, (size_t)wg.rows, x.rows, wg.rows, act};
-        return launch<true>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, wg.rows, ep, dev, stream);
+        return launch<true>(operands(x, wg, wu, k), 1, wg.rows, ep, dev, stream);
     });
 }
 
 hipError_t launch_mx_gated_quantized(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, uint8_t *codes,
                                      uint8_t *scales, int k, const DeviceInfo &dev, hipStream_t stream)
 {
-    const int stages = (k + kLineFp4 - 1) / kLineFp4;
     const int n = wg.rows;
-    if (stages == 0) {
+    if (k == 0) {
         hipError_t e = fill_rows<kOutF32>(codes, nullptr, (size_t)x.rows, mx_code_stride(n) / 4, stream);
         return e == hipSuccess ? fill_rows<kOutF32>(scales, nullptr, (size_t)x.rows, mx_scale_stride(n) / 4, stream) : e;
     }
+    if (x.rows <= kSkinnyRows)
+        return launch_mx_gated_quantized_skinny(x, wg, wu, act, codes, scales, k, stream);
     const GatedMxEpilogue ep{codes, scales, mx_code_stride(n), mx_scale_stride(n), x.rows, n, act};
     // (the grid covers the padding at the end of h's rows)
-    return launch<true>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, (int)(mx_code_stride(n) * 2), ep, dev, stream);
+    return launch<true>(operands(x, wg, wu, k), 1, (int)(mx_code_stride(n) * 2), ep, dev, stream);
 }
 
 hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
                                      uint16_t *d, size_t ld_n, uint16_t *dt, size_t ld_m, int k, const DeviceInfo &dev,
                                      hipStream_t stream)
 {
-    const int stages = (k + kLineFp4 - 1) / kLineFp4;
     const GradientEpilogue ep{(const __bf16 *)dh, (__bf16 *)d, (__bf16 *)dt, ld_n, ld_m, x.rows, wg.rows, act, wg.rows % 4 == 0};
-    return launch<true>(rows_of(x, k), rows_of(wg, k), rows_of(wu, k), 0, 1, stages, wg.rows, ep, dev, stream);
+    return launch<true>(operands(x, wg, wu, k), 1, wg.rows, ep, dev, stream);
 }
 
-hipError_t launch_bf16_gemm(const uint16_t *a, size_t ld_a, int m, const uint16_t *b, size_t ld_b, int n, int k, void *y0, void *y1,
-                            int batch, int out, const DeviceInfo &dev, hipStream_t stream)
+hipError_t launch_bf16_gemm(const uint16_t *a, int m, const uint16_t *b, int n, size_t ld, int k, void *y0, void *y1, int batch,
+                            int out, const DeviceInfo &dev, hipStream_t stream)
 {
-    const int stages = (k + kLineBf16 - 1) / kLineBf16;
-    const LineRows ra{(const uint8_t *)a, nullptr, ld_a * 2, 0, m}, rb{(const uint8_t *)b, nullptr, ld_b * 2, 0, n};
+    const LineOperands o{(const uint8_t *)a, (const uint8_t *)b, (const uint8_t *)b, nullptr, nullptr, nullptr, (size_t)m * ld * 2,
+                         (unsigned)(ld * 2), 0, m, n, (k + kLineBf16 - 1) / kLineBf16};
     auto run = [&](auto type, auto columns) {
         constexpr int OUT = decltype(type)::value;
-        if (stages == 0) {
+        if (k == 0) {
             hipError_t e = hipSuccess;
             for (int z = 0; z < batch && e == hipSuccess; ++z)
                 e = fill_rows<OUT>(z ? y1 : y0, nullptr, (size_t)m, (size_t)n, stream);
             return e;
         }
         const PlainEpilogue<OUT, decltype(columns)::value> ep{y0, y1, nullptr, (size_t)n, m, n};
-        return launch<false>(ra, rb, rb, (size_t)m * ld_a * 2, batch, stages, n, ep, dev, stream);
+        return launch<false>(o, batch, n, ep, dev, stream);
     };
     if (out == kOutF32)
         return run(std::integral_constant<int, kOutF32>{}, std::true_type{});

@@ -10,6 +10,7 @@
 // denormal maximum has the field 0 and meets the lower bound.  A block that holds an infinity or a NaN gets
 // the scale code 255 and stands for 32 NaNs.
 #include "mxfp4.h"
+#include "mxfp4_epilogue.h"
 
 namespace int4linear {
 
@@ -57,16 +58,6 @@ __device__ __forceinline__ unsigned quad_max(unsigned v)
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));  // lanes 1 0 3 2
     v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));  // lanes 2 3 0 1
     return v;
-}
-
-__device__ __forceinline__ unsigned encode8(const float (&v)[8])
-{
-    unsigned c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], 1.0f, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], 1.0f, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], 1.0f, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], 1.0f, 3);
-    return c;
 }
 
 // A lane converts 8 values, a quad of lanes a block, a wave kUnroll segments of 512 k (wave w those
@@ -117,14 +108,10 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const typename El
             big = max(big, __builtin_bit_cast(unsigned, v[i]) & 0x7FFFFFFFu);
         }
         big = quad_max(big);
-        const int field = (int)(big >> 23);           // 255: an infinity or a NaN
-        const int code = field == 255 ? 255 : max(field - 2, 0);
-        const float inverse = power_of_two(field == 255 ? -127 : 127 - code);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = field == 255 ? 0.0f : v[i] * inverse;
+        unsigned code;
+        const unsigned bits = encode_block_part(v, big, code);
         if ((size_t)c0 < code_stride * 2)
-            *(unsigned *)(codes + (size_t)row * code_stride + c0 / 2) = encode8(v);
+            *(unsigned *)(codes + (size_t)row * code_stride + c0 / 2) = bits;
         if ((lane & 3) == 0)
             scales[(size_t)row * scale_stride + c0 / kMxBlock] = (uint8_t)code;
     }

@@ -57,15 +57,21 @@ hipError_t launch_mx_gated(const MxMatrix &x, const MxMatrix &wg, const MxMatrix
 // ... or in MXFP4.
 hipError_t launch_mx_gated_quantized(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, uint8_t *codes,
                                      uint8_t *scales, int k, const DeviceInfo &dev, hipStream_t stream);
+// The same for few rows of x (k > 0; any number is taken): w is streamed (kernels_mxfp4_skinny.hip).
+hipError_t launch_mx_linear_skinny(const MxMatrix &x, const MxMatrix &w, const float *bias, void *y, int out, int k, hipStream_t stream);
+hipError_t launch_mx_gated_skinny(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, void *h, int out, int k,
+                                  hipStream_t stream);
+hipError_t launch_mx_gated_quantized_skinny(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, uint8_t *codes,
+                                            uint8_t *scales, int k, hipStream_t stream);
 // Gradients of the two projections (k > 0) from dh (m x n bfloat16): d is m x 2 * ld_n, dg in columns 0 .. ld_n - 1 and du
 // behind them, dt is 2 * n x ld_m, the transposes of both; bfloat16, padding written as zeros.
 hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
                                      uint16_t *d, size_t ld_n, uint16_t *dt, size_t ld_m, int k, const DeviceInfo &dev,
                                      hipStream_t stream);
 // y[z] = a[z] b^T for bfloat16 operands whose rows are `k` values, padded with zeros to a multiple of 64 (`ld`
-// elements between rows, a multiple of 64).  a is `batch` (1 or 2) matrices of m rows back to back.
-hipError_t launch_bf16_gemm(const uint16_t *a, size_t ld_a, int m, const uint16_t *b, size_t ld_b, int n, int k, void *y0, void *y1,
-                            int batch, int out, const DeviceInfo &dev, hipStream_t stream);
+// elements between rows of either, a multiple of 64).  a is `batch` (1 or 2) matrices of m rows back to back.
+hipError_t launch_bf16_gemm(const uint16_t *a, int m, const uint16_t *b, int n, size_t ld, int k, void *y0, void *y1, int batch, int out,
+                            const DeviceInfo &dev, hipStream_t stream);
 
 // Between the files of the C ABI (api.hip): the current device's record, set up for work on `stream`, and a
 // HIP error as the status of a call.  Both return an INT4LINEAR_* status.
