@@ -588,7 +588,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
 
 using Tile256 = LineTile<4, 2, 2, 4, 2, 2>;
 using Tile128 = LineTile<2, 2, 2, 2, 2, 2>;
-using TileWide = LineTile<2, 2, 1, 2, 3, 2>;  // 64 x 128
+using Tile64x128 = LineTile<2, 2, 1, 2, 3, 2>;
+using Tile64 = LineTile<2, 2, 1, 1, 4, 2>;  // (too narrow for pairs of blocks)
 
 // Workgroups of a tile that a CU's LDS holds.
 template <class C, bool FP4>
@@ -604,14 +605,51 @@ hipError_t launch_tile(const LineOperands &o, int batch, int n, const Ep &ep, co
     return hipGetLastError();
 }
 
+// What a tile costs, in units of 10 ns: a stage on a CU that is busy with such tiles, and what a launch spends
+// before its first and after its last.  Read off products that fill the device (8192^3 in 283, 343, 520 and 573 us) and
+// ones of a few stages (1024^3 in 11.8, 6.3, 5.4, 4.9 us; 130 x 1001 x 515 in 21.3, 11.7, 7.9, 5.7 us).
+struct TileCost {
+    int m, n, stage, fixed;
+};
+constexpr TileCost kTiles[] = {{256, 256, 175, 1100}, {128, 128, 65, 650}, {64, 128, 50, 550}, {64, 64, 28, 500}};
+
+// The tile that such costs make the quickest for a product of m x n (columns of b) in `stages` stages.  It was the quickest or
+// within a tenth of it at 512 x 4096 x 11008 (us by size: 64, 33.6, 27.0, 30.5), 333 x 11008 x 4999 (36.5, 23.8, 35.2, 34.0),
+// 2048 x 4096 x 4096 (33, 26, 41, 49), 128 x 14336 x 4096 (26.0, 14.9, 12.0, 13.6) and 64 x 4096 x 4096 (23.3, 12.8, 10.8, 9.4).
+int quickest_tile(long m, long n, int batch, int stages, bool pair, const DeviceInfo &dev)
+{
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < 3 + !pair; ++i) {
+        const TileCost &t = kTiles[i];
+        const long tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n) * batch;
+        const long turns = (tiles + dev.cu_count - 1) / (dev.cu_count > 0 ? dev.cu_count : 1);
+        const double cost = (double)turns * stages * t.stage + t.fixed;
+        if (i == 0 || cost < least) {
+            best = i;
+            least = cost;
+        }
+    }
+    return best;
+}
+
 // n: columns of the product that have to be covered.
 template <bool FP4, class Ep>
 hipError_t launch(const LineOperands &o, int batch, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
-    const long tiles256 = (long)((o.a_rows + 255) / 256) * ((n + (Ep::kPair ? 127 : 255)) / (Ep::kPair ? 128 : 256)) * batch;
-    if (tiles256 >= 128)
+    switch (quickest_tile(o.a_rows, (long)n * (Ep::kPair ? 2 : 1), batch, o.stages, Ep::kPair, dev)) {
+    case 0:
         return launch_tile<FP4, Tile256>(o, batch, n, ep, dev, stream);
-    return launch_tile<FP4, Tile128>(o, batch, n, ep, dev, stream);
+    case 1:
+        return launch_tile<FP4, Tile128>(o, batch, n, ep, dev, stream);
+    case 2:
+        return launch_tile<FP4, Tile64x128>(o, batch, n, ep, dev, stream);
+    default:
+        if constexpr (Ep::kPair)
+            return hipErrorInvalidValue;
+        else
+            return launch_tile<FP4, Tile64>(o, batch, n, ep, dev, stream);
+    }
 }
 
 LineOperands operands(const MxMatrix &x, const MxMatrix &w0, const MxMatrix &w1, int k)
@@ -645,8 +683,11 @@ static hipError_t allow_lds()
         if (e == hipSuccess)
             e = hipFuncSetAttribute((const void *)line_gemm_kernel<FP4, C, Ep>, hipFuncAttributeMaxDynamicSharedMemorySize, C::template LDS<FP4>);
     };
-    allow(Tile128{});
     allow(Tile256{});
+    allow(Tile128{});
+    allow(Tile64x128{});
+    if constexpr (!Ep::kPair)
+        allow(Tile64{});
     return e;
 }
 
