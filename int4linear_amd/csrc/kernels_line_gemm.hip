@@ -283,19 +283,21 @@ constexpr int kChunkRows = 8;    // rows of a 1-KiB load
 constexpr int kScaleStages = 2;  // stages whose scales are 16 bytes of a row
 constexpr int kSteps = 4;        // steps of a stage
 
-// WAVES_M x WAVES_N wavefronts, each FM x FN blocks of 32 x 32; STAGES stages in LDS; OCC waves per SIMD.
-template <int WAVES_M_, int WAVES_N_, int FM_, int FN_, int STAGES_, int OCC_>
+// WAVES_M x WAVES_N wavefronts multiply, each FM x FN blocks of 32 x 32; LOADERS more load for them (0: each of the
+// others loads its share); STAGES stages in LDS; OCC waves per SIMD.
+template <int WAVES_M_, int WAVES_N_, int FM_, int FN_, int LOADERS_, int STAGES_, int OCC_>
 struct LineTile {
-    static constexpr int WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, FM = FM_, FN = FN_, STAGES = STAGES_, OCC = OCC_;
-    static constexpr int NWAVES = WAVES_M * WAVES_N, THREADS = NWAVES * 64;
+    static constexpr int WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, FM = FM_, FN = FN_, LOADERS = LOADERS_, STAGES = STAGES_, OCC = OCC_;
+    static constexpr int NWAVES = WAVES_M * WAVES_N, THREADS = (NWAVES + LOADERS) * 64;
+    static constexpr int LOADING = LOADERS ? LOADERS : NWAVES;    // waves that load
     static constexpr int BM = WAVES_M * FM * kFrag, BN = WAVES_N * FN * kFrag;
     static constexpr int STAGE = (BM + BN) * kLineBytes;
     static constexpr int SCALES = (BM + BN) * 16;                 // scales of two stages
     template <bool FP4>
     static constexpr int LDS = STAGES * (STAGE + (FP4 ? SCALES : 0));
-    static constexpr int A_CH = BM / kChunkRows / NWAVES, B_CH = BN / kChunkRows / NWAVES;  // loads per wave and stage
+    static constexpr int A_CH = BM / kChunkRows / LOADING, B_CH = BN / kChunkRows / LOADING;  // loads per wave and stage
     static constexpr int SLOTS = FM * FN;                         // matrix instructions per step
-    static_assert(BM % (kChunkRows * NWAVES) == 0 && BN % (kChunkRows * NWAVES) == 0 && BM % 64 == 0 && BN % 64 == 0);
+    static_assert(BM % (kChunkRows * LOADING) == 0 && BN % (kChunkRows * LOADING) == 0 && LOADING % 2 == 0 && BM % 64 == 0 && BN % 64 == 0);
 };
 
 // Order of tiles: workgroup ids go round-robin over the 8 XCDs; ids congruent mod 8 get consecutive
@@ -339,7 +341,10 @@ hipError_t fill_rows(void *y, const float *bias, size_t m, size_t n, hipStream_t
 }
 
 // Persistent: a workgroup walks tiles blockIdx.x, + gridDim.x, ... and its loads run ahead of the
-// arithmetic across the ends of tiles.  STAGES stages ring in LDS.  A stage is four steps of FM x FN matrix
+// arithmetic across the ends of tiles.  With the smaller tiles four waves of their own do the loading: a load holds up the
+// wave that issues it, and these tiles have fewer matrix instructions to hide that behind (64 x 128 tiles, four loaders
+// against none: 512 x 4096 x 11008 23.6 us and 26.2; 64 x 4096 x 4096 8.6 and 10.5).  The 256 x 256 tile has no registers left
+// for more waves.  STAGES stages ring in LDS.  A stage is four steps of FM x FN matrix
 // instructions; while a step's instructions run, the next step's operands are read from LDS into the other register
 // set.  Before a stage's last step every read of the stage has been made: there the waves meet, the next stage must
 // have landed (younger ones stay in flight), and the stage's buffer is given to the loads of the stage STAGES further on.
@@ -372,16 +377,18 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
     };
     clear();
 
-    // ---- loads.  Load c of a wave fills LDS rows 8 (c * NWAVES + wave) .. + 7 of its operand's part of a
-    // stage, lane l the 16 bytes at place l % 8 of row l / 8.  The chunk that lies at place p of row r is
+    // ---- loads.  Load c of loading wave l fills LDS rows 8 (c * LOADING + l) .. + 7 of its operand's part of a
+    // stage, each lane the 16 bytes at place lane % 8 of row lane / 8.  The chunk that lies at place p of row r is
     // p ^ (r / 2 % 8): the 16 lanes that an LDS read serves together then touch every bank once.
     const unsigned lds_base = (unsigned)(size_t)I4L_LDS(lds);
-    const int ld_row = wave * kChunkRows + (lane >> 3);
+    const int loader = C::LOADERS ? wave - C::NWAVES : wave;
+    const int ld_row = loader * kChunkRows + (lane >> 3);
     const unsigned ld_chunk = (unsigned)(((lane & 7) ^ ((ld_row >> 1) & 7)) * 16);
-    const uint8_t *a_base = nullptr, *b_base[2] = {};  // this tile's rows, this stage's bytes
+    const uint8_t *a_base = nullptr, *b_base[2] = {};  // this tile's rows, this stage's line
     unsigned a_off[C::A_CH], b_off[C::B_CH];
-    const uint8_t *scale_at = nullptr;  // FP4: this lane's row of scales (wave w moves those of LDS rows 64 w ..)
-    static_assert((C::BM + C::BN) / 64 <= C::NWAVES);
+    // FP4: loads of scales, 64 rows each; a wave's are rows 64 (c * LOADING + l) .. of the stage
+    constexpr int kScaleLoads = (C::BM + C::BN) / 64, kMyScales = (kScaleLoads + C::LOADING - 1) / C::LOADING;
+    const uint8_t *scale_at[kMyScales] = {};
     int ld_it = 0, ld_s = 0;
     unsigned ld_buffer = 0, ld_slot = 0;
 
@@ -398,40 +405,47 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
         const int last_a = o.a_rows - 1 - m0, last_b = o.b_rows - 1 - n0;
 #pragma unroll
         for (int c = 0; c < C::A_CH; ++c)
-            a_off[c] = (unsigned)min(c * C::NWAVES * kChunkRows + ld_row, last_a) * o.stride + ld_chunk;
+            a_off[c] = (unsigned)min(c * C::LOADING * kChunkRows + ld_row, last_a) * o.stride + ld_chunk;
         // (last_b is negative where h's padding alone is in the tile: then the matrix's last row)
         const int nb = min(n0, o.b_rows - 1);
         b_base[0] = uniform(o.b0 + (size_t)nb * o.stride);
         b_base[1] = uniform(o.b1 + (size_t)nb * o.stride);
 #pragma unroll
         for (int c = 0; c < C::B_CH; ++c)
-            b_off[c] = (unsigned)max(min(b_row(c * C::NWAVES * kChunkRows + ld_row), last_b), 0) * o.stride + ld_chunk;
+            b_off[c] = (unsigned)max(min(b_row(c * C::LOADING * kChunkRows + ld_row), last_b), 0) * o.stride + ld_chunk;
         if constexpr (FP4) {
-            const int r = wave * 64 + lane;
-            if (r < C::BM) {
-                scale_at = o.a_scales + (size_t)(m0 + min(r, last_a)) * o.scale_stride;
-            } else {
-                const int br = r - C::BM;
-                scale_at = (b_second(br) ? o.b1_scales : o.b0_scales) + (size_t)(nb + max(min(b_row(br), last_b), 0)) * o.scale_stride;
+#pragma unroll
+            for (int c = 0; c < kMyScales; ++c) {
+                const int r = (c * C::LOADING + loader) * 64 + lane;
+                if (r < C::BM) {
+                    scale_at[c] = o.a_scales + (size_t)(m0 + min(r, last_a)) * o.scale_stride;
+                } else {
+                    const int br = r - C::BM;
+                    scale_at[c] = (b_second(br) ? o.b1_scales : o.b0_scales) + (size_t)(nb + max(min(b_row(br), last_b), 0)) * o.scale_stride;
+                }
             }
         }
     };
     constexpr int kLoads = C::A_CH + C::B_CH;
     auto load = [&](int c) {
-        const unsigned to = lds_base + ld_buffer + (unsigned)wave * 1024u;
+        const unsigned to = lds_base + ld_buffer + (unsigned)loader * 1024u;
         if (c < C::A_CH)
-            dma16(a_base, a_off[c], to + (unsigned)(c * C::NWAVES) * 1024u);
+            dma16(a_base, a_off[c], to + (unsigned)(c * C::LOADING) * 1024u);
         else
-            dma16(b_base[b_second(((c - C::A_CH) * C::NWAVES + wave) * kChunkRows)], b_off[c - C::A_CH],
-                  to + (unsigned)(C::BM * kLineBytes) + (unsigned)((c - C::A_CH) * C::NWAVES) * 1024u);
+            dma16(b_base[b_second(((c - C::A_CH) * C::LOADING + loader) * kChunkRows)], b_off[c - C::A_CH],
+                  to + (unsigned)(C::BM * kLineBytes) + (unsigned)((c - C::A_CH) * C::LOADING) * 1024u);
     };
     auto next_in_ring = [](unsigned at, unsigned step) { return at == (C::STAGES - 1) * step ? 0u : at + step; };
     // After a stage's loads: its scales, if they are not there already, and on to the next stage.  Behind the
     // last stage the cursor stays: it is loaded again, into buffers that nobody reads.
     auto load_rest = [&] {
         if constexpr (FP4) {
-            if (ld_s % kScaleStages == 0 && ((C::BM + C::BN) / 64 == C::NWAVES || wave < (C::BM + C::BN) / 64))
-                dma16(scale_at, lds_base + C::STAGES * C::STAGE + ld_slot + (unsigned)wave * 1024u);
+            if (ld_s % kScaleStages == 0) {
+#pragma unroll
+                for (int c = 0; c < kMyScales; ++c)
+                    if (kScaleLoads % C::LOADING == 0 || c * C::LOADING + loader < kScaleLoads)
+                        dma16(scale_at[c], lds_base + C::STAGES * C::STAGE + ld_slot + (unsigned)(c * C::LOADING + loader) * 1024u);
+            }
         }
         ld_buffer = next_in_ring(ld_buffer, C::STAGE);
         if (ld_s + 1 < stages) {
@@ -440,7 +454,9 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
             b_base[0] += kLineBytes;
             b_base[1] += kLineBytes;
             if (FP4 && ld_s % kScaleStages == 0) {
-                scale_at += 16;
+#pragma unroll
+                for (int c = 0; c < kMyScales; ++c)
+                    scale_at[c] += 16;
                 ld_slot = next_in_ring(ld_slot, C::SCALES);
             }
         } else if (ld_it + 1 < my_tiles) {
@@ -449,14 +465,44 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
             ld_tile(++ld_it);
         }
     };
+    // All but the youngest IN_FLIGHT stages have landed, this wave's reads are done, and every wave is here.  (Loads
+    // complete in order; scales and stores in between only make the wait a little longer.)
+    auto meet = [&](auto in_flight) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(decltype(in_flight)::value * kLoads) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto meet_without_loads = [&] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    static_assert((C::STAGES - 1) * kLoads <= 63);
 
-    ld_tile(0);
+    if (C::LOADERS == 0 || wave >= C::NWAVES) {
+        ld_tile(0);
 #pragma unroll
-    for (int st = 0; st < C::STAGES; ++st) {
+        for (int st = 0; st < C::STAGES; ++st) {
 #pragma unroll
-        for (int c = 0; c < kLoads; ++c)
-            load(c);
-        load_rest();
+            for (int c = 0; c < kLoads; ++c)
+                load(c);
+            load_rest();
+        }
+        meet(std::integral_constant<int, C::STAGES - 1>{});
+        if constexpr (C::LOADERS != 0) {
+            for (int left = my_tiles * stages; left > 0; --left) {
+                meet(std::integral_constant<int, C::STAGES - 2>{});
+#pragma unroll
+                for (int c = 0; c < kLoads; ++c)
+                    load(c);
+                load_rest();
+            }
+            // (loads into buffers that nobody reads may be in flight: they end before the LDS is given away)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            return;
+        }
+    } else {
+        meet_without_loads();
     }
 
     // ---- arithmetic
@@ -522,15 +568,6 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
     constexpr int kReadsPerSlot = (kReads + C::SLOTS - 1) / C::SLOTS;
     constexpr int kLoadsPerSlot = (kLoads + C::SLOTS - 1) / C::SLOTS;
 
-    // All but the youngest IN_FLIGHT stages have landed, this wave's reads are done, and every wave is here.  (Loads
-    // complete in order; scales and stores in between only make the wait a little longer.)
-    auto meet = [&](auto in_flight) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(decltype(in_flight)::value * kLoads) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    static_assert((C::STAGES - 1) * kLoads <= 63);
-    meet(std::integral_constant<int, C::STAGES - 1>{});
 #pragma unroll
     for (int r = 0; r < kReads; ++r)
         read(0, 0, 0, r);
@@ -557,7 +594,10 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
                   }),
              ...);
         }(std::make_integer_sequence<int, kSteps - 1>{});
-        meet(std::integral_constant<int, C::STAGES - 2>{});
+        if constexpr (C::LOADERS == 0)
+            meet(std::integral_constant<int, C::STAGES - 2>{});
+        else
+            meet_without_loads();
         const bool last = s + 1 == stages;
         const int next_s = last ? 0 : s + 1;
         if (FP4 && next_s % kScaleStages == 0)
@@ -569,11 +609,14 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
 #pragma unroll
             for (int r = at; r < at + kReadsPerSlot && r < kReads; ++r)
                 read(next_buffer, 0, 0, r);
+            if constexpr (C::LOADERS == 0) {
 #pragma unroll
-            for (int c = load_at; c < load_at + kLoadsPerSlot && c < kLoads; ++c)
-                load(c);
+                for (int c = load_at; c < load_at + kLoadsPerSlot && c < kLoads; ++c)
+                    load(c);
+            }
         });
-        load_rest();
+        if constexpr (C::LOADERS == 0)
+            load_rest();
         buffer = next_buffer;
         s = next_s;
         if (last) {
@@ -586,10 +629,10 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-using Tile256 = LineTile<4, 2, 2, 4, 2, 2>;
-using Tile128 = LineTile<2, 2, 2, 2, 2, 2>;
-using Tile64x128 = LineTile<2, 2, 1, 2, 3, 2>;
-using Tile64 = LineTile<2, 2, 1, 1, 4, 2>;  // (too narrow for pairs of blocks)
+using Tile256 = LineTile<4, 2, 2, 4, 0, 2, 2>;
+using Tile128 = LineTile<2, 2, 2, 2, 4, 2, 4>;
+using Tile64x128 = LineTile<2, 2, 1, 2, 4, 3, 4>;
+using Tile64 = LineTile<2, 2, 1, 1, 4, 4, 4>;  // (too narrow for pairs of blocks)
 
 // Workgroups of a tile that a CU's LDS holds.
 template <class C, bool FP4>
@@ -605,26 +648,35 @@ hipError_t launch_tile(const LineOperands &o, int batch, int n, const Ep &ep, co
     return hipGetLastError();
 }
 
-// What a tile costs, in units of 10 ns: a stage on a CU that is busy with such tiles, and what a launch spends
-// before its first and after its last.  Read off products that fill the device (8192^3 in 283, 343, 520 and 573 us) and
-// ones of a few stages (1024^3 in 11.8, 6.3, 5.4, 4.9 us; 130 x 1001 x 515 in 21.3, 11.7, 7.9, 5.7 us).
+// What a tile costs, in units of 10 ns: a stage of each, where every CU is busy with such tiles (`full`) and where there
+// are few (`few`: nothing hides the way to memory), and what a launch spends before its first stage and after its
+// last.  Read off the products below, products that fill the device (8192^3: 283, 342, 461 us, 64 x 64 about 600) and short ones
+// (1024^3: 11.7, 5.9, 5.2, 4.8 us).
 struct TileCost {
-    int m, n, stage, fixed;
+    int m, n, per_cu, full, few, fixed;
 };
-constexpr TileCost kTiles[] = {{256, 256, 175, 1100}, {128, 128, 65, 650}, {64, 128, 50, 550}, {64, 64, 28, 500}};
+constexpr TileCost kTiles[] = {{256, 256, per_cu<Tile256, true>, 175, 175, 1100},
+                               {128, 128, per_cu<Tile128, true>, 62, 70, 600},
+                               {64, 128, per_cu<Tile64x128, true>, 46, 45, 380},
+                               {64, 64, per_cu<Tile64, true>, 29, 29, 330}};
 
-// The tile that such costs make the quickest for a product of m x n (columns of b) in `stages` stages.  It was the quickest or
-// within a tenth of it at 512 x 4096 x 11008 (us by size: 64, 33.6, 27.0, 30.5), 333 x 11008 x 4999 (36.5, 23.8, 35.2, 34.0),
-// 2048 x 4096 x 4096 (33, 26, 41, 49), 128 x 14336 x 4096 (26.0, 14.9, 12.0, 13.6) and 64 x 4096 x 4096 (23.3, 12.8, 10.8, 9.4).
+// The tile that makes a product of m x n (columns of b) in `stages` stages quickest by these costs.  Measured, us by tile:
+//   512 x 4096 x 11008   64, 32.9, 23.6, 29.8        333 x 11008 x 4999   36, 21.2, 27.8, 27.1
+//   2048 x 4096 x 4096   33, 25.6, 34.5, 44.7        128 x 14336 x 4096   26, 14.4, 10.3, 12.3
+//   64 x 4096 x 4096     23, 10.1, 8.6, 7.5          200 x 4096 x 14336   -, 37.7, 24.1, 20.4
 int quickest_tile(long m, long n, int batch, int stages, bool pair, const DeviceInfo &dev)
 {
+    const long cus = dev.cu_count > 0 ? dev.cu_count : 256;
     int best = 0;
     double least = 0;
     for (int i = 0; i < 3 + !pair; ++i) {
         const TileCost &t = kTiles[i];
         const long tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n) * batch;
-        const long turns = (tiles + dev.cu_count - 1) / (dev.cu_count > 0 ? dev.cu_count : 1);
-        const double cost = (double)turns * stages * t.stage + t.fixed;
+        const long places = cus * t.per_cu, rounds = tiles / places, rest = tiles % places;
+        double stage = (double)rounds * t.per_cu * t.full;
+        if (rest)
+            stage += max((double)t.few, (double)rest / cus * t.full);
+        const double cost = stage * stages + t.fixed;
         if (i == 0 || cost < least) {
             best = i;
             least = cost;
