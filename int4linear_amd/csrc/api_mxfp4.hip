@@ -232,20 +232,33 @@ int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, co
     const int st = api_begin(stream, &info);
     if (st != INT4LINEAR_OK)
         return st;
-    const uint16_t *dy = (const uint16_t *)dy_d;
     const bool ragged = n % 64 != 0;
-    hipError_t e = hipSuccess;
-    if (n > 0 && (want_dw || want_sums || (want_dx && ragged)))
-        e = launch_bf16_transpose(dy, m, n, want_dw ? p.dy_t : nullptr, p.ld_m, want_dx && ragged ? p.dy_padded : nullptr, p.ld_n,
-                                  want_sums ? dbias_d : nullptr, p.sums, stream);
-    if (e == hipSuccess && want_dw && m > 0)
-        e = launch_mx_dequantize_transposed(matrix(x_codes_d, x_scales_d, m), p.x_t, p.ld_m, k, stream);
-    if (e == hipSuccess && want_dw)
-        e = launch_bf16_gemm(p.dy_t, n, p.x_t, k, p.ld_m, m, dw_d, dw_d, 1, dw_type, info, stream);
-    if (e == hipSuccess && want_dx && n > 0)
-        e = launch_mx_dequantize_transposed(matrix(w_codes_d, w_scales_d, n), p.w_t, p.ld_n, k, stream);
-    if (e == hipSuccess && want_dx)
-        e = launch_bf16_gemm(ragged ? p.dy_padded : dy, m, p.w_t, k, p.ld_n, n, dx_d, dx_d, 1, kOutBF16, info, stream);
+    Prepared prepared{};
+    prepared.k = k;
+    if (want_dw && m > 0)
+        prepared.matrix[prepared.matrices++] = {matrix(x_codes_d, x_scales_d, m), p.x_t, p.ld_m};
+    if (want_dx && n > 0)
+        prepared.matrix[prepared.matrices++] = {matrix(w_codes_d, w_scales_d, n), p.w_t, p.ld_n};
+    if (m > 0 && n > 0 && (want_dw || want_sums || ragged)) {
+        prepared.dy = (const uint16_t *)dy_d;
+        prepared.rows = m;
+        prepared.cols = n;
+        prepared.transposed = want_dw ? p.dy_t : nullptr;
+        prepared.ld_t = p.ld_m;
+        prepared.padded = want_dx && ragged ? p.dy_padded : nullptr;
+        prepared.ld_p = p.ld_n;
+        prepared.partial = want_sums ? p.sums : nullptr;
+    }
+    hipError_t e = launch_prepare(prepared, stream);
+    Bf16Product products[2];
+    int count = 0;
+    if (want_dw)
+        products[count++] = {p.dy_t, n, p.x_t, k, p.ld_m, m, dw_d, dw_type};
+    if (want_dx)
+        products[count++] = {ragged ? p.dy_padded : (const uint16_t *)dy_d, m, p.w_t, k, p.ld_n, n, dx_d, kOutBF16};
+    const ColumnSums sums{want_sums ? dbias_d : nullptr, p.sums, (int)(p.ld_m / 64), n};
+    if (e == hipSuccess)
+        e = launch_bf16_products(products, count, sums, info, stream);
     return api_status(e);
 }
 
@@ -284,18 +297,27 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
     if (m > 0 && n > 0)
         e = launch_mx_gated_gradients(x, wg, wu, (Activation)activation, (const uint16_t *)dh_d, p.d, p.ld_n, p.d_t, p.ld_m, k, info,
                                       stream);
-    if (e == hipSuccess && want_dw && m > 0)
-        e = launch_mx_dequantize_transposed(x, p.x_t, p.ld_m, k, stream);
-    if (e == hipSuccess && want_dw)
-        e = launch_bf16_gemm(p.d_t, n, p.x_t, k, p.ld_m, m, dwg_d, dwu_d, 2, dw_type, info, stream);
     // wg and wu side by side: row c of w_t is column c of wg, then column c of wu
-    if (e == hipSuccess && want_dx && n > 0)
-        e = launch_mx_dequantize_transposed(wg, p.w_t, 2 * p.ld_n, k, stream);
-    if (e == hipSuccess && want_dx && n > 0)
-        e = launch_mx_dequantize_transposed(wu, p.w_t + p.ld_n, 2 * p.ld_n, k, stream);
-    if (e == hipSuccess && want_dx)
-        e = launch_bf16_gemm(p.d, m, p.w_t, k, 2 * p.ld_n, (int)(n > 0 ? 2 * p.ld_n : 0), dx_d, dx_d, 1, kOutBF16, info,
-                             stream);
+    Prepared prepared{};
+    prepared.k = k;
+    if (want_dw && m > 0)
+        prepared.matrix[prepared.matrices++] = {x, p.x_t, p.ld_m};
+    if (want_dx && n > 0) {
+        prepared.matrix[prepared.matrices++] = {wg, p.w_t, 2 * p.ld_n};
+        prepared.matrix[prepared.matrices++] = {wu, p.w_t + p.ld_n, 2 * p.ld_n};
+    }
+    if (e == hipSuccess)
+        e = launch_prepare(prepared, stream);
+    Bf16Product products[3];
+    int count = 0;
+    if (want_dw) {
+        products[count++] = {p.d_t, n, p.x_t, k, p.ld_m, m, dwg_d, dw_type};
+        products[count++] = {p.d_t + (size_t)n * p.ld_m, n, p.x_t, k, p.ld_m, m, dwu_d, dw_type};
+    }
+    if (want_dx)
+        products[count++] = {p.d, m, p.w_t, k, 2 * p.ld_n, (int)(n > 0 ? 2 * p.ld_n : 0), dx_d, kOutBF16};
+    if (e == hipSuccess)
+        e = launch_bf16_products(products, count, ColumnSums{}, info, stream);
     return api_status(e);
 }
 

@@ -32,7 +32,6 @@ constexpr int kFrag = 32;
 struct LineOperands {
     const uint8_t *a, *b0, *b1;
     const uint8_t *a_scales, *b0_scales, *b1_scales;
-    size_t a_batch;  // bytes from the matrix a of blockIdx.z to the next
     unsigned stride, scale_stride;
     int a_rows, b_rows, stages;
 };
@@ -102,7 +101,7 @@ __device__ __forceinline__ void store_block(void *y, size_t ld, int m, int n, in
 template <int OUT, bool COLUMNS>
 struct PlainEpilogue {
     static constexpr bool kPair = false, kColumns = COLUMNS;
-    void *y0, *y1;  // by blockIdx.z
+    void *y;
     const float *bias;
     size_t ld;
     int m, n;
@@ -110,7 +109,6 @@ struct PlainEpilogue {
     template <int FM, int FN>
     __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
-        void *dst = blockIdx.z ? y1 : y0;
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
             const int c = col + kFrag * i;
@@ -136,7 +134,7 @@ struct PlainEpilogue {
 #pragma unroll
                 for (int t = 0; t < 16; ++t)
                     v[t] = acc[j][i][t] + add[t];
-                store_block<OUT, COLUMNS>(dst, ld, m, n, row + kFrag * j, c, lane, v);
+                store_block<OUT, COLUMNS>(y, ld, m, n, row + kFrag * j, c, lane, v);
             }
         }
     }
@@ -340,7 +338,7 @@ hipError_t fill_rows(void *y, const float *bias, size_t m, size_t n, hipStream_t
     return hipGetLastError();
 }
 
-// Persistent: a workgroup walks tiles blockIdx.x, + gridDim.x, ... and its loads run ahead of the
+// Persistent: a workgroup walks tiles first, first + by, ... and its loads run ahead of the
 // arithmetic across the ends of tiles.  With the smaller tiles four waves of their own do the loading: a load holds up the
 // wave that issues it, and these tiles have fewer matrix instructions to hide that behind (64 x 128 tiles, four loaders
 // against none: 512 x 4096 x 11008 23.6 us and 26.2; 64 x 4096 x 4096 8.6 and 10.5).  The 256 x 256 tile has no registers left
@@ -349,15 +347,15 @@ hipError_t fill_rows(void *y, const float *bias, size_t m, size_t n, hipStream_t
 // set.  Before a stage's last step every read of the stage has been made: there the waves meet, the next stage must
 // have landed (younger ones stay in flight), and the stage's buffer is given to the loads of the stage STAGES further on.
 template <bool FP4, class C, class Ep>
-__global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOperands o, int tiles_m, int tiles_n, Ep ep)
+__device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, int tiles_n, const Ep &ep, int first, int by)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / C::WAVES_N, wn = wave % C::WAVES_N;
     const int total = tiles_m * tiles_n;
-    const int my_tiles = (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
-    const uint8_t *a_data = o.a + blockIdx.z * o.a_batch;
+    const int my_tiles = (total - first + by - 1) / by;
+    const uint8_t *a_data = o.a;
     const int stages = o.stages;
     constexpr int kTileN = Ep::kPair ? C::BN / 2 : C::BN;  // columns of y
 
@@ -371,7 +369,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
     };
     auto finish = [&](int it) {
         int tm, tn;
-        tile_coords(blockIdx.x + it * gridDim.x, total, tiles_m, tiles_n, tm, tn);
+        tile_coords(first + it * by, total, tiles_m, tiles_n, tm, tn);
         ep(acc, tm * C::BM + wm * C::FM * kFrag, tn * kTileN + wn * C::FN * kFrag / (Ep::kPair ? 2 : 1), lane);
         clear();
     };
@@ -398,7 +396,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
 
     auto ld_tile = [&](int it) {
         int tm, tn;
-        tile_coords(blockIdx.x + it * gridDim.x, total, tiles_m, tiles_n, tm, tn);
+        tile_coords(first + it * by, total, tiles_m, tiles_n, tm, tn);
         const int m0 = tm * C::BM, n0 = tn * kTileN;
         a_base = uniform(a_data + (size_t)m0 * o.stride);
         // rows behind the matrix: the last one again
@@ -629,6 +627,55 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+template <bool FP4, class C, class Ep>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOperands o, int tiles_m, int tiles_n, Ep ep)
+{
+    line_gemm<FP4, C>(o, tiles_m, tiles_n, ep, blockIdx.x, gridDim.x);
+}
+
+// Up to three products in one launch, a tile per workgroup: those of a small layer's backward pass, each of which would leave
+// most CUs idle, by blockIdx.z.  The last one is dx; the others, the weights', share a type.
+struct LineGroup {
+    LineOperands o[3];
+    int tiles_m[3], tiles_n[3];
+    void *y[3];
+    int count;
+    // Column sums to be completed on the way (sums null: none): of `parts` rows of partial sums.
+    float *sums;
+    const float *partial;
+    int parts, columns;
+};
+
+__device__ __forceinline__ void complete_sums(float *sums, const float *partial, int parts, int columns, int first, int by)
+{
+    for (int c = first; c < columns; c += by) {
+        float sum = 0.0f;
+        for (int i = 0; i < parts; ++i)
+            sum += partial[(size_t)i * columns + c];
+        sums[c] = sum;
+    }
+}
+
+template <class C, class EpW, class EpX>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void line_group_kernel(LineGroup g, EpW ep_w, EpX ep_x)
+{
+    const int z = blockIdx.z;
+    if (g.sums && z == 0)
+        complete_sums(g.sums, g.partial, g.parts, g.columns, blockIdx.x * C::THREADS + threadIdx.x, gridDim.x * C::THREADS);
+    const int tiles = g.tiles_m[z] * g.tiles_n[z];
+    if ((int)blockIdx.x >= tiles)
+        return;
+    auto run = [&](auto ep) {
+        ep.y = g.y[z];
+        ep.m = g.o[z].a_rows;
+        line_gemm<false, C>(g.o[z], g.tiles_m[z], g.tiles_n[z], ep, blockIdx.x, tiles);
+    };
+    if (z == g.count - 1)
+        run(ep_x);
+    else
+        run(ep_w);
+}
+
 using Tile256 = LineTile<4, 2, 2, 4, 0, 2, 2>;
 using Tile128 = LineTile<2, 2, 2, 2, 4, 2, 4>;
 using Tile64x128 = LineTile<2, 2, 1, 2, 4, 3, 4>;
@@ -639,12 +686,12 @@ template <class C, bool FP4>
 constexpr int per_cu = 160 * 1024 / C::template LDS<FP4>;
 
 template <bool FP4, class C, class Ep>
-hipError_t launch_tile(const LineOperands &o, int batch, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
+hipError_t launch_tile(const LineOperands &o, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
     const int bn = Ep::kPair ? C::BN / 2 : C::BN;
     const int tiles_m = (o.a_rows + C::BM - 1) / C::BM, tiles_n = (n + bn - 1) / bn;
-    const int groups = min(tiles_m * tiles_n, max(1, dev.cu_count * per_cu<C, FP4> / batch));
-    line_gemm_kernel<FP4, C, Ep><<<dim3((unsigned)groups, 1, (unsigned)batch), C::THREADS, C::template LDS<FP4>, stream>>>(o, tiles_m, tiles_n, ep);
+    const int groups = min(tiles_m * tiles_n, max(1, dev.cu_count * per_cu<C, FP4>));
+    line_gemm_kernel<FP4, C, Ep><<<groups, C::THREADS, C::template LDS<FP4>, stream>>>(o, tiles_m, tiles_n, ep);
     return hipGetLastError();
 }
 
@@ -664,14 +711,14 @@ constexpr TileCost kTiles[] = {{256, 256, per_cu<Tile256, true>, 175, 175, 1100}
 //   512 x 4096 x 11008   64, 32.9, 23.6, 29.8        333 x 11008 x 4999   36, 21.2, 27.8, 27.1
 //   2048 x 4096 x 4096   33, 25.6, 34.5, 44.7        128 x 14336 x 4096   26, 14.4, 10.3, 12.3
 //   64 x 4096 x 4096     23, 10.1, 8.6, 7.5          200 x 4096 x 14336   -, 37.7, 24.1, 20.4
-int quickest_tile(long m, long n, int batch, int stages, bool pair, const DeviceInfo &dev)
+int quickest_tile(long m, long n, int stages, bool pair, const DeviceInfo &dev)
 {
     const long cus = dev.cu_count > 0 ? dev.cu_count : 256;
     int best = 0;
     double least = 0;
     for (int i = 0; i < 3 + !pair; ++i) {
         const TileCost &t = kTiles[i];
-        const long tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n) * batch;
+        const long tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
         const long places = cus * t.per_cu, rounds = tiles / places, rest = tiles % places;
         double stage = (double)rounds * t.per_cu * t.full;
         if (rest)
@@ -687,26 +734,26 @@ int quickest_tile(long m, long n, int batch, int stages, bool pair, const Device
 
 // n: columns of the product that have to be covered.
 template <bool FP4, class Ep>
-hipError_t launch(const LineOperands &o, int batch, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
+hipError_t launch(const LineOperands &o, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
-    switch (quickest_tile(o.a_rows, (long)n * (Ep::kPair ? 2 : 1), batch, o.stages, Ep::kPair, dev)) {
+    switch (quickest_tile(o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev)) {
     case 0:
-        return launch_tile<FP4, Tile256>(o, batch, n, ep, dev, stream);
+        return launch_tile<FP4, Tile256>(o, n, ep, dev, stream);
     case 1:
-        return launch_tile<FP4, Tile128>(o, batch, n, ep, dev, stream);
+        return launch_tile<FP4, Tile128>(o, n, ep, dev, stream);
     case 2:
-        return launch_tile<FP4, Tile64x128>(o, batch, n, ep, dev, stream);
+        return launch_tile<FP4, Tile64x128>(o, n, ep, dev, stream);
     default:
         if constexpr (Ep::kPair)
             return hipErrorInvalidValue;
         else
-            return launch_tile<FP4, Tile64>(o, batch, n, ep, dev, stream);
+            return launch_tile<FP4, Tile64>(o, n, ep, dev, stream);
     }
 }
 
 LineOperands operands(const MxMatrix &x, const MxMatrix &w0, const MxMatrix &w1, int k)
 {
-    return {x.codes, w0.codes, w1.codes, x.scales, w0.scales, w1.scales, 0, (unsigned)mx_code_stride(k), (unsigned)mx_scale_stride(k),
+    return {x.codes, w0.codes, w1.codes, x.scales, w0.scales, w1.scales, (unsigned)mx_code_stride(k), (unsigned)mx_scale_stride(k),
             x.rows, w0.rows, (k + kLineFp4 - 1) / kLineFp4};
 }
 
@@ -743,9 +790,23 @@ static hipError_t allow_lds()
     return e;
 }
 
+template <class EpW, class EpX>
+static hipError_t allow_group_lds()
+{
+    return hipFuncSetAttribute((const void *)line_group_kernel<Tile64, EpW, EpX>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                               Tile64::LDS<false>);
+}
+
 hipError_t line_gemm_init(const DeviceInfo &)
 {
     hipError_t e = hipSuccess;
+    using Columns32 = PlainEpilogue<kOutF32, true>;
+    using Columns16 = PlainEpilogue<kOutBF16, true>;
+    using Rows16 = PlainEpilogue<kOutBF16, false>;
+    for (auto allow : {allow_group_lds<Columns32, Columns16>, allow_group_lds<Columns32, Rows16>, allow_group_lds<Columns16, Columns16>,
+                       allow_group_lds<Rows16, Rows16>})
+        if (e == hipSuccess)
+            e = allow();
     for (auto allow : {allow_lds<true, PlainEpilogue<kOutF32, true>>, allow_lds<true, PlainEpilogue<kOutF16, true>>,
                        allow_lds<true, PlainEpilogue<kOutF16, false>>, allow_lds<true, PlainEpilogue<kOutBF16, true>>,
                        allow_lds<true, PlainEpilogue<kOutBF16, false>>, allow_lds<true, GatedEpilogue<kOutF32, true>>,
@@ -768,8 +829,8 @@ hipError_t launch_mx_linear(const MxMatrix &x, const MxMatrix &w, const float *b
         constexpr int OUT = decltype(type)::value;
         if (k == 0)
             return fill_rows<OUT>(y, bias, (size_t)x.rows, (size_t)w.rows, stream);
-        const PlainEpilogue<OUT, decltype(columns)::value> ep{y, nullptr, bias, (size_t)w.rows, x.rows, w.rows};
-        return launch<true>(operands(x, w, w, k), 1, w.rows, ep, dev, stream);
+        const PlainEpilogue<OUT, decltype(columns)::value> ep{y, bias, (size_t)w.rows, x.rows, w.rows};
+        return launch<true>(operands(x, w, w, k), w.rows, ep, dev, stream);
     });
 }
 
@@ -783,7 +844,7 @@ hipError_t launch_mx_gated(const MxMatrix &x, const MxMatrix &wg, const MxMatrix
         if (k == 0)
             return fill_rows<OUT>(h, nullptr, (size_t)x.rows, (size_t)wg.rows, stream);
         const GatedEpilogue<OUT, decltype(columns)::value> ep{h, (size_t)wg.rows, x.rows, wg.rows, act};
-        return launch<true>(operands(x, wg, wu, k), 1, wg.rows, ep, dev, stream);
+        return launch<true>(operands(x, wg, wu, k), wg.rows, ep, dev, stream);
     });
 }
 
@@ -799,7 +860,7 @@ hipError_t launch_mx_gated_quantized(const MxMatrix &x, const MxMatrix &wg, cons
         return launch_mx_gated_quantized_skinny(x, wg, wu, act, codes, scales, k, stream);
     const GatedMxEpilogue ep{codes, scales, mx_code_stride(n), mx_scale_stride(n), x.rows, n, act};
     // (the grid covers the padding at the end of h's rows)
-    return launch<true>(operands(x, wg, wu, k), 1, (int)(mx_code_stride(n) * 2), ep, dev, stream);
+    return launch<true>(operands(x, wg, wu, k), (int)(mx_code_stride(n) * 2), ep, dev, stream);
 }
 
 hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
@@ -807,28 +868,78 @@ hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, cons
                                      hipStream_t stream)
 {
     const GradientEpilogue ep{(const __bf16 *)dh, (__bf16 *)d, (__bf16 *)dt, ld_n, ld_m, x.rows, wg.rows, act, wg.rows % 4 == 0};
-    return launch<true>(operands(x, wg, wu, k), 1, wg.rows, ep, dev, stream);
+    return launch<true>(operands(x, wg, wu, k), wg.rows, ep, dev, stream);
 }
 
-hipError_t launch_bf16_gemm(const uint16_t *a, int m, const uint16_t *b, int n, size_t ld, int k, void *y0, void *y1, int batch,
-                            int out, const DeviceInfo &dev, hipStream_t stream)
+static LineOperands operands(const Bf16Product &p)
 {
-    const LineOperands o{(const uint8_t *)a, (const uint8_t *)b, (const uint8_t *)b, nullptr, nullptr, nullptr, (size_t)m * ld * 2,
-                         (unsigned)(ld * 2), 0, m, n, (k + kLineBf16 - 1) / kLineBf16};
-    auto run = [&](auto type, auto columns) {
-        constexpr int OUT = decltype(type)::value;
-        if (k == 0) {
-            hipError_t e = hipSuccess;
-            for (int z = 0; z < batch && e == hipSuccess; ++z)
-                e = fill_rows<OUT>(z ? y1 : y0, nullptr, (size_t)m, (size_t)n, stream);
-            return e;
-        }
-        const PlainEpilogue<OUT, decltype(columns)::value> ep{y0, y1, nullptr, (size_t)n, m, n};
-        return launch<false>(o, batch, n, ep, dev, stream);
-    };
-    if (out == kOutF32)
-        return run(std::integral_constant<int, kOutF32>{}, std::true_type{});
-    return n % 8 ? run(std::integral_constant<int, kOutBF16>{}, std::true_type{}) : run(std::integral_constant<int, kOutBF16>{}, std::false_type{});
+    return {(const uint8_t *)p.a, (const uint8_t *)p.b, (const uint8_t *)p.b, nullptr, nullptr, nullptr, (unsigned)(p.ld * 2), 0, p.m, p.n,
+            (p.k + kLineBf16 - 1) / kLineBf16};
+}
+
+template <int OUT, bool COLUMNS>
+static PlainEpilogue<OUT, COLUMNS> epilogue(const Bf16Product &p)
+{
+    return {p.y, nullptr, (size_t)p.n, p.m, p.n};
+}
+
+// One product by itself.
+static hipError_t launch_bf16(const Bf16Product &p, const DeviceInfo &dev, hipStream_t stream)
+{
+    if (p.k == 0)
+        return p.out == kOutF32 ? fill_rows<kOutF32>(p.y, nullptr, (size_t)p.m, (size_t)p.n, stream)
+                                : fill_rows<kOutBF16>(p.y, nullptr, (size_t)p.m, (size_t)p.n, stream);
+    if (p.out == kOutF32)
+        return launch<false>(operands(p), p.n, epilogue<kOutF32, true>(p), dev, stream);
+    return p.n % 8 ? launch<false>(operands(p), p.n, epilogue<kOutBF16, true>(p), dev, stream)
+                   : launch<false>(operands(p), p.n, epilogue<kOutBF16, false>(p), dev, stream);
+}
+
+template <class C, class EpW, class EpX>
+static hipError_t launch_group(LineGroup g, const EpW &ep_w, const EpX &ep_x, hipStream_t stream)
+{
+    int most = 1;
+    for (int i = 0; i < g.count; ++i) {
+        g.tiles_m[i] = (g.o[i].a_rows + C::BM - 1) / C::BM;
+        g.tiles_n[i] = (g.o[i].b_rows + C::BN - 1) / C::BN;
+        most = max(most, g.tiles_m[i] * g.tiles_n[i]);
+    }
+    line_group_kernel<C, EpW, EpX><<<dim3((unsigned)most, 1, (unsigned)g.count), C::THREADS, C::template LDS<false>, stream>>>(g, ep_w, ep_x);
+    return hipGetLastError();
+}
+
+hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const DeviceInfo &dev, hipStream_t stream)
+{
+    // Together where two rounds of workgroups hold all tiles of 64 x 64: beyond that each fills the device alone, on larger
+    // tiles.  (257 x 1400 x 1000, gated: one launch 19 us, three 34; 130 x 1001 x 515, linear: 14 and 21.)
+    long tiles = 0;
+    bool together = count > 1 && p[count - 1].out == kOutBF16;
+    for (int i = 0; i < count; ++i) {
+        tiles += ((p[i].m + 63l) / 64) * ((p[i].n + 63l) / 64);
+        together = together && p[i].k > 0 && p[i].n == p[0].n && (i == count - 1 || p[i].out == p[0].out);
+    }
+    if (!together || tiles > 4l * dev.cu_count) {
+        hipError_t e = hipSuccess;
+        for (int i = 0; i < count && e == hipSuccess; ++i)
+            e = launch_bf16(p[i], dev, stream);
+        return e == hipSuccess && sums.sums ? launch_column_sums(sums, stream) : e;
+    }
+    LineGroup g{};
+    g.count = count;
+    for (int i = 0; i < count; ++i) {
+        g.o[i] = operands(p[i]);
+        g.y[i] = p[i].y;
+    }
+    g.sums = sums.sums;
+    g.partial = sums.partial;
+    g.parts = sums.parts;
+    g.columns = sums.columns;
+    const Bf16Product &w = p[0], &x = p[count - 1];
+    if (w.out == kOutF32)
+        return x.n % 8 ? launch_group<Tile64>(g, epilogue<kOutF32, true>(w), epilogue<kOutBF16, true>(x), stream)
+                       : launch_group<Tile64>(g, epilogue<kOutF32, true>(w), epilogue<kOutBF16, false>(x), stream);
+    return x.n % 8 ? launch_group<Tile64>(g, epilogue<kOutBF16, true>(w), epilogue<kOutBF16, true>(x), stream)
+                   : launch_group<Tile64>(g, epilogue<kOutBF16, false>(w), epilogue<kOutBF16, false>(x), stream);
 }
 
 }  // namespace int4linear

@@ -184,91 +184,101 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const uint8_t *
 constexpr int kTile = 64;
 constexpr int kTileStride = kTile + 2;  // elements between rows in LDS: an odd number of words
 
-__global__ __launch_bounds__(kThreads) void mx_dequantize_transposed_kernel(const uint8_t *__restrict__ codes,
-                                                                            const uint8_t *__restrict__ scales, int rows, int k,
-                                                                            size_t code_stride, size_t scale_stride,
-                                                                            uint16_t *__restrict__ dst, size_t ld)
+__device__ __forceinline__ void transpose_matrix(uint16_t *tile, const Transposed &t, int k, size_t code_stride, size_t scale_stride)
 {
-    __shared__ uint16_t tile[kTile * kTileStride];
     const int r0 = blockIdx.x * kTile, c0 = blockIdx.y * kTile;
+    if (r0 >= t.q.rows || c0 >= k)
+        return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int t = threadIdx.x + h * kThreads;
-        const int r = t >> 3, c = (t & 7) * 8;
+        const int i = threadIdx.x + h * kThreads;
+        const int r = i >> 3, c = (i & 7) * 8;
         float v[8] = {};
-        if (r0 + r < rows)
-            decode8(*(const unsigned *)(codes + (size_t)(r0 + r) * code_stride + (c0 + c) / 2),
-                    scales[(size_t)(r0 + r) * scale_stride + (c0 + c) / kMxBlock], v);
+        if (r0 + r < t.q.rows)
+            decode8(*(const unsigned *)(t.q.codes + (size_t)(r0 + r) * code_stride + (c0 + c) / 2),
+                    t.q.scales[(size_t)(r0 + r) * scale_stride + (c0 + c) / kMxBlock], v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            tile[(c + i) * kTileStride + r] = __builtin_bit_cast(uint16_t, (__bf16)v[i]);
+        for (int e = 0; e < 8; ++e)
+            tile[(c + e) * kTileStride + r] = __builtin_bit_cast(uint16_t, (__bf16)v[e]);
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int t = threadIdx.x + h * kThreads;
-        const int c = t >> 3, r = (t & 7) * 8;
+        const int i = threadIdx.x + h * kThreads;
+        const int c = i >> 3, r = (i & 7) * 8;
         if (c0 + c >= k)
             continue;
         v8us out;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            out[i] = tile[c * kTileStride + r + i];
-        *(v8us *)(dst + (size_t)(c0 + c) * ld + r0 + r) = out;
+        for (int e = 0; e < 8; ++e)
+            out[e] = tile[c * kTileStride + r + e];
+        *(v8us *)(t.dst + (size_t)(c0 + c) * t.ld + r0 + r) = out;
     }
 }
 
-__global__ __launch_bounds__(kThreads) void bf16_transpose_kernel(const uint16_t *__restrict__ src, int rows, int cols,
-                                                                  uint16_t *__restrict__ transposed, size_t ld_t,
-                                                                  uint16_t *__restrict__ padded, size_t ld_p,
-                                                                  float *__restrict__ partial)
+__device__ __forceinline__ void transpose_dy(uint16_t *tile, const Prepared &p)
 {
-    __shared__ uint16_t tile[kTile * kTileStride];
     const int r0 = blockIdx.x * kTile, c0 = blockIdx.y * kTile;
+    if (r0 >= p.rows || c0 >= p.cols)
+        return;
 #pragma unroll
     for (int h = 0; h < kTile * kTile / kThreads; ++h) {
-        const int t = threadIdx.x + h * kThreads;
-        const int r = t >> 6, c = t & 63;
-        const uint16_t v = r0 + r < rows && c0 + c < cols ? src[(size_t)(r0 + r) * cols + c0 + c] : (uint16_t)0;
+        const int i = threadIdx.x + h * kThreads;
+        const int r = i >> 6, c = i & 63;
+        const uint16_t v = r0 + r < p.rows && c0 + c < p.cols ? p.dy[(size_t)(r0 + r) * p.cols + c0 + c] : (uint16_t)0;
         tile[c * kTileStride + r] = v;
-        if (padded && r0 + r < rows && (size_t)(c0 + c) < ld_p)
-            padded[(size_t)(r0 + r) * ld_p + c0 + c] = v;
+        if (p.padded && r0 + r < p.rows && (size_t)(c0 + c) < p.ld_p)
+            p.padded[(size_t)(r0 + r) * p.ld_p + c0 + c] = v;
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int t = threadIdx.x + h * kThreads;
-        const int c = t >> 3, r = (t & 7) * 8;
+        const int i = threadIdx.x + h * kThreads;
+        const int c = i >> 3, r = (i & 7) * 8;
         v8us out;
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            out[i] = tile[c * kTileStride + r + i];
-            sum += __builtin_bit_cast(float, (unsigned)out[i] << 16);
+        for (int e = 0; e < 8; ++e) {
+            out[e] = tile[c * kTileStride + r + e];
+            sum += __builtin_bit_cast(float, (unsigned)out[e] << 16);
         }
-        if (transposed && c0 + c < cols)
-            *(v8us *)(transposed + (size_t)(c0 + c) * ld_t + r0 + r) = out;
-        if (partial) {
+        if (p.transposed && c0 + c < p.cols)
+            *(v8us *)(p.transposed + (size_t)(c0 + c) * p.ld_t + r0 + r) = out;
+        if (p.partial) {
 #pragma unroll
             for (int s = 1; s < 8; s *= 2)
                 sum += __shfl_xor(sum, s);
-            if ((t & 7) == 0 && c0 + c < cols)
-                partial[(size_t)blockIdx.x * cols + c0 + c] = sum;
+            if ((i & 7) == 0 && c0 + c < p.cols)
+                p.partial[(size_t)blockIdx.x * p.cols + c0 + c] = sum;
         }
     }
 }
 
-// sums[c] = the column's partial sums, added in order of their rows.
-__global__ __launch_bounds__(kThreads) void column_sums_kernel(const float *__restrict__ partial, int count, int cols,
-                                                               float *__restrict__ sums)
+// blockIdx.z: one of the matrices, or dy behind them.
+__global__ __launch_bounds__(kThreads) void prepare_kernel(Prepared p, size_t code_stride, size_t scale_stride)
 {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols)
-        return;
+    __shared__ uint16_t tile[kTile * kTileStride];
+    if ((int)blockIdx.z < p.matrices)
+        transpose_matrix(tile, p.matrix[blockIdx.z], p.k, code_stride, scale_stride);
+    else
+        transpose_dy(tile, p);
+}
+
+// 64 columns per workgroup; the waves take every fourth row each, and their sums are added in order.
+__global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSums s)
+{
+    __shared__ float part[kThreads];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63);
     float sum = 0.0f;
-    for (int i = 0; i < count; ++i)
-        sum += partial[(size_t)i * cols + c];
-    sums[c] = sum;
+    if (c < s.columns) {
+#pragma unroll 8
+        for (int i = threadIdx.x >> 6; i < s.parts; i += kThreads / 64)
+            sum += s.partial[(size_t)i * s.columns + c];
+    }
+    part[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < 64 && c < s.columns)
+        s.sums[c] = ((part[threadIdx.x] + part[threadIdx.x + 64]) + part[threadIdx.x + 128]) + part[threadIdx.x + 192];
 }
 
 int conversion_grid(int rows, int segments)
@@ -329,28 +339,24 @@ hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld,
     }
 }
 
-hipError_t launch_mx_dequantize_transposed(const MxMatrix &q, uint16_t *dst, size_t ld, int k, hipStream_t stream)
+hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
 {
-    const dim3 grid((unsigned)((q.rows + kTile - 1) / kTile), (unsigned)((k + kTile - 1) / kTile));
-    mx_dequantize_transposed_kernel<<<grid, kThreads, 0, stream>>>(q.codes, q.scales, q.rows, k, mx_code_stride(k),
-                                                                   mx_scale_stride(k), dst, ld);
+    int rows = p.dy ? p.rows : 0, cols = p.dy ? p.cols : 0;
+    for (int i = 0; i < p.matrices; ++i) {
+        rows = max(rows, p.matrix[i].q.rows);
+        cols = max(cols, p.k);
+    }
+    if (rows == 0 || cols == 0)
+        return hipSuccess;
+    const dim3 grid((unsigned)((rows + kTile - 1) / kTile), (unsigned)((cols + kTile - 1) / kTile), (unsigned)(p.matrices + (p.dy != nullptr)));
+    prepare_kernel<<<grid, kThreads, 0, stream>>>(p, mx_code_stride(p.k), mx_scale_stride(p.k));
     return hipGetLastError();
 }
 
-hipError_t launch_bf16_transpose(const uint16_t *src, int rows, int cols, uint16_t *transposed, size_t ld_t, uint16_t *padded,
-                                 size_t ld_p, float *sums, float *partial, hipStream_t stream)
+hipError_t launch_column_sums(const ColumnSums &s, hipStream_t stream)
 {
-    const dim3 grid((unsigned)((rows + kTile - 1) / kTile), (unsigned)((cols + kTile - 1) / kTile));
-    hipError_t e = hipSuccess;
-    if (rows > 0) {  // (without rows the sums are zeros)
-        bf16_transpose_kernel<<<grid, kThreads, 0, stream>>>(src, rows, cols, transposed, ld_t, padded, ld_p, sums ? partial : nullptr);
-        e = hipGetLastError();
-    }
-    if (e == hipSuccess && sums) {
-        column_sums_kernel<<<(cols + kThreads - 1) / kThreads, kThreads, 0, stream>>>(partial, (int)grid.x, cols, sums);
-        e = hipGetLastError();
-    }
-    return e;
+    column_sums_kernel<<<(s.columns + 63) / 64, kThreads, 0, stream>>>(s);
+    return hipGetLastError();
 }
 
 }  // namespace int4linear

@@ -38,13 +38,33 @@ hipError_t launch_mx_quantize(const void *x, int type, size_t ld, uint8_t *codes
                               hipStream_t stream);
 // The way back: y = what codes and scales stand for.
 hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld, int k, hipStream_t stream);
-// dst[c * ld + r] = q[r][c] in bfloat16 for c < k; r goes on to the next multiple of 64 with zeros.
-hipError_t launch_mx_dequantize_transposed(const MxMatrix &q, uint16_t *dst, size_t ld, int k, hipStream_t stream);
-// src (rows x cols bfloat16, contiguous) -> transposed (cols x ld_t, zeros behind the rows); where they are
-// not null, padded (rows x ld_p, zeros behind the columns) and sums (cols floats: each column's sum, by way of
-// partial: ceil(rows / 64) x cols floats).
-hipError_t launch_bf16_transpose(const uint16_t *src, int rows, int cols, uint16_t *transposed, size_t ld_t, uint16_t *padded,
-                                 size_t ld_p, float *sums, float *partial, hipStream_t stream);
+// What a backward pass's products want of its operands, in one launch: up to three matrices q dequantised and transposed,
+// dst[c * ld + r] = q[r][c] in bfloat16 for c < k, r going on to the next multiple of 64 with zeros; and of dy (rows x cols
+// bfloat16, contiguous), where they are not null, the transpose (cols x ld_t, zeros behind the rows), a copy whose rows
+// are padded with zeros (rows x ld_p), and every column's sum over 64 rows at a time (partial: ceil(rows / 64) x cols).
+struct Transposed {
+    MxMatrix q;
+    uint16_t *dst;
+    size_t ld;
+};
+struct Prepared {
+    Transposed matrix[3];
+    int matrices, k;
+    const uint16_t *dy;
+    int rows, cols;
+    uint16_t *transposed, *padded;
+    size_t ld_t, ld_p;
+    float *partial;
+};
+hipError_t launch_prepare(const Prepared &p, hipStream_t stream);
+
+// sums[c] = the sum of `parts` rows of partial sums of `columns` columns, added in order (sums null: nothing to do).
+struct ColumnSums {
+    float *sums;
+    const float *partial;
+    int parts, columns;
+};
+hipError_t launch_column_sums(const ColumnSums &s, hipStream_t stream);
 
 hipError_t line_gemm_init(const DeviceInfo &dev);
 
@@ -68,10 +88,20 @@ hipError_t launch_mx_gated_quantized_skinny(const MxMatrix &x, const MxMatrix &w
 hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
                                      uint16_t *d, size_t ld_n, uint16_t *dt, size_t ld_m, int k, const DeviceInfo &dev,
                                      hipStream_t stream);
-// y[z] = a[z] b^T for bfloat16 operands whose rows are `k` values, padded with zeros to a multiple of 64 (`ld`
-// elements between rows of either, a multiple of 64).  a is `batch` (1 or 2) matrices of m rows back to back.
-hipError_t launch_bf16_gemm(const uint16_t *a, int m, const uint16_t *b, int n, size_t ld, int k, void *y0, void *y1, int batch, int out,
-                            const DeviceInfo &dev, hipStream_t stream);
+// y = a b^T for bfloat16 operands of m and n rows of k values, padded with zeros to a multiple of 64; `ld` elements
+// between rows of either, a multiple of 64.  out: kOutF32 or kOutBF16.
+struct Bf16Product {
+    const uint16_t *a;
+    int m;
+    const uint16_t *b;
+    int n;
+    size_t ld;
+    int k;
+    void *y;
+    int out;
+};
+// Up to three of them, and the column sums.
+hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const DeviceInfo &dev, hipStream_t stream);
 
 // Between the files of the C ABI (api.hip): the current device's record, set up for work on `stream`, and a
 // HIP error as the status of a call.  Both return an INT4LINEAR_* status.
