@@ -66,9 +66,19 @@ struct Parts {
     }
 };
 
+// Where slices of small products meet (of products that have terms at all).
+SliceSpace slice_space(Parts &p, bool terms)
+{
+    SliceSpace s;
+    s.partial = p.take<float>(terms ? (size_t)kMostSlices * 64 * 64 : 0);
+    s.arrivals = p.take<unsigned>(terms ? kMostSlices * 4 : 0);
+    return s;
+}
+
 struct LinearBackwardParts {
     uint16_t *dy_t, *dy_padded, *x_t, *w_t;
     float *sums;
+    SliceSpace slices;
     size_t ld_m, ld_n, bytes;
 };
 
@@ -83,12 +93,14 @@ LinearBackwardParts linear_backward_parts(void *work, int m, int n, int k)
     r.x_t = p.take<uint16_t>((size_t)k * r.ld_m);
     r.w_t = p.take<uint16_t>((size_t)k * r.ld_n);
     r.sums = p.take<float>((size_t)n * (r.ld_m / 64));
+    r.slices = slice_space(p, m > 0 && n > 0 && k > 0);
     r.bytes = p.used;
     return r;
 }
 
 struct GatedBackwardParts {
     uint16_t *d, *d_t, *x_t, *w_t;
+    SliceSpace slices;
     size_t ld_m, ld_n, bytes;
 };
 
@@ -102,6 +114,7 @@ GatedBackwardParts gated_backward_parts(void *work, int m, int n, int k)
     r.d_t = p.take<uint16_t>(2 * (size_t)n * r.ld_m);
     r.x_t = p.take<uint16_t>((size_t)k * r.ld_m);
     r.w_t = p.take<uint16_t>((size_t)k * 2 * r.ld_n);
+    r.slices = slice_space(p, m > 0 && n > 0 && k > 0);
     r.bytes = p.used;
     return r;
 }
@@ -235,6 +248,8 @@ int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, co
     const bool ragged = n % 64 != 0;
     Prepared prepared{};
     prepared.k = k;
+    prepared.zeros = p.slices.arrivals;
+    prepared.zero_count = m > 0 && n > 0 && k > 0 ? kMostSlices * 4 : 0;
     if (want_dw && m > 0)
         prepared.matrix[prepared.matrices++] = {matrix(x_codes_d, x_scales_d, m), p.x_t, p.ld_m};
     if (want_dx && n > 0)
@@ -250,15 +265,11 @@ int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, co
         prepared.partial = want_sums ? p.sums : nullptr;
     }
     hipError_t e = launch_prepare(prepared, stream);
-    Bf16Product products[2];
-    int count = 0;
-    if (want_dw)
-        products[count++] = {p.dy_t, n, p.x_t, k, p.ld_m, m, dw_d, dw_type};
-    if (want_dx)
-        products[count++] = {ragged ? p.dy_padded : (const uint16_t *)dy_d, m, p.w_t, k, p.ld_n, n, dx_d, kOutBF16};
+    const Bf16Product products[] = {{p.dy_t, n, p.x_t, k, p.ld_m, m, want_dw ? dw_d : nullptr, dw_type},
+                                    {ragged ? p.dy_padded : (const uint16_t *)dy_d, m, p.w_t, k, p.ld_n, n, want_dx ? dx_d : nullptr, kOutBF16}};
     const ColumnSums sums{want_sums ? dbias_d : nullptr, p.sums, (int)(p.ld_m / 64), n};
     if (e == hipSuccess)
-        e = launch_bf16_products(products, count, sums, info, stream);
+        e = launch_bf16_products(products, 2, sums, p.slices, info, stream);
     return api_status(e);
 }
 
@@ -300,6 +311,8 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
     // wg and wu side by side: row c of w_t is column c of wg, then column c of wu
     Prepared prepared{};
     prepared.k = k;
+    prepared.zeros = p.slices.arrivals;
+    prepared.zero_count = m > 0 && n > 0 && k > 0 ? kMostSlices * 4 : 0;
     if (want_dw && m > 0)
         prepared.matrix[prepared.matrices++] = {x, p.x_t, p.ld_m};
     if (want_dx && n > 0) {
@@ -308,16 +321,12 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
     }
     if (e == hipSuccess)
         e = launch_prepare(prepared, stream);
-    Bf16Product products[3];
-    int count = 0;
-    if (want_dw) {
-        products[count++] = {p.d_t, n, p.x_t, k, p.ld_m, m, dwg_d, dw_type};
-        products[count++] = {p.d_t + (size_t)n * p.ld_m, n, p.x_t, k, p.ld_m, m, dwu_d, dw_type};
-    }
-    if (want_dx)
-        products[count++] = {p.d, m, p.w_t, k, 2 * p.ld_n, (int)(n > 0 ? 2 * p.ld_n : 0), dx_d, kOutBF16};
+    const Bf16Product products[] = {
+        {p.d_t, n, p.x_t, k, p.ld_m, m, want_dw ? dwg_d : nullptr, dw_type},
+        {p.d_t + (size_t)n * p.ld_m, n, p.x_t, k, p.ld_m, m, want_dw ? dwu_d : nullptr, dw_type},
+        {p.d, m, p.w_t, k, 2 * p.ld_n, (int)(n > 0 ? 2 * p.ld_n : 0), want_dx ? dx_d : nullptr, kOutBF16}};
     if (e == hipSuccess)
-        e = launch_bf16_products(products, count, ColumnSums{}, info, stream);
+        e = launch_bf16_products(products, 3, ColumnSums{}, p.slices, info, stream);
     return api_status(e);
 }
 

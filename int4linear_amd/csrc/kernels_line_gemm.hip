@@ -19,6 +19,7 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
@@ -282,9 +283,10 @@ constexpr int kScaleStages = 2;  // stages whose scales are 16 bytes of a row
 constexpr int kSteps = 4;        // steps of a stage
 
 // WAVES_M x WAVES_N wavefronts multiply, each FM x FN blocks of 32 x 32; LOADERS more load for them (0: each of the
-// others loads its share); STAGES stages in LDS; OCC waves per SIMD.
-template <int WAVES_M_, int WAVES_N_, int FM_, int FN_, int LOADERS_, int STAGES_, int OCC_>
+// others loads its share); STAGES stages in LDS; operands are read AHEAD steps ahead; OCC waves per SIMD.
+template <int WAVES_M_, int WAVES_N_, int FM_, int FN_, int LOADERS_, int STAGES_, int AHEAD_, int OCC_>
 struct LineTile {
+    static constexpr int AHEAD = AHEAD_, SETS = AHEAD == 1 ? 2 : 4;  // register sets of a step's operands
     static constexpr int WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, FM = FM_, FN = FN_, LOADERS = LOADERS_, STAGES = STAGES_, OCC = OCC_;
     static constexpr int NWAVES = WAVES_M * WAVES_N, THREADS = (NWAVES + LOADERS) * 64;
     static constexpr int LOADING = LOADERS ? LOADERS : NWAVES;    // waves that load
@@ -343,8 +345,8 @@ hipError_t fill_rows(void *y, const float *bias, size_t m, size_t n, hipStream_t
 // wave that issues it, and these tiles have fewer matrix instructions to hide that behind (64 x 128 tiles, four loaders
 // against none: 512 x 4096 x 11008 23.6 us and 26.2; 64 x 4096 x 4096 8.6 and 10.5).  The 256 x 256 tile has no registers left
 // for more waves.  STAGES stages ring in LDS.  A stage is four steps of FM x FN matrix
-// instructions; while a step's instructions run, the next step's operands are read from LDS into the other register
-// set.  Before a stage's last step every read of the stage has been made: there the waves meet, the next stage must
+// instructions; while a step's instructions run, those of the step AHEAD further on are read from LDS into another register
+// set.  Before a stage's AHEAD last steps every read of the stage has been made: there the waves meet, the next stage must
 // have landed (younger ones stay in flight), and the stage's buffer is given to the loads of the stage STAGES further on.
 template <bool FP4, class C, class Ep>
 __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, int tiles_n, const Ep &ep, int first, int by)
@@ -513,7 +515,7 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
     const unsigned b_rd = (unsigned)((C::BM + wn * C::FN * kFrag) * kLineBytes);
     const unsigned as_rd = (unsigned)(C::STAGES * C::STAGE + (wm * C::FM * kFrag + fr) * 16 + 4 * fg);
     const unsigned bs_rd = (unsigned)(C::STAGES * C::STAGE + (C::BM + wn * C::FN * kFrag + fr) * 16 + 4 * fg);
-    v4i fa[2][C::FM], fb[2][C::FN];
+    v4i fa[C::SETS][C::FM], fb[C::SETS][C::FN];
     int sa[2][C::FM] = {}, sb[2][C::FN] = {};
 
     // Operand r of step J of the stage in `buffer`, into register set p.
@@ -538,7 +540,7 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
     };
     // The matrix instructions of step J, `behind` called after each with its number.
     auto step = [&](auto j_tag, auto &&behind) {
-        constexpr int J = decltype(j_tag)::value, p = J & 1;
+        constexpr int J = decltype(j_tag)::value, p = J % C::SETS;
         [&]<int... SLOT>(std::integer_sequence<int, SLOT...>) {
             ([&] {
                 constexpr int j = SLOT / C::FN, i = SLOT % C::FN;
@@ -567,8 +569,10 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
     constexpr int kLoadsPerSlot = (kLoads + C::SLOTS - 1) / C::SLOTS;
 
 #pragma unroll
-    for (int r = 0; r < kReads; ++r)
-        read(0, 0, 0, r);
+    for (int J = 0; J < C::AHEAD; ++J)
+#pragma unroll
+        for (int r = 0; r < kReads; ++r)
+            read(0, J, J, r);
     read_scales(0, 0, 1);
 
     unsigned buffer = 0, slot = 0;
@@ -582,37 +586,34 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
             for (int i = 0; i < C::FN; ++i)
                 sb[0][i] = sb[1][i];
         }
-        [&]<int... J>(std::integer_sequence<int, J...>) {
-            (step(std::integral_constant<int, J>{},
-                  [&](auto slot_tag) {
-                      constexpr int at = decltype(slot_tag)::value * kReadsPerSlot;
-#pragma unroll
-                      for (int r = at; r < at + kReadsPerSlot && r < kReads; ++r)
-                          read(buffer, J + 1, (J + 1) & 1, r);
-                  }),
-             ...);
-        }(std::make_integer_sequence<int, kSteps - 1>{});
-        if constexpr (C::LOADERS == 0)
-            meet(std::integral_constant<int, C::STAGES - 2>{});
-        else
-            meet_without_loads();
         const bool last = s + 1 == stages;
         const int next_s = last ? 0 : s + 1;
-        if (FP4 && next_s % kScaleStages == 0)
-            slot = next_in_ring(slot, C::SCALES);
         const unsigned next_buffer = next_in_ring(buffer, C::STAGE);
-        read_scales(slot, next_s, 1);
-        step(std::integral_constant<int, kSteps - 1>{}, [&](auto slot_tag) {
-            constexpr int at = decltype(slot_tag)::value * kReadsPerSlot, load_at = decltype(slot_tag)::value * kLoadsPerSlot;
+        [&]<int... J>(std::integer_sequence<int, J...>) {
+            ([&] {
+                if constexpr (J == kSteps - C::AHEAD) {
+                    if constexpr (C::LOADERS == 0)
+                        meet(std::integral_constant<int, C::STAGES - 2>{});
+                    else
+                        meet_without_loads();
+                    if (FP4 && next_s % kScaleStages == 0)
+                        slot = next_in_ring(slot, C::SCALES);
+                    read_scales(slot, next_s, 1);
+                }
+                step(std::integral_constant<int, J>{}, [&](auto slot_tag) {
+                    constexpr int at = decltype(slot_tag)::value * kReadsPerSlot, then = J + C::AHEAD;
 #pragma unroll
-            for (int r = at; r < at + kReadsPerSlot && r < kReads; ++r)
-                read(next_buffer, 0, 0, r);
-            if constexpr (C::LOADERS == 0) {
+                    for (int r = at; r < at + kReadsPerSlot && r < kReads; ++r)
+                        read(then < kSteps ? buffer : next_buffer, then % kSteps, then % C::SETS, r);
+                    if constexpr (C::LOADERS == 0 && J == kSteps - 1) {
+                        constexpr int load_at = decltype(slot_tag)::value * kLoadsPerSlot;
 #pragma unroll
-                for (int c = load_at; c < load_at + kLoadsPerSlot && c < kLoads; ++c)
-                    load(c);
-            }
-        });
+                        for (int c = load_at; c < load_at + kLoadsPerSlot && c < kLoads; ++c)
+                            load(c);
+                    }
+                });
+            }(), ...);
+        }(std::make_integer_sequence<int, kSteps>{});
         if constexpr (C::LOADERS == 0)
             load_rest();
         buffer = next_buffer;
@@ -633,26 +634,90 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOpera
     line_gemm<FP4, C>(o, tiles_m, tiles_n, ep, blockIdx.x, gridDim.x);
 }
 
-// Up to three products in one launch, a tile per workgroup: those of a small layer's backward pass, each of which would leave
-// most CUs idle, by blockIdx.z.  The last one is dx; the others, the weights', share a type.
+// Up to three products in one launch, by blockIdx.z: those of a small layer's backward pass, each of which would leave
+// most CUs idle.  A workgroup makes one slice of one tile of 64 x 64: slice blockIdx.x % slices of stages
+// slice * stages / slices on.  The last product is dx; the others, the weights', share a type.
 struct LineGroup {
     LineOperands o[3];
-    int tiles_m[3], tiles_n[3];
+    int tiles_m[3], tiles_n[3], slices[3];
     void *y[3];
+    int first[3];  // number of a product's first tile-slice and, times waves, of its first counter
     int count;
+    float *partial;      // sums of a tile-slice: 64 x 64 floats
+    unsigned *arrivals;  // counters, zero before the launch
     // Column sums to be completed on the way (sums null: none): of `parts` rows of partial sums.
     float *sums;
-    const float *partial;
+    const float *sum_parts;
     int parts, columns;
+};
+
+// An epilogue behind sums that are one of `slices` shares: every wave leaves its share, waits until that has been acknowledged
+// and counts itself in.  The last of a tile's waves of one number to arrive adds all shares up in the order of their
+// slices, whoever came when, and goes on to the epilogue; nobody waits for anybody.  (Relaxed atomic operations at device scope go
+// through to the level that all XCDs share.)
+template <class Ep>
+struct SliceEpilogue {
+    static constexpr bool kPair = Ep::kPair, kColumns = Ep::kColumns;
+    Ep ep;
+    float *partial;     // of this tile's slice 0, wave 0
+    unsigned *arrived;  // of this tile's wave 0
+    int slice, slices;
+
+    __device__ __forceinline__ void operator()(v16f (&acc)[1][1], int row, int col, int lane) const
+    {
+        typedef unsigned long long u64;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (slices > 1) {
+            constexpr int kSlice = 64 * 64 / 2, kWords = 8;  // words of two floats, of a slice and of a lane
+            u64 *mine = (u64 *)partial + (size_t)wave * kWords * 64 + lane;
+            float v[16];
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                v[t] = acc[0][0][t];
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                __hip_atomic_store(mine + (size_t)slice * kSlice + i * 64, __builtin_bit_cast(u64, (v2f){v[2 * i], v[2 * i + 1]}),
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            int before = 0;
+            if (lane == 0)
+                before = (int)__hip_atomic_fetch_add(arrived + wave, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (__builtin_amdgcn_readfirstlane(before) != slices - 1)
+                return;
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                v[t] = 0.0f;
+            for (int from = 0; from < slices; ++from) {
+                u64 got[kWords];
+#pragma unroll
+                for (int i = 0; i < kWords; ++i)
+                    got[i] = __hip_atomic_load(mine + (size_t)from * kSlice + i * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const v2f pair = __builtin_bit_cast(v2f, got[i]);
+                    v[2 * i] += pair[0];
+                    v[2 * i + 1] += pair[1];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                acc[0][0][t] = v[t];
+        }
+        ep(acc, row, col, lane);
+    }
 };
 
 __device__ __forceinline__ void complete_sums(float *sums, const float *partial, int parts, int columns, int first, int by)
 {
     for (int c = first; c < columns; c += by) {
-        float sum = 0.0f;
-        for (int i = 0; i < parts; ++i)
-            sum += partial[(size_t)i * columns + c];
-        sums[c] = sum;
+        float sum[4] = {};  // in the order of column_sums_kernel
+        for (int i = 0; i < parts; i += 4)
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                if (i + w < parts)
+                    sum[w] += partial[(size_t)(i + w) * columns + c];
+        sums[c] = ((sum[0] + sum[1]) + sum[2]) + sum[3];
     }
 }
 
@@ -661,14 +726,23 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_group_kernel(LineGrou
 {
     const int z = blockIdx.z;
     if (g.sums && z == 0)
-        complete_sums(g.sums, g.partial, g.parts, g.columns, blockIdx.x * C::THREADS + threadIdx.x, gridDim.x * C::THREADS);
-    const int tiles = g.tiles_m[z] * g.tiles_n[z];
-    if ((int)blockIdx.x >= tiles)
+        complete_sums(g.sums, g.sum_parts, g.parts, g.columns, blockIdx.x * C::THREADS + threadIdx.x, gridDim.x * C::THREADS);
+    const int tiles = g.tiles_m[z] * g.tiles_n[z], slices = g.slices[z];
+    const int tile = (int)blockIdx.x / slices, slice = (int)blockIdx.x % slices;
+    if (tile >= tiles)
         return;
+    LineOperands o = g.o[z];
+    const int from = (int)((long)slice * o.stages / slices), to = (int)((long)(slice + 1) * o.stages / slices);
+    o.a += (size_t)from * kLineBytes;
+    o.b0 += (size_t)from * kLineBytes;
+    o.b1 = o.b0;
+    o.stages = to - from;
     auto run = [&](auto ep) {
         ep.y = g.y[z];
-        ep.m = g.o[z].a_rows;
-        line_gemm<false, C>(g.o[z], g.tiles_m[z], g.tiles_n[z], ep, blockIdx.x, tiles);
+        ep.m = o.a_rows;
+        const SliceEpilogue<decltype(ep)> shared{ep, g.partial + (size_t)(g.first[z] + tile * slices) * 64 * 64,
+                                                 g.arrivals + (g.first[z] + tile * slices) * C::NWAVES, slice, slices};
+        line_gemm<false, C>(o, g.tiles_m[z], g.tiles_n[z], shared, tile, tiles);
     };
     if (z == g.count - 1)
         run(ep_x);
@@ -676,10 +750,10 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_group_kernel(LineGrou
         run(ep_w);
 }
 
-using Tile256 = LineTile<4, 2, 2, 4, 0, 2, 2>;
-using Tile128 = LineTile<2, 2, 2, 2, 4, 2, 4>;
-using Tile64x128 = LineTile<2, 2, 1, 2, 4, 3, 4>;
-using Tile64 = LineTile<2, 2, 1, 1, 4, 4, 4>;  // (too narrow for pairs of blocks)
+using Tile256 = LineTile<4, 2, 2, 4, 0, 2, 1, 2>;
+using Tile128 = LineTile<2, 2, 2, 2, 4, 2, 1, 4>;
+using Tile64x128 = LineTile<2, 2, 1, 2, 4, 3, 2, 4>;
+using Tile64 = LineTile<2, 2, 1, 1, 4, 4, 2, 4>;  // (too narrow for pairs of blocks)
 
 // Workgroups of a tile that a CU's LDS holds.
 template <class C, bool FP4>
@@ -895,33 +969,37 @@ static hipError_t launch_bf16(const Bf16Product &p, const DeviceInfo &dev, hipSt
                    : launch<false>(operands(p), p.n, epilogue<kOutBF16, false>(p), dev, stream);
 }
 
-template <class C, class EpW, class EpX>
-static hipError_t launch_group(LineGroup g, const EpW &ep_w, const EpX &ep_x, hipStream_t stream)
+template <class EpW, class EpX>
+static hipError_t launch_group(const LineGroup &g, const EpW &ep_w, const EpX &ep_x, hipStream_t stream)
 {
     int most = 1;
-    for (int i = 0; i < g.count; ++i) {
-        g.tiles_m[i] = (g.o[i].a_rows + C::BM - 1) / C::BM;
-        g.tiles_n[i] = (g.o[i].b_rows + C::BN - 1) / C::BN;
-        most = max(most, g.tiles_m[i] * g.tiles_n[i]);
-    }
-    line_group_kernel<C, EpW, EpX><<<dim3((unsigned)most, 1, (unsigned)g.count), C::THREADS, C::template LDS<false>, stream>>>(g, ep_w, ep_x);
+    for (int i = 0; i < g.count; ++i)
+        most = max(most, g.tiles_m[i] * g.tiles_n[i] * g.slices[i]);
+    line_group_kernel<Tile64, EpW, EpX><<<dim3((unsigned)most, 1, (unsigned)g.count), Tile64::THREADS, Tile64::LDS<false>, stream>>>(g, ep_w, ep_x);
     return hipGetLastError();
 }
 
-hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const DeviceInfo &dev, hipStream_t stream)
+// How long a slice of k is at least, in stages: meeting costs as much as about six.
+constexpr int kLeastSlice = 6;
+
+hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const SliceSpace &space, const DeviceInfo &dev,
+                                hipStream_t stream)
 {
-    // Together where two rounds of workgroups hold all tiles of 64 x 64: beyond that each fills the device alone, on larger
-    // tiles.  (257 x 1400 x 1000, gated: one launch 19 us, three 34; 130 x 1001 x 515, linear: 14 and 21.)
+    // Together where kMostSlices workgroups hold all tiles of 64 x 64: beyond that each fills the device alone, on larger
+    // tiles.  Long k is cut into slices as far as they go.  (Backward pass of a gated layer, 257 x 1400 x 1000, and of a linear one,
+    // 130 x 1001 x 515: a launch for each product and operand 39 and 27 us, grouped 33 and 14, with slices 29 and 14: the
+    // gated products 21 us, with dx in four slices 17.)
     long tiles = 0;
-    bool together = count > 1 && p[count - 1].out == kOutBF16;
+    bool together = count > 0 && p[count - 1].out == kOutBF16;
     for (int i = 0; i < count; ++i) {
         tiles += ((p[i].m + 63l) / 64) * ((p[i].n + 63l) / 64);
         together = together && p[i].k > 0 && p[i].n == p[0].n && (i == count - 1 || p[i].out == p[0].out);
     }
-    if (!together || tiles > 4l * dev.cu_count) {
+    if (!together || tiles > kMostSlices) {
         hipError_t e = hipSuccess;
         for (int i = 0; i < count && e == hipSuccess; ++i)
-            e = launch_bf16(p[i], dev, stream);
+            if (p[i].y)
+                e = launch_bf16(p[i], dev, stream);
         return e == hipSuccess && sums.sums ? launch_column_sums(sums, stream) : e;
     }
     LineGroup g{};
@@ -929,17 +1007,40 @@ hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSum
     for (int i = 0; i < count; ++i) {
         g.o[i] = operands(p[i]);
         g.y[i] = p[i].y;
+        g.tiles_m[i] = (p[i].m + 63) / 64;
+        g.tiles_n[i] = (p[i].n + 63) / 64;
     }
+    int total = 0;
+    for (int least = kLeastSlice;; least += least / 4) {
+        total = 0;
+        for (int i = 0; i < count; ++i) {
+            g.slices[i] = min(max(g.o[i].stages / least, 1), 16);
+            g.first[i] = total;
+            total += g.tiles_m[i] * g.tiles_n[i] * g.slices[i];
+        }
+        if (total <= kMostSlices || total == tiles)
+            break;
+    }
+    bool any = false;
+    for (int i = 0; i < count; ++i) {
+        any = any || p[i].y;
+        if (!p[i].y)
+            g.tiles_m[i] = 0;  // not wanted; the others' slices are the same with it and without
+    }
+    if (!any)
+        return sums.sums ? launch_column_sums(sums, stream) : hipSuccess;
+    g.partial = space.partial;
+    g.arrivals = space.arrivals;
     g.sums = sums.sums;
-    g.partial = sums.partial;
+    g.sum_parts = sums.partial;
     g.parts = sums.parts;
     g.columns = sums.columns;
     const Bf16Product &w = p[0], &x = p[count - 1];
     if (w.out == kOutF32)
-        return x.n % 8 ? launch_group<Tile64>(g, epilogue<kOutF32, true>(w), epilogue<kOutBF16, true>(x), stream)
-                       : launch_group<Tile64>(g, epilogue<kOutF32, true>(w), epilogue<kOutBF16, false>(x), stream);
-    return x.n % 8 ? launch_group<Tile64>(g, epilogue<kOutBF16, true>(w), epilogue<kOutBF16, true>(x), stream)
-                   : launch_group<Tile64>(g, epilogue<kOutBF16, false>(w), epilogue<kOutBF16, false>(x), stream);
+        return x.n % 8 ? launch_group(g, epilogue<kOutF32, true>(w), epilogue<kOutBF16, true>(x), stream)
+                       : launch_group(g, epilogue<kOutF32, true>(w), epilogue<kOutBF16, false>(x), stream);
+    return x.n % 8 ? launch_group(g, epilogue<kOutBF16, true>(w), epilogue<kOutBF16, true>(x), stream)
+                   : launch_group(g, epilogue<kOutBF16, false>(w), epilogue<kOutBF16, false>(x), stream);
 }
 
 }  // namespace int4linear

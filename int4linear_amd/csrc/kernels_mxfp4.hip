@@ -258,6 +258,9 @@ __device__ __forceinline__ void transpose_dy(uint16_t *tile, const Prepared &p)
 __global__ __launch_bounds__(kThreads) void prepare_kernel(Prepared p, size_t code_stride, size_t scale_stride)
 {
     __shared__ uint16_t tile[kTile * kTileStride];
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+        for (int i = threadIdx.x; i < p.zero_count; i += kThreads)
+            p.zeros[i] = 0;
     if ((int)blockIdx.z < p.matrices)
         transpose_matrix(tile, p.matrix[blockIdx.z], p.k, code_stride, scale_stride);
     else

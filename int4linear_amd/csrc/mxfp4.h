@@ -38,7 +38,7 @@ hipError_t launch_mx_quantize(const void *x, int type, size_t ld, uint8_t *codes
                               hipStream_t stream);
 // The way back: y = what codes and scales stand for.
 hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld, int k, hipStream_t stream);
-// What a backward pass's products want of its operands, in one launch: up to three matrices q dequantised and transposed,
+// What a backward pass's products want of its operands, in one launch: words cleared; up to three matrices q dequantised and transposed,
 // dst[c * ld + r] = q[r][c] in bfloat16 for c < k, r going on to the next multiple of 64 with zeros; and of dy (rows x cols
 // bfloat16, contiguous), where they are not null, the transpose (cols x ld_t, zeros behind the rows), a copy whose rows
 // are padded with zeros (rows x ld_p), and every column's sum over 64 rows at a time (partial: ceil(rows / 64) x cols).
@@ -55,6 +55,8 @@ struct Prepared {
     uint16_t *transposed, *padded;
     size_t ld_t, ld_p;
     float *partial;
+    unsigned *zeros;  // words to be cleared
+    int zero_count;
 };
 hipError_t launch_prepare(const Prepared &p, hipStream_t stream);
 
@@ -100,8 +102,15 @@ struct Bf16Product {
     void *y;
     int out;
 };
-// Up to three of them, and the column sums.
-hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const DeviceInfo &dev, hipStream_t stream);
+// Up to three of them, and the column sums.  Small ones are cut into slices of k, whose sums meet in `space`.  One whose
+// y is null is not wanted; results do not depend on which are.
+constexpr int kMostSlices = 1024;  // tiles of 64 x 64, times the slices of each
+struct SliceSpace {
+    float *partial;      // kMostSlices * 64 * 64
+    unsigned *arrivals;  // kMostSlices * 4, zeros
+};
+hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const SliceSpace &space, const DeviceInfo &dev,
+                                hipStream_t stream);
 
 // Between the files of the C ABI (api.hip): the current device's record, set up for work on `stream`, and a
 // HIP error as the status of a call.  Both return an INT4LINEAR_* status.

@@ -289,7 +289,7 @@ def test_gated(gpu, m, n, k, kind):
     assert torch.equal(got[:, n:], torch.zeros(m, 32 * blocks - n, dtype=torch.float64))
 
 
-BACKWARD = [(1, 1, 1), (1, 64, 256), (3, 65, 40), (16, 128, 300), (64, 64, 64), (65, 130, 257), (100, 300, 100), (130, 257, 515), (192, 320, 512)]
+BACKWARD = [(1000, 64, 64), (2500, 40, 72), (64, 2000, 64), (700, 130, 40), (40, 900, 520), (1, 1, 1), (1, 64, 256), (3, 65, 40), (16, 128, 300), (64, 64, 64), (65, 130, 257), (100, 300, 100), (130, 257, 515), (192, 320, 512)]
 
 
 @pytest.mark.gpu
