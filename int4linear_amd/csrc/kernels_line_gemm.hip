@@ -22,7 +22,9 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
@@ -223,6 +225,29 @@ struct GradientEpilogue {
     template <int FM, int FN>
     __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
+        // (all loads first: behind one another they cost a way to memory each)
+        v4bf in[FM][FN / 2][4];
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+            for (int i = 0; i < FN / 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r = row + kFrag * j + (lane & 31), c = col + kFrag * i + 8 * q + 4 * (lane >> 5);
+                    in[j][i][q] = (v4bf){};
+                    if (r < m) {
+                        const __bf16 *src = dh + (size_t)r * n + c;
+                        if (vec) {
+                            if (c < n)
+                                in[j][i][q] = *(const v4bf *)src;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (c + e < n)
+                                    in[j][i][q][e] = src[e];
+                        }
+                    }
+                }
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
             const int r = row + kFrag * j + (lane & 31);
@@ -231,47 +256,45 @@ struct GradientEpilogue {
                 const int c0 = col + kFrag * (i / 2);
                 float dg[16], du[16];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int c = c0 + 8 * q + 4 * (lane >> 5);
-                    v4bf in = {};
-                    if (r < m) {
-                        const __bf16 *src = dh + (size_t)r * n + c;
-                        if (vec) {
-                            if (c < n)
-                                in = *(const v4bf *)src;
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (c + e < n)
-                                    in[e] = src[e];
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int t = 4 * q + e;
-                        float value, slope;
-                        activate_with_slope(act, acc[j][i][t], value, slope);
-                        // padding: exact zeros, whatever the clamped rows gave
-                        const bool there = r < m && c + e < n;
-                        const float g = (float)in[e];
-                        dg[t] = there ? g * acc[j][i + 1][t] * slope : 0.0f;
-                        du[t] = there ? g * value : 0.0f;
-                    }
+                for (int t = 0; t < 16; ++t) {
+                    float value, slope;
+                    activate_with_slope(act, acc[j][i][t], value, slope);
+                    // padding: exact zeros, whatever the clamped rows gave
+                    const bool there = r < m && c0 + 8 * (t / 4) + 4 * (lane >> 5) + t % 4 < n;
+                    const float g = (float)in[j][i / 2][t / 4][t % 4];
+                    dg[t] = there ? g * acc[j][i + 1][t] * slope : 0.0f;
+                    du[t] = there ? g * value : 0.0f;
                 }
                 store_block<kOutBF16, false>(d, 2 * ld_n, m, (int)ld_n, row + kFrag * j, c0, lane, dg);
                 store_block<kOutBF16, false>(d + ld_n, 2 * ld_n, m, (int)ld_n, row + kFrag * j, c0, lane, du);
-                // the transposes: 32 neighbouring rows a store
                 if ((size_t)r < ld_m) {
-#pragma unroll
-                    for (int t = 0; t < 16; ++t) {
-                        const int c = c0 + 8 * (t / 4) + 4 * (lane >> 5) + t % 4;
-                        if (c < n) {
-                            dt[(size_t)c * ld_m + r] = (__bf16)dg[t];
-                            dt[((size_t)n + c) * ld_m + r] = (__bf16)du[t];
-                        }
-                    }
+                    store_transposed(dt, r, c0, lane, dg);
+                    store_transposed(dt + (size_t)n * ld_m, r, c0, lane, du);
                 }
             }
+        }
+    }
+
+    // The transposes.  A quad's 4 rows x 4 columns change places, twice: between neighbours, then between pairs.  A lane then has four rows of
+    // column lane % 4 of each four: 8 bytes a store.  (With stores of 2 bytes, and dh fetched block by block, 4096 x 14336 x 4096 takes
+    // 466 us, so 400; the product alone with h as its result 275.)
+    __device__ __forceinline__ void store_transposed(__bf16 *to, int r, int c0, int lane, const float (&v)[16]) const
+    {
+        const unsigned halves = lane & 1 ? 0x03020706u : 0x05040100u;
+        const bool upper = lane & 2;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            unsigned two[2];  // rows r & ~1, r | 1 of column 2 i + lane % 2 of the four
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const unsigned own = __builtin_bit_cast(unsigned, (v2bf){(__bf16)v[4 * q + 2 * i], (__bf16)v[4 * q + 2 * i + 1]});
+                two[i] = __builtin_amdgcn_perm((unsigned)__builtin_amdgcn_mov_dpp((int)own, 0xB1, 0xF, 0xF, true), own, halves);
+            }
+            const unsigned kept = upper ? two[1] : two[0];
+            const unsigned got = (unsigned)__builtin_amdgcn_mov_dpp((int)(upper ? two[0] : two[1]), 0x4E, 0xF, 0xF, true);
+            const int c = c0 + 8 * q + 4 * (lane >> 5) + (lane & 3);
+            if (c < n)
+                *(v2u *)(to + (size_t)c * ld_m + (r & ~3)) = upper ? (v2u){got, kept} : (v2u){kept, got};
         }
     }
 };
