@@ -12,13 +12,13 @@
 #include "mxfp4.h"
 #include "mxfp4_epilogue.h"
 
+#include <type_traits>
+
 namespace int4linear {
 
 namespace {
 
-typedef int v2i __attribute__((ext_vector_type(2)));
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef unsigned short v8us __attribute__((ext_vector_type(8)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kSegment = 512;  // k that one wave converts at a time: 8 per lane
@@ -179,92 +179,138 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const uint8_t *
     }
 }
 
-// 64 rows x 64 k of q -> 64 rows of dst, by way of LDS.  Values of E2M1 times a power of two down to
-// 2^-126 are bfloat16 numbers; smaller ones are rounded.
+// Transposes for the gradients.  A lane takes 8 x 8 values, 16-bit, whose rows are four registers each: a byte permutation of
+// two rows' registers gives two values of one column, so 32 permutations turn the square and neither LDS nor other lanes
+// take part (through LDS: 124 us for 91).  A wave takes 64 rows x 64 columns, eight lanes down and eight across: it stores whole 128-byte lines.  Values of
+// E2M1 times a power of two from 2^-127 are bfloat16 numbers.
 constexpr int kTile = 64;
-constexpr int kTileStride = kTile + 2;  // elements between rows in LDS: an odd number of words
+constexpr int kTilesAcross = 4;  // a workgroup's: a whole line of codes
 
-__device__ __forceinline__ void transpose_matrix(uint16_t *tile, const Transposed &t, int k, size_t code_stride, size_t scale_stride)
+// The values at (row 8i + r, column 8j + c) of a wave's tile, i = lane % 8, j = lane / 8: rows[r] -> dst, from the tile's
+// first column on.
+__device__ __forceinline__ void store_transposed(const v4u (&rows)[8], uint16_t *dst, size_t ld, int columns)
 {
-    const int r0 = blockIdx.x * kTile, c0 = blockIdx.y * kTile;
+    const int lane = threadIdx.x & 63, c0 = (lane >> 3) * 8;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        v4u out;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            out[w] = __builtin_amdgcn_perm(rows[2 * w + 1][c / 2], rows[2 * w][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+        if (c0 + c < columns)
+            *(v4u *)(dst + (size_t)(c0 + c) * ld + (lane & 7) * 8) = out;
+    }
+}
+
+template <int DOWN>
+__device__ __forceinline__ void transpose_matrix(const Transposed &t, int k, size_t code_stride, size_t scale_stride)
+{
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = (blockIdx.x * DOWN + wave / kTilesAcross) * kTile, c0 = (blockIdx.y * kTilesAcross + wave % kTilesAcross) * kTile;
     if (r0 >= t.q.rows || c0 >= k)
         return;
+    const int row = r0 + (lane & 7) * 8, col = c0 + (lane >> 3) * 8;
+    unsigned codes[8], scales[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int i = threadIdx.x + h * kThreads;
-        const int r = i >> 3, c = (i & 7) * 8;
-        float v[8] = {};
-        if (r0 + r < t.q.rows)
-            decode8(*(const unsigned *)(t.q.codes + (size_t)(r0 + r) * code_stride + (c0 + c) / 2),
-                    t.q.scales[(size_t)(r0 + r) * scale_stride + (c0 + c) / kMxBlock], v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            tile[(c + e) * kTileStride + r] = __builtin_bit_cast(uint16_t, (__bf16)v[e]);
+    for (int r = 0; r < 8; ++r) {
+        codes[r] = scales[r] = 0;
+        if (row + r < t.q.rows) {
+            codes[r] = *(const unsigned *)(t.q.codes + (size_t)(row + r) * code_stride + col / 2);
+            scales[r] = t.q.scales[(size_t)(row + r) * scale_stride + col / kMxBlock];
+        }
     }
-    __syncthreads();
+    v4u rows[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int i = threadIdx.x + h * kThreads;
-        const int c = i >> 3, r = (i & 7) * 8;
-        if (c0 + c >= k)
-            continue;
-        v8us out;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            out[e] = tile[c * kTileStride + r + e];
-        *(v8us *)(t.dst + (size_t)(c0 + c) * t.ld + r0 + r) = out;
+    for (int r = 0; r < 8; ++r) {
+        const float scale = __builtin_bit_cast(float, scales[r] << 23);
+        rows[r] = (v4u){__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[r], scale, 0)),
+                        __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[r], scale, 1)),
+                        __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[r], scale, 2)),
+                        __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[r], scale, 3))};
+        if (scales[r] == 255)
+            rows[r] = (v4u)0x7FC07FC0u;
     }
+    store_transposed(rows, t.dst + (size_t)c0 * t.ld + r0, t.ld, k - c0);
 }
 
-__device__ __forceinline__ void transpose_dy(uint16_t *tile, const Prepared &p)
+template <int DPP>
+__device__ __forceinline__ float lanes(float v)
 {
-    const int r0 = blockIdx.x * kTile, c0 = blockIdx.y * kTile;
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), DPP, 0xF, 0xF, true));
+}
+
+template <int DOWN>
+__device__ __forceinline__ void transpose_dy(const Prepared &p)
+{
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = (blockIdx.x * DOWN + wave / kTilesAcross) * kTile, c0 = (blockIdx.y * kTilesAcross + wave % kTilesAcross) * kTile;
     if (r0 >= p.rows || c0 >= p.cols)
         return;
+    const int row = r0 + (lane & 7) * 8, col = c0 + (lane >> 3) * 8;
+    v4u rows[8];
+    if (p.cols >= 8) {
+        // Eight elements at once, aligned to the element only (the hardware splits such loads); at a row's end the row's last
+        // eight, shifted to their places.
+        const int over = max(col + 8 - p.cols, 0);
 #pragma unroll
-    for (int h = 0; h < kTile * kTile / kThreads; ++h) {
-        const int i = threadIdx.x + h * kThreads;
-        const int r = i >> 6, c = i & 63;
-        const uint16_t v = r0 + r < p.rows && c0 + c < p.cols ? p.dy[(size_t)(r0 + r) * p.cols + c0 + c] : (uint16_t)0;
-        tile[c * kTileStride + r] = v;
-        if (p.padded && r0 + r < p.rows && (size_t)(c0 + c) < p.ld_p)
-            p.padded[(size_t)(r0 + r) * p.ld_p + c0 + c] = v;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int i = threadIdx.x + h * kThreads;
-        const int c = i >> 3, r = (i & 7) * 8;
-        v8us out;
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            out[e] = tile[c * kTileStride + r + e];
-            sum += __builtin_bit_cast(float, (unsigned)out[e] << 16);
+        for (int r = 0; r < 8; ++r) {
+            rows[r] = (v4u)0u;
+            if (row + r < p.rows)
+                __builtin_memcpy(&rows[r], p.dy + (size_t)(row + r) * p.cols + (col - over), 16);
         }
-        if (p.transposed && c0 + c < p.cols)
-            *(v8us *)(p.transposed + (size_t)(c0 + c) * p.ld_t + r0 + r) = out;
-        if (p.partial) {
+        if (over) {
 #pragma unroll
-            for (int s = 1; s < 8; s *= 2)
-                sum += __shfl_xor(sum, s);
-            if ((i & 7) == 0 && c0 + c < p.cols)
-                p.partial[(size_t)blockIdx.x * p.cols + c0 + c] = sum;
+            for (int r = 0; r < 8; ++r)
+                rows[r] = over < 8 ? __builtin_bit_cast(v4u, __builtin_bit_cast(unsigned __int128, rows[r]) >> (16 * over)) : (v4u)0u;
+        }
+    } else {
+        unsigned __int128 v[8] = {};
+#pragma unroll 1
+        for (int c = p.cols - 1; c >= 0 && col == 0; --c)
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                v[r] = v[r] << 16 | (row + r < p.rows ? p.dy[(size_t)(row + r) * p.cols + c] : (uint16_t)0);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            rows[r] = __builtin_bit_cast(v4u, v[r]);
+    }
+    if (p.padded && (size_t)col < p.ld_p) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (row + r < p.rows)
+                *(v4u *)(p.padded + (size_t)(row + r) * p.ld_p + col) = rows[r];
+    }
+    if (p.transposed)
+        store_transposed(rows, p.transposed + (size_t)c0 * p.ld_t + r0, p.ld_t, p.cols - c0);
+    if (p.partial) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                sum += __builtin_bit_cast(float, c & 1 ? rows[r][c / 2] & 0xFFFF0000u : rows[r][c / 2] << 16);
+            sum += lanes<0xB1>(sum);   // 1 0 3 2
+            sum += lanes<0x4E>(sum);   // 2 3 0 1
+            sum += lanes<0x141>(sum);  // 7 .. 0: the other quad's
+            if ((lane & 7) == 0 && col + c < p.cols)
+                p.partial[(size_t)(r0 / kTile) * p.cols + col + c] = sum;
         }
     }
 }
 
-// blockIdx.z: one of the matrices, or dy behind them.
-__global__ __launch_bounds__(kThreads) void prepare_kernel(Prepared p, size_t code_stride, size_t scale_stride)
+// blockIdx.z: one of the matrices, or dy behind them.  A workgroup takes DOWN x kTilesAcross tiles.
+template <int DOWN>
+__global__ __launch_bounds__(DOWN *kTilesAcross * 64) void prepare_kernel(Prepared p, size_t code_stride, size_t scale_stride)
 {
-    __shared__ uint16_t tile[kTile * kTileStride];
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
-        for (int i = threadIdx.x; i < p.zero_count; i += kThreads)
+        for (int i = threadIdx.x; i < p.zero_count; i += DOWN * kTilesAcross * 64)
             p.zeros[i] = 0;
     if ((int)blockIdx.z < p.matrices)
-        transpose_matrix(tile, p.matrix[blockIdx.z], p.k, code_stride, scale_stride);
+        transpose_matrix<DOWN>(p.matrix[blockIdx.z], p.k, code_stride, scale_stride);
     else
-        transpose_dy(tile, p);
+        transpose_dy<DOWN>(p);
 }
 
 // 64 columns per workgroup; the waves take every fourth row each, and their sums are added in order.
@@ -342,6 +388,11 @@ hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld,
     }
 }
 
+// From a tile of 256 x 256 for each CU on, workgroups of 16 waves, whose tiles' rows are written 512 bytes at a time; below, of 4,
+// which come to more CUs.  (us, 4 waves or 16: x, w and dy of 4096 x 4096 x 14336 106, 91; two weights of 14336 x 4096 and x 106, 102-108;
+// 257 x 1400 x 1000 6.2, 9.2; 130 x 1001 x 515 6.7, 9.)
+constexpr long kLargeTranspose = 256l * 256 * 256;
+
 hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
 {
     int rows = p.dy ? p.rows : 0, cols = p.dy ? p.cols : 0;
@@ -351,8 +402,15 @@ hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
     }
     if (rows == 0 || cols == 0)
         return hipSuccess;
-    const dim3 grid((unsigned)((rows + kTile - 1) / kTile), (unsigned)((cols + kTile - 1) / kTile), (unsigned)(p.matrices + (p.dy != nullptr)));
-    prepare_kernel<<<grid, kThreads, 0, stream>>>(p, mx_code_stride(p.k), mx_scale_stride(p.k));
+    auto run = [&](auto down) {
+        constexpr int DOWN = decltype(down)::value, kSide = DOWN * kTile, kWide = kTilesAcross * kTile;
+        const dim3 grid((unsigned)((rows + kSide - 1) / kSide), (unsigned)((cols + kWide - 1) / kWide), (unsigned)(p.matrices + (p.dy != nullptr)));
+        prepare_kernel<DOWN><<<grid, DOWN * kTilesAcross * 64, 0, stream>>>(p, mx_code_stride(p.k), mx_scale_stride(p.k));
+    };
+    if ((long)rows * cols >= kLargeTranspose)
+        run(std::integral_constant<int, 4>{});
+    else
+        run(std::integral_constant<int, 1>{});
     return hipGetLastError();
 }
 

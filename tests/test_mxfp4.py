@@ -289,7 +289,7 @@ def test_gated(gpu, m, n, k, kind):
     assert torch.equal(got[:, n:], torch.zeros(m, 32 * blocks - n, dtype=torch.float64))
 
 
-BACKWARD = [(1000, 64, 64), (2500, 40, 72), (64, 2000, 64), (700, 130, 40), (40, 900, 520), (1, 1, 1), (1, 64, 256), (3, 65, 40), (16, 128, 300), (64, 64, 64), (65, 130, 257), (100, 300, 100), (130, 257, 515), (192, 320, 512)]
+BACKWARD = [(70, 5, 40), (75, 15, 40), (1000, 64, 64), (2500, 40, 72), (64, 2000, 64), (700, 130, 40), (40, 900, 520), (1, 1, 1), (1, 64, 256), (3, 65, 40), (16, 128, 300), (64, 64, 64), (65, 130, 257), (100, 300, 100), (130, 257, 515), (192, 320, 512)]
 
 
 @pytest.mark.gpu
@@ -316,6 +316,23 @@ def test_linear_backward(gpu, m, n, k, dw_type):
         args = [p if j == i else None for j, p in enumerate(parts)]
         lib.mxfp4_linear_backward(dy.cuda(), *xq, *wq, args[0], args[1], dw_type, args[2], work, m, n, k)
     assert all(torch.equal(a, b) for a, b in zip(parts, (dx, dw, db)))
+
+
+@pytest.mark.gpu
+def test_gradients_read_every_scale_and_code(gpu):
+    """dx = I w: every value that a code and a scale from 2^-127 to 2^125 stand for is a bfloat16 number and comes out."""
+    n = 253
+    codes, scales = torch.zeros(n, 128, dtype=torch.uint8), torch.zeros(n, 16, dtype=torch.uint8)
+    codes[:, :16] = torch.tensor([16 * (i % 8 * 2 + 1) + i % 8 * 2 for i in range(16)], dtype=torch.uint8)
+    scales[:, 0] = torch.arange(n)
+    size = lib.mxfp4_linear_backward_bytes(n, n, 32)
+    work, dx = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(n, 32, dtype=torch.bfloat16, device="cuda")
+    args = (torch.eye(n, dtype=torch.bfloat16).cuda(), codes.cuda(), scales.cuda(), codes.cuda(), scales.cuda())
+    lib.mxfp4_linear_backward(*args, dx, None, "f32", None, work, n, n, 32)
+    assert torch.equal(dx.cpu().double(), ref.decode(codes, scales, 32))
+    args[4][7, 0] = 255
+    lib.mxfp4_linear_backward(*args, dx, None, "f32", None, work, n, n, 32)
+    assert bool(torch.isnan(dx).all())
 
 
 @pytest.mark.gpu
