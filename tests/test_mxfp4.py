@@ -336,6 +336,36 @@ def test_gradients_read_every_scale_and_code(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(6390, 4090, 4860), (6390, 2800, 2810), (2810, 6390, 2800), (4096, 2048, 2816)])
+def test_gradients_of_large_layers_with_integers(gpu, m, n, k):
+    """Sums of integers below 2^24 are exact in any order: whole tiles, shared ones and both float outputs have to hit them."""
+    r = torch.Generator().manual_seed(m + n + k)
+    value = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], device="cuda") * 2
+
+    def integers(rows):
+        codes, scales = torch.zeros(rows, ref.code_stride(k), dtype=torch.uint8), torch.zeros(rows, ref.scale_stride(k), dtype=torch.uint8)
+        codes[:, : k // 2] = torch.randint(0, 256, (rows, k // 2), generator=r, dtype=torch.uint8)
+        scales[:, : (k + 31) // 32] = 128
+        codes, scales = codes.cuda(), scales.cuda()
+        low, high = codes[:, : k // 2].long() & 15, codes[:, : k // 2].long() >> 4
+        return (codes, scales), value[torch.stack([low, high], 2).view(rows, k)]
+
+    (xq, x), (wq, w) = integers(m), integers(n)
+    dy = torch.randint(-8, 9, (m, n), generator=r).float().cuda()
+    work = torch.empty(lib.mxfp4_linear_backward_bytes(m, n, k), dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        dx, dw = torch.empty(m, k, dtype=torch.bfloat16, device="cuda"), torch.empty(n, k, device="cuda")
+        db = torch.empty(n, device="cuda")
+        lib.mxfp4_linear_backward(dy.bfloat16(), *xq, *wq, dx, dw, "f32", db, work, m, n, k)
+        assert torch.equal(dw, dy.T.contiguous() @ x)
+        assert torch.equal(dx, (dy @ w).bfloat16())
+        assert torch.equal(db, dy.sum(0))
+        dw16 = torch.empty(n, k, dtype=torch.bfloat16, device="cuda")
+        lib.mxfp4_linear_backward(dy.bfloat16(), *xq, *wq, None, dw16, "bf16", None, work, m, n, k)
+        assert torch.equal(dw16, dw.bfloat16())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m, n, k", BACKWARD)
 @pytest.mark.parametrize("kind", ["silu", "gelu"])
 def test_gated_backward(gpu, m, n, k, kind):
