@@ -55,7 +55,8 @@ enum {
     INT4LINEAR_ERR_NO_DEVICE = 6,   /* no gfx950 device is visible                       */
     INT4LINEAR_ERR_SCRATCH = 7,     /* int4linear_gemm_s4s4s32_static: the only fast kernel
                                        for the shape needs more scratch memory than
-                                       INT4LINEAR_STATIC_SCRATCH_BYTES                   */
+                                       INT4LINEAR_STATIC_SCRATCH_BYTES; the MXFP4 gradients:
+                                       work_bytes is too small                           */
     INT4LINEAR_ERR_NOT_INITIALISED = 8 /* first call on this device while its stream is being
                                        captured: call int4linear_init() before capturing */
 };
@@ -241,7 +242,9 @@ int int4linear_mxfp4_gated_quantized(const void *x_codes_d, const void *x_scales
  *   dx (m x k, bfloat16) = dy W,  dw (n x k, dw_type) = dy^T X,  dbias (n floats) = column sums of dy.
  * dy_d is m x n bfloat16, contiguous, 16-byte aligned like dx_d and dw_d; dx_d, dw_d and dbias_d may
  * each be NULL (not wanted).  dw_type: INT4LINEAR_OUT_BF16 or _F32.  work_d: a 256-byte aligned device
- * buffer of at least int4linear_mxfp4_linear_backward_bytes(m, n, k) bytes, else INT4LINEAR_ERR_SCRATCH. */
+ * buffer of at least int4linear_mxfp4_linear_backward_bytes(m, n, k) bytes, else INT4LINEAR_ERR_SCRATCH; what
+ * it holds before does not matter, and two calls that may overlap need one each.  Results are the same bits from
+ * call to call, whichever of them are wanted. */
 size_t int4linear_mxfp4_linear_backward_bytes(int m, int n, int k);
 int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, const void *x_scales_d,
                                      const void *w_codes_d, const void *w_scales_d, void *dx_d, void *dw_d,

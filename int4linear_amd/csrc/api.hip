@@ -95,7 +95,7 @@ hipError_t set_up_device(PerDevice &pd, int dev)
 }
 
 // Set-up for the device that is current on the calling thread; returns its record.  Set-up
-// queries the device, raises the dynamic-LDS limit of some 400 kernels and takes the address
+// queries the device, raises the dynamic-LDS limit of some 450 kernels and takes the address
 // of the scratch arrays (which loads the device image): none of that belongs inside a graph
 // capture, so a first call that arrives with `work_stream` capturing is refused
 // (`for_work`: the call is about to enqueue work on work_stream).
@@ -649,7 +649,8 @@ const char *int4linear_status_string(int status)
     case INT4LINEAR_ERR_NOT_INITIALISED:
         return "first call on this device came while its stream was being captured: call int4linear_init() before the capture";
     case INT4LINEAR_ERR_SCRATCH:
-        return "only a kernel with more scratch memory than the static array of int4linear_gemm_s4s4s32_static holds is fast for this shape";
+        return "only a kernel with more scratch memory than the static array of int4linear_gemm_s4s4s32_static holds is fast for this shape, "
+               "or a gradient's workspace is smaller than its _bytes function says";
     default:
         return "unknown status";
     }

@@ -1,5 +1,6 @@
 """MXFP4 operators: refusals and sizes (CPU), and their results on the device against float64."""
 import math
+from pathlib import Path
 
 import pytest
 import torch
@@ -500,3 +501,28 @@ def test_a_block_captured_into_a_graph(gpu):
         block()
         torch.cuda.synchronize()
         assert got.any() and torch.equal(got, y)
+
+
+@pytest.mark.gpu
+def test_the_example_learns_and_serves(gpu):
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("mxfp4_feed_forward", Path(__file__).resolve().parent.parent / "examples" / "mxfp4_feed_forward.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    x = torch.randn(96, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).bfloat16()
+    target = example.FeedForward(96, 128, 320, seed=2).forward(x).float()
+    block = example.FeedForward(96, 128, 320)
+    losses = example.train(block, x, target, 40, 0.02)
+    assert losses[-1] < losses[0] / 2
+    token = x[:1].clone()
+    want = [block.forward(x[i : i + 1].contiguous()).clone() for i in range(4)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = block.forward(token)
+    for i in range(4):
+        token.copy_(x[i : i + 1])
+        graph.replay()
+        assert torch.equal(y, want[i])
+        block.forward(x)  # eager work between the replays
+        torch.cuda.synchronize()
