@@ -74,8 +74,8 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const typename El
     typedef T v8t __attribute__((ext_vector_type(8)));
     const int lane = threadIdx.x & 63;
     const long items = (long)rows * segments;
-    const long waves = (long)gridDim.x * (kThreads / 64);
-    const long first = (long)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long waves = (long)gridDim.x * gridDim.y * (kThreads / 64);
+    const long first = ((long)blockIdx.y * gridDim.x + blockIdx.x) * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     v8t in[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const uint8_t *
     typedef T v8t __attribute__((ext_vector_type(8)));
     const int lane = threadIdx.x & 63;
     const long items = (long)rows * segments;
-    const long waves = (long)gridDim.x * (kThreads / 64);
-    const long first = (long)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long waves = (long)gridDim.x * gridDim.y * (kThreads / 64);
+    const long first = ((long)blockIdx.y * gridDim.x + blockIdx.x) * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned c[kUnroll], s[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -330,11 +330,13 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSums s)
         s.sums[c] = ((part[threadIdx.x] + part[threadIdx.x + 64]) + part[threadIdx.x + 128]) + part[threadIdx.x + 192];
 }
 
-int conversion_grid(int rows, int segments)
+// (A launch holds fewer than 2^32 threads along x.)
+dim3 conversion_grid(int rows, int segments)
 {
+    constexpr size_t kMostAlongX = 1 << 22;
     const size_t items = (size_t)rows * segments;
-    const size_t per_group = (size_t)kUnroll * (kThreads / 64);
-    return (int)((items + per_group - 1) / per_group);
+    const size_t per_group = (size_t)kUnroll * (kThreads / 64), groups = (items + per_group - 1) / per_group;
+    return dim3((unsigned)min(groups, kMostAlongX), (unsigned)((groups + kMostAlongX - 1) / kMostAlongX));
 }
 
 template <int TYPE>

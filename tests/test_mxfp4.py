@@ -454,6 +454,21 @@ def test_large_offsets(gpu):
 
 
 @pytest.mark.gpu
+def test_conversion_of_very_many_rows(gpu):
+    """More rows than one axis of a launch holds; every value is represented exactly."""
+    rows, k = (1 << 28) + 5, 3
+    x = torch.randint(0, 4, (rows, k), dtype=torch.int8, device="cuda").bfloat16()
+    x = torch.where(x == 3, 4.0, x).bfloat16()
+    codes = torch.full((lib.mxfp4_code_bytes(rows, k),), 0x77, dtype=torch.uint8, device="cuda")
+    scales = torch.full((lib.mxfp4_scale_bytes(rows, k),), 0x77, dtype=torch.uint8, device="cuda")
+    lib.mxfp4_quantize(x, codes, scales, rows, k)
+    y = torch.empty_like(x)
+    lib.mxfp4_dequantize(codes, scales, y, rows, k)
+    assert torch.equal(x, y)
+    assert not codes.view(rows, -1)[-3:, 2:].any() and not scales.view(rows, -1)[-3:, 1:].any()
+
+
+@pytest.mark.gpu
 def test_results_do_not_change_from_call_to_call(gpu):
     """No atomics, no order that depends on timing: the same bits every time, on any stream."""
     m, n, k = 130, 300, 1100
