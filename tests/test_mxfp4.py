@@ -519,6 +519,37 @@ def test_a_block_captured_into_a_graph(gpu):
 
 
 @pytest.mark.gpu
+def test_gradients_captured_into_a_graph(gpu):
+    """Long sums in slices, whose counters every call clears: each replay gives the eager call's bits."""
+    m, n, k = 70, 900, 520
+    (xq, _), (gq, _), (uq, _), (wq, _) = matrix(1, m, k), matrix(2, n, k, 0.1), matrix(3, n, k, 0.1), matrix(4, n, k, 0.1)
+    dh = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    bytes_needed = lib.mxfp4_linear_backward_bytes(m, n, k), lib.mxfp4_gated_backward_bytes(m, n, k)
+    work = torch.full((max(bytes_needed),), 0xFF, dtype=torch.uint8, device="cuda")
+    outs = [torch.empty(m, k, dtype=torch.bfloat16, device="cuda") for _ in range(2)] + [torch.empty(n, k, device="cuda") for _ in range(3)]
+    outs.append(torch.empty(n, device="cuda"))
+
+    def step():
+        lib.mxfp4_linear_backward(dh, *xq, *wq, outs[0], outs[2], "f32", outs[5], work, m, n, k)
+        lib.mxfp4_gated_backward(dh, *xq, *gq, *uq, outs[1], outs[3], outs[4], "f32", work, m, n, k)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in range(4):
+        dh.copy_(torch.randn(m, n, generator=torch.Generator().manual_seed(seed)))
+        work.fill_(0xFF)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for t in outs:
+            t.zero_()
+        step()
+        torch.cuda.synchronize()
+        assert all(bool(a.any()) and torch.equal(a, b) for a, b in zip(got, outs))
+
+
+@pytest.mark.gpu
 def test_the_example_learns_and_serves(gpu):
     import importlib.util
 
