@@ -52,7 +52,8 @@ __device__ __forceinline__ void activate_with_slope(int act, float g, float &val
 {
     const float s = logistic(act == kSilu ? g : kGeluScale * (g + kGeluCubic * g * g * g));
     value = g * s;
-    slope = s + g * s * (1.0f - s) * (act == kSilu ? 1.0f : kGeluScale * (1.0f + 3.0f * kGeluCubic * g * g));
+    // (g^2 stays finite: far out its factor s (1 - s) is 0)
+    slope = s + g * s * (1.0f - s) * (act == kSilu ? 1.0f : kGeluScale * (1.0f + 3.0f * kGeluCubic * fminf(g * g, 1e30f)));
 }
 
 // Eight values as E2M1 codes, the first in the lowest four bits.  The hardware's conversion rounds to nearest

@@ -413,6 +413,25 @@ def test_gated_gradients_against_differences(gpu, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_gated_at_gates_whose_square_is_no_float(gpu, kind):
+    """g = 2^65, 0 and -2^65: act is g, 0 and 0, its slope 1, 1/2 and 0."""
+    x, wg, wu = torch.zeros(1, 32).double(), torch.zeros(3, 32).double(), torch.full((3, 32), 3.0).double()
+    x[0, 0], wg[0, 0], wg[2, 0] = 1.0, 2.0**65, -(2.0**65)
+    (xq, gq, uq) = ([t.cuda() for t in ref.encode(v)] for v in (x, wg, wu))
+    h, dh = torch.empty(1, 3, device="cuda"), torch.ones(1, 3, dtype=torch.bfloat16, device="cuda")
+    lib.mxfp4_gated(*xq, *gq, *uq, h, "f32", 1, 3, 32, activation=kind)
+    assert h.tolist() == [[3 * 2.0**65, 0.0, 0.0]]
+    dx, dwg, dwu = torch.empty(1, 32, dtype=torch.bfloat16, device="cuda"), *torch.empty(2, 3, 32, device="cuda")
+    work = torch.empty(lib.mxfp4_gated_backward_bytes(1, 3, 32), dtype=torch.uint8, device="cuda")
+    lib.mxfp4_gated_backward(dh, *xq, *gq, *uq, dx, dwg, dwu, "f32", work, 1, 3, 32, activation=kind)
+    assert dwg[:, 0].tolist() == [3.0, 1.5, 0.0] and dwu[:, 0].tolist() == [2.0**65, 0.0, 0.0]
+    assert not dwg[:, 1:].any() and not dwu[:, 1:].any()
+    # (the columns behind the first: du wu alone)
+    assert dx[0, 0].item() == 6 * 2.0**65 and bool((dx[0, 1:] == 3 * 2.0**65).all())
+
+
+@pytest.mark.gpu
 def test_gradients_of_empty_sums(gpu):
     (xq, _), (wq, _) = matrix(1, 5, 40), matrix(2, 6, 40)
     dw, db = torch.full((6, 40), 7.0, device="cuda"), torch.full((6,), 7.0, device="cuda")
