@@ -50,23 +50,20 @@ struct LineOperands {
 // kPair: two operands b share the tile, blocks i even of the first, odd of the second, each pair over the same
 // 32 columns.
 
-// A lane's 16 columns of a row (kColumns = false), rounded to 16 bits -> 8 columns from 8 * (lane / 32) on
-// in out[0], from 16 + 8 * (lane / 32) on in out[1].
+// Elements 8 * half .. of a lane's 16 columns of a row (kColumns = false), rounded to 16 bits -> 8 columns from
+// 16 * half + 8 * (lane / 32) on.
 template <int OUT>
-__device__ __forceinline__ void gather_row(const float (&v)[16], v4i (&out)[2])
+__device__ __forceinline__ v4i gather_row(const float *v)
 {
     using T = OutElement<OUT>;
     typedef T v2t __attribute__((ext_vector_type(2)));
-    int p[8];
+    int p[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 4; ++e)
         p[e] = __builtin_bit_cast(int, (v2t){(T)v[2 * e], (T)v[2 * e + 1]});
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const auto x = __builtin_amdgcn_permlane32_swap(p[4 * half], p[4 * half + 2], false, false);
-        const auto y = __builtin_amdgcn_permlane32_swap(p[4 * half + 1], p[4 * half + 3], false, false);
-        out[half] = (v4i){(int)x[0], (int)y[0], (int)x[1], (int)y[1]};
-    }
+    const auto x = __builtin_amdgcn_permlane32_swap(p[0], p[2], false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(p[1], p[3], false, false);
+    return (v4i){(int)x[0], (int)y[0], (int)x[1], (int)y[1]};
 }
 
 // The 16 results v of a lane's part of a block of y (ld elements between rows) at (row, col).
@@ -87,8 +84,7 @@ __device__ __forceinline__ void store_block(void *y, size_t ld, int m, int n, in
             }
         }
     } else {
-        v4i out[2];
-        gather_row<OUT>(v, out);
+        const v4i out[2] = {gather_row<OUT>(v), gather_row<OUT>(v + 8)};
         const int r = row + (lane & 31), c = col + 8 * (lane >> 5);
         dst += (size_t)r * ld + c;
         if (r < m) {  // (n is a multiple of 8)
@@ -225,51 +221,67 @@ struct GradientEpilogue {
     template <int FM, int FN>
     __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
-        // (all loads first: behind one another they cost a way to memory each)
+        // (All loads first, where there are registers for them: behind one another they cost a way to memory each.)
+        constexpr bool kAhead = FM * FN > 4;
         v4bf in[FM][FN / 2][4];
+        auto fetch = [&](int j, int i, int q) {
+            const int r = row + kFrag * j + (lane & 31), c = col + kFrag * i + 8 * q + 4 * (lane >> 5);
+            in[j][i][q] = (v4bf){};
+            if (r < m) {
+                const __bf16 *src = dh + (size_t)r * n + c;
+                if (vec) {
+                    if (c < n)
+                        in[j][i][q] = *(const v4bf *)src;
+                } else {
 #pragma unroll
-        for (int j = 0; j < FM; ++j)
-#pragma unroll
-            for (int i = 0; i < FN / 2; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int r = row + kFrag * j + (lane & 31), c = col + kFrag * i + 8 * q + 4 * (lane >> 5);
-                    in[j][i][q] = (v4bf){};
-                    if (r < m) {
-                        const __bf16 *src = dh + (size_t)r * n + c;
-                        if (vec) {
-                            if (c < n)
-                                in[j][i][q] = *(const v4bf *)src;
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (c + e < n)
-                                    in[j][i][q][e] = src[e];
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < n)
+                            in[j][i][q][e] = src[e];
                 }
+            }
+        };
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+#pragma unroll
+                for (int i = 0; i < FN / 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        fetch(j, i, q);
+        }
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
             const int r = row + kFrag * j + (lane & 31);
 #pragma unroll
             for (int i = 0; i < FN; i += 2) {
                 const int c0 = col + kFrag * (i / 2);
-                float dg[16], du[16];
 #pragma unroll
-                for (int t = 0; t < 16; ++t) {
-                    float value, slope;
-                    activate_with_slope(act, acc[j][i][t], value, slope);
-                    // padding: exact zeros, whatever the clamped rows gave
-                    const bool there = r < m && c0 + 8 * (t / 4) + 4 * (lane >> 5) + t % 4 < n;
-                    const float g = (float)in[j][i / 2][t / 4][t % 4];
-                    dg[t] = there ? g * acc[j][i + 1][t] * slope : 0.0f;
-                    du[t] = there ? g * value : 0.0f;
-                }
-                store_block<kOutBF16, false>(d, 2 * ld_n, m, (int)ld_n, row + kFrag * j, c0, lane, dg);
-                store_block<kOutBF16, false>(d + ld_n, 2 * ld_n, m, (int)ld_n, row + kFrag * j, c0, lane, du);
-                if ((size_t)r < ld_m) {
-                    store_transposed(dt, r, c0, lane, dg);
-                    store_transposed(dt + (size_t)n * ld_m, r, c0, lane, du);
+                for (int half = 0; half < 2; ++half) {
+                    float dg[8], du[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int t = 8 * half + e;
+                        if (!kAhead && t % 4 == 0)
+                            fetch(j, i / 2, t / 4);
+                        float value, slope;
+                        activate_with_slope(act, acc[j][i][t], value, slope);
+                        // padding: exact zeros, whatever the clamped rows gave
+                        const bool there = r < m && c0 + 8 * (t / 4) + 4 * (lane >> 5) + t % 4 < n;
+                        const float g = (float)in[j][i / 2][t / 4][t % 4];
+                        dg[e] = there ? g * acc[j][i + 1][t] * slope : 0.0f;
+                        du[e] = there ? g * value : 0.0f;
+                    }
+                    const v4i g8 = gather_row<kOutBF16>(dg), u8 = gather_row<kOutBF16>(du);
+                    const int c = c0 + 16 * half + 8 * (lane >> 5);
+                    if (r < m && (size_t)c < ld_n) {
+                        __bf16 *to = d + (size_t)r * 2 * ld_n + c;
+                        *(v4i *)to = g8;
+                        *(v4i *)(to + ld_n) = u8;
+                    }
+                    if ((size_t)r < ld_m) {
+                        store_transposed(dt, r, c0 + 16 * half, lane, dg);
+                        store_transposed(dt + (size_t)n * ld_m, r, c0 + 16 * half, lane, du);
+                    }
                 }
             }
         }
@@ -278,12 +290,12 @@ struct GradientEpilogue {
     // The transposes.  A quad's 4 rows x 4 columns change places, twice: between neighbours, then between pairs.  A lane then has four rows of
     // column lane % 4 of each four: 8 bytes a store.  (With stores of 2 bytes, and dh fetched block by block, 4096 x 14336 x 4096 takes
     // 466 us, so 400; the product alone with h as its result 275.)
-    __device__ __forceinline__ void store_transposed(__bf16 *to, int r, int c0, int lane, const float (&v)[16]) const
+    __device__ __forceinline__ void store_transposed(__bf16 *to, int r, int c0, int lane, const float (&v)[8]) const
     {
         const unsigned halves = lane & 1 ? 0x03020706u : 0x05040100u;
         const bool upper = lane & 2;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
             unsigned two[2];  // rows r & ~1, r | 1 of column 2 i + lane % 2 of the four
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
