@@ -1014,14 +1014,16 @@ static hipError_t launch_group(const LineGroup &g, const EpW &ep_w, const EpX &e
     return hipGetLastError();
 }
 
+constexpr int kMostTogether = 1536;
+
 // How long a slice of k is at least, in stages: meeting costs as much as about six.
 constexpr int kLeastSlice = 6;
 
 hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const SliceSpace &space, const DeviceInfo &dev,
                                 hipStream_t stream)
 {
-    // Together where kMostSlices workgroups hold all tiles of 64 x 64: beyond that each fills the device alone, on larger
-    // tiles.  Long k is cut into slices as far as they go.  (Backward pass of a gated layer, 257 x 1400 x 1000, and of a linear one,
+    // Together up to three rounds of tiles of 64 x 64 (us apart and together: 700 x 2000 x 1000, gated, 1200 tiles 60, 54; 1000 x 2000 x 2000,
+    // linear, 1536 tiles 51, 48; 2048^3, 2048 tiles 66, 70): beyond that each fills the device alone, on larger tiles.  Long k is cut into slices as far as they go.  (Backward pass of a gated layer, 257 x 1400 x 1000, and of a linear one,
     // 130 x 1001 x 515: a launch for each product and operand 39 and 27 us, grouped 33 and 14, with slices 29 and 14: the
     // gated products 21 us, with dx in four slices 17.)
     long tiles = 0;
@@ -1030,7 +1032,7 @@ hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSum
         tiles += ((p[i].m + 63l) / 64) * ((p[i].n + 63l) / 64);
         together = together && p[i].k > 0 && p[i].n == p[0].n && (i == count - 1 || p[i].out == p[0].out);
     }
-    if (!together || tiles > kMostSlices) {
+    if (!together || tiles > kMostTogether) {
         hipError_t e = hipSuccess;
         for (int i = 0; i < count && e == hipSuccess; ++i)
             if (p[i].y)

@@ -337,7 +337,7 @@ def test_gradients_read_every_scale_and_code(gpu):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m, n, k", [(6390, 4090, 4860), (6390, 2800, 2810), (2810, 6390, 2800), (4096, 2048, 2816)])
+@pytest.mark.parametrize("m, n, k", [(6390, 4090, 4860), (6390, 2800, 2810), (2810, 6390, 2800), (4096, 2048, 2816), (1000, 2000, 1990), (1030, 2000, 1990)])
 def test_gradients_of_large_layers_with_integers(gpu, m, n, k):
     """Sums of integers below 2^24 are exact in any order: whole tiles, shared ones and both float outputs have to hit them."""
     r = torch.Generator().manual_seed(m + n + k)
