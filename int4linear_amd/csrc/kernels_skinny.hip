@@ -113,7 +113,11 @@ __device__ __forceinline__ unsigned uniform(unsigned v) { return (unsigned)__bui
 __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p)
 {
     const unsigned long long v = (unsigned long long)p;
-    return (const uint8_t *)((unsigned long long)uniform((unsigned)v) | ((unsigned long long)uniform((unsigned)(v >> 32)) << 32));
+    unsigned long long s = (unsigned long long)uniform((unsigned)v) | ((unsigned long long)uniform((unsigned)(v >> 32)) << 32);
+    // The hardware lets a load read a scalar register up to five instructions after a vector instruction (the
+    // readfirstlane) wrote it without waiting; the compiler keeps them apart for its own loads, not for those above.
+    asm volatile("s_nop 4" : "+s"(s));
+    return (const uint8_t *)s;
 }
 
 // f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
