@@ -18,7 +18,8 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p)
 
 // 16 bytes per lane from base + offset straight into LDS at to + 16 * lane (NT: read once).  A load may read a scalar
 // register no sooner than five instructions after a vector instruction wrote it (a reload of a spilled one, say), which the
-// compiler sees to for its own loads only: hence the long s_nop.
+// compiler sees to for its own loads only: hence the long s_nop.  (M0 is reserved: the compiler keeps nothing there, refuses it
+// among the clobbers, and has no instruction in these kernels that would read it.)
 template <bool NT = false>
 __device__ __forceinline__ void dma16(const void *base, unsigned offset, unsigned to)
 {

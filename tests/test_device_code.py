@@ -79,15 +79,54 @@ def test_the_reader_of_device_code_sees_an_early_read():
     assert not early_reads(["v_readfirstlane_b32 s6, v18", load]) and not early_reads(["s_mov_b32 s4, s5", load])
 
 
-def test_no_load_reads_a_scalar_register_that_is_still_being_written(tmp_path):
+@pytest.fixture(scope="module")
+def device_code(tmp_path_factory):
+    """The lines of every code object of the built library."""
     if not Path(OBJDUMP).exists():
         pytest.skip("no llvm-objdump here")
-    objects = list(code_objects(build.LIB_PATH.read_bytes()))
-    assert len(objects) >= 10  # a code object for every file with kernels
-    found = []
-    for i, code in enumerate(objects):
-        (tmp_path / f"{i}.co").write_bytes(code)
-        text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", "--no-leading-addr", str(tmp_path / f"{i}.co")], check=True,
-                              stdout=subprocess.PIPE, text=True).stdout
-        found += early_reads(text.splitlines())
+    out = []
+    for code in code_objects(build.LIB_PATH.read_bytes()):
+        path = tmp_path_factory.mktemp("code") / "object.co"
+        path.write_bytes(code)
+        out.append(subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", "--no-leading-addr", str(path)], check=True,
+                                  stdout=subprocess.PIPE, text=True).stdout.splitlines())
+    assert len(out) >= 10  # one for every file with kernels
+    return out
+
+
+def test_no_load_reads_a_scalar_register_that_is_still_being_written(device_code):
+    found = [f for lines in device_code for f in early_reads(lines)]
     assert not found, f"{len(found)} loads, the first: {found[0]}"
+
+
+def other_uses_of_m0(lines):
+    """Instructions with M0 other than a load to LDS (which reads its address there) and, one wait state before it, the write
+    that belongs to it."""
+    code = [line.split("//")[0].strip() for line in lines]
+    code = [line for line in code if line]
+    found, mine = [], set()
+    for i, line in enumerate(code):
+        if line.startswith("global_load_lds_"):
+            mine.add(i - 2)
+            if not (re.match(r"s_(mov_b32|add_u32) m0, ", code[i - 2]) and code[i - 1].startswith("s_nop ")):
+                found.append(line)
+    for i, line in enumerate(code):
+        if i not in mine and (re.search(r"\bm0\b", line) or re.match(r"v_movrel|s_movrel|s_set_gpr_idx|v_interp|s_sendmsg|ds_gws", line)):
+            found.append(line)
+    return found
+
+
+def test_the_reader_of_device_code_sees_a_second_user_of_m0():
+    own = ["s_add_u32 m0, s8, 0x400", "s_nop 0", "global_load_lds_dwordx4 v4, s[4:5] nt"]
+    assert not other_uses_of_m0([*own, "s_add_u32 s8, s8, 1", *own])
+    for line in ("s_mov_b32 m0, s3", "v_movrels_b32_e32 v1, v2", "s_set_gpr_idx_on s3, gpr_idx(SRC0)", "v_readlane_b32 s3, v1, m0"):
+        assert other_uses_of_m0([*own, line, *own])
+    assert other_uses_of_m0(own[1:]) and other_uses_of_m0([own[0], own[2]])
+
+
+def test_nothing_but_the_loads_to_lds_uses_m0(device_code):
+    """The statements that load to LDS write M0 and cannot say so (the compiler reserves the register and warns of it in a list
+    of clobbers): nothing else may rely on what it holds."""
+    found = [f for lines in device_code for f in other_uses_of_m0(lines)]
+    assert not found, f"{len(found)} instructions, the first: {found[0]}"
+    assert sum(line.lstrip().startswith("global_load_lds_") for lines in device_code for line in lines) > 1000
