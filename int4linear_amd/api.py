@@ -15,14 +15,16 @@ from . import _lib
 KERNELS = {"auto": 0, "simple": 1, "mfma": 2, "skinny": 3, "fp6": 4, "mfma128": 5, "mfma256": 6}
 
 
+_HOST_KINDS = (int, np.ndarray)
+
+
 def _ptr(obj) -> int:
     """Device (or host) address of a torch tensor / numpy array / raw int."""
     if obj is None:
         return 0
-    try:
-        return obj.data_ptr()  # torch.Tensor, first: a call asks for up to ten, at 0.1 us each
-    except AttributeError:
-        return obj.ctypes.data if isinstance(obj, np.ndarray) else obj
+    if isinstance(obj, _HOST_KINDS):  # (one check for both: a call asks for up to ten tensors, at 0.2 us each)
+        return obj if isinstance(obj, int) else obj.ctypes.data
+    return obj.data_ptr()  # torch.Tensor
 
 
 def _current_stream() -> int:
