@@ -219,9 +219,13 @@ def mxfp4_gated_quantized(x_codes_d, x_scales_d, wg_codes_d, wg_scales_d, wu_cod
                                                     stream))
 
 
-def _work(work_d) -> tuple[int, int]:
-    """Address and bytes of a workspace: a tensor, or None."""
-    return (0, 0) if work_d is None else (work_d.data_ptr(), work_d.numel() * work_d.element_size())
+def _work(work_d, work_bytes: int | None) -> tuple[int, int]:
+    """Address and bytes of a workspace: a tensor, None, or an address, which needs work_bytes."""
+    if work_bytes is None:
+        if isinstance(work_d, int):
+            raise TypeError("a workspace given as an address needs work_bytes")
+        work_bytes = 0 if work_d is None else work_d.numel() * work_d.element_size()
+    return _ptr(work_d), work_bytes
 
 
 def mxfp4_linear_backward_bytes(m: int, n: int, k: int) -> int:
@@ -230,16 +234,16 @@ def mxfp4_linear_backward_bytes(m: int, n: int, k: int) -> int:
 
 
 def mxfp4_linear_backward(dy_d, x_codes_d, x_scales_d, w_codes_d, w_scales_d, dx_d, dw_d, dw_type: str, dbias_d, work_d,
-                          m: int, n: int, k: int, *, stream: int | None = None) -> None:
+                          m: int, n: int, k: int, *, work_bytes: int | None = None, stream: int | None = None) -> None:
     """dx (bfloat16) = dy W, dw (dw_type "bf16" or "f32") = dy^T X, dbias (float32) = column sums of dy
     (bfloat16); dx_d, dw_d and dbias_d may each be None.  work_d: a tensor of at least
-    mxfp4_linear_backward_bytes(m, n, k) bytes."""
+    mxfp4_linear_backward_bytes(m, n, k) bytes, or a device address with its work_bytes."""
     lib = _lib.load()
     if stream is None:
         stream = _current_stream()
     _lib.check(lib.int4linear_mxfp4_linear_backward(_ptr(dy_d), _ptr(x_codes_d), _ptr(x_scales_d), _ptr(w_codes_d),
                                                     _ptr(w_scales_d), _ptr(dx_d), _ptr(dw_d), OUT_TYPES[dw_type],
-                                                    _ptr(dbias_d), *_work(work_d), m, n, k, stream))
+                                                    _ptr(dbias_d), *_work(work_d, work_bytes), m, n, k, stream))
 
 
 def mxfp4_gated_backward_bytes(m: int, n: int, k: int) -> int:
@@ -249,17 +253,17 @@ def mxfp4_gated_backward_bytes(m: int, n: int, k: int) -> int:
 
 def mxfp4_gated_backward(dh_d, x_codes_d, x_scales_d, wg_codes_d, wg_scales_d, wu_codes_d, wu_scales_d, dx_d, dwg_d,
                          dwu_d, dw_type: str, work_d, m: int, n: int, k: int, *, activation: str = "silu",
-                         stream: int | None = None) -> None:
+                         work_bytes: int | None = None, stream: int | None = None) -> None:
     """Gradients of mxfp4_gated from dh (bfloat16): dx (bfloat16), dwg and dwu (dw_type "bf16" or "f32");
     dx_d, or dwg_d and dwu_d together, may be None.  work_d: a tensor of at least
-    mxfp4_gated_backward_bytes(m, n, k) bytes."""
+    mxfp4_gated_backward_bytes(m, n, k) bytes, or a device address with its work_bytes."""
     lib = _lib.load()
     if stream is None:
         stream = _current_stream()
     _lib.check(lib.int4linear_mxfp4_gated_backward(_ptr(dh_d), _ptr(x_codes_d), _ptr(x_scales_d), _ptr(wg_codes_d),
                                                    _ptr(wg_scales_d), _ptr(wu_codes_d), _ptr(wu_scales_d),
                                                    ACTIVATIONS[activation], _ptr(dx_d), _ptr(dwg_d), _ptr(dwu_d),
-                                                   OUT_TYPES[dw_type], *_work(work_d), m, n, k, stream))
+                                                   OUT_TYPES[dw_type], *_work(work_d, work_bytes), m, n, k, stream))
 
 
 def workspace_bytes(m: int, n: int, k: int) -> int:

@@ -24,3 +24,31 @@ def test_objects_without_an_address_are_refused(wrong):
     for call in calls:
         with pytest.raises(AttributeError, match="data_ptr"):
             call()
+
+
+def test_a_workspace_may_be_an_address_with_its_size():
+    """Each is refused by the library for what it is (2: null, 3: alignment, 7: too small), not by Python on the way."""
+    A, need = 4096, lib.mxfp4_linear_backward_bytes(10, 20, 30)
+
+    def linear(work, **size):
+        lib.mxfp4_linear_backward(A, A, A, A, A, A, A, "f32", A, work, 10, 20, 30, stream=0, **size)
+
+    def gated(work, **size):
+        lib.mxfp4_gated_backward(A, A, A, A, A, A, A, A, A, A, "f32", work, 10, 20, 30, stream=0, **size)
+
+    for call in (linear, gated):
+        for work, size, status in ((A, 0, 7), (A + 16, 1 << 40, 3), (None, 0, 2)):
+            with pytest.raises(lib.Int4LinearError, match=f"status {status}"):
+                call(work, work_bytes=size)
+        with pytest.raises(lib.Int4LinearError, match="status 2"):
+            call(None)
+        with pytest.raises(TypeError, match="work_bytes"):
+            call(A)
+    with pytest.raises(lib.Int4LinearError, match="status 7"):
+        linear(A, work_bytes=need - 1)
+    # a tensor says its size itself; a smaller one given for it is believed
+    work = torch.empty(need + 512, dtype=torch.uint8)
+    work = work[-work.data_ptr() % 256 :]
+    assert api._work(work, None) == (work.data_ptr(), work.numel()) and api._work(work, 256) == (work.data_ptr(), 256)
+    with pytest.raises(lib.Int4LinearError, match="status 7"):
+        linear(work, work_bytes=need - 1)
