@@ -7,6 +7,7 @@
 // group lane / 32 takes chunk (16 bytes) 4 * (lane / 32) + j of its rows in step j = 0 .. 3, for a and b
 // alike, which is all that a sum over k asks for.  With 4-bit operands a chunk is one block of 32, and the
 // scales of the four chunks that a lane sees in a stage are the four bytes of one aligned dword.
+#include "line_tiles.h"
 #include "mxfp4.h"
 #include "mxfp4_epilogue.h"
 
@@ -804,48 +805,19 @@ hipError_t launch_tile(const LineOperands &o, int n, const Ep &ep, const DeviceI
     return hipGetLastError();
 }
 
-// What a tile costs, in units of 10 ns: a stage of each, where every CU is busy with such tiles (`full`) and where there
-// are few (`few`: nothing hides the way to memory), and what a launch spends before its first stage and after its
-// last.  Read off the products below, products that fill the device (8192^3: 283, 342, 461 us, 64 x 64 about 600) and short ones
-// (1024^3: 11.7, 5.9, 5.2, 4.8 us).
-struct TileCost {
-    int m, n, per_cu, full, few, fixed;
-};
-constexpr TileCost kTiles[] = {{256, 256, per_cu<Tile256, true>, 175, 175, 1100},
-                               {128, 128, per_cu<Tile128, true>, 62, 70, 600},
-                               {64, 128, per_cu<Tile64x128, true>, 46, 45, 380},
-                               {64, 64, per_cu<Tile64, true>, 29, 29, 330}};
-
-// The tile that makes a product of m x n (columns of b) in `stages` stages quickest by these costs.  Measured, us by tile:
-//   512 x 4096 x 11008   64, 32.9, 23.6, 29.8        333 x 11008 x 4999   36, 21.2, 27.8, 27.1
-//   2048 x 4096 x 4096   33, 25.6, 34.5, 44.7        128 x 14336 x 4096   26, 14.4, 10.3, 12.3
-//   64 x 4096 x 4096     23, 10.1, 8.6, 7.5          200 x 4096 x 14336   -, 37.7, 24.1, 20.4
-int quickest_tile(long m, long n, int stages, bool pair, const DeviceInfo &dev)
+template <class C>
+constexpr bool described_by(const LineTileCost &t)
 {
-    const long cus = dev.cu_count > 0 ? dev.cu_count : 256;
-    int best = 0;
-    double least = 0;
-    for (int i = 0; i < 3 + !pair; ++i) {
-        const TileCost &t = kTiles[i];
-        const long tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
-        const long places = cus * t.per_cu, rounds = tiles / places, rest = tiles % places;
-        double stage = (double)rounds * t.per_cu * t.full;
-        if (rest)
-            stage += max((double)t.few, (double)rest / cus * t.full);
-        const double cost = stage * stages + t.fixed;
-        if (i == 0 || cost < least) {
-            best = i;
-            least = cost;
-        }
-    }
-    return best;
+    return t.m == C::BM && t.n == C::BN && t.lds[0] == C::template LDS<false> && t.lds[1] == C::template LDS<true>;
 }
+static_assert(described_by<Tile256>(kLineTiles[0]) && described_by<Tile128>(kLineTiles[1]) && described_by<Tile64x128>(kLineTiles[2]) &&
+              described_by<Tile64>(kLineTiles[3]));
 
 // n: columns of the product that have to be covered.
 template <bool FP4, class Ep>
 hipError_t launch(const LineOperands &o, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
-    switch (quickest_tile(o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev)) {
+    switch (quickest_tile(FP4, o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev.cu_count)) {
     case 0:
         return launch_tile<FP4, Tile256>(o, n, ep, dev, stream);
     case 1:
