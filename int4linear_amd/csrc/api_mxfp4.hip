@@ -11,9 +11,11 @@ using namespace int4linear;
 
 // Row and column numbers are 32-bit in the kernels, rounded up to tiles; offsets are 64-bit.
 constexpr int kMostRows = 1 << 30;
-// A tile's loads are a base and 32 bits of offset over at most 256 rows, and the transposes have 65535 rows of
-// tiles of 64: k of a product, and every size of a gradient, which is some product's k.
+// A tile's loads are a base and 32 bits of offset over at most 256 rows of an operand.  The longest rows of a product are k / 2 bytes;
+// those of a gradient's products are bfloat16, 2 bytes of any of its sizes, and 4 of n where dg and du lie side by side.
 constexpr int kMostK = 1 << 22;
+constexpr int kMostGradient = kMostK - 64;
+static_assert(255ull * (kMostK / 2) + 128 <= 1ull << 32 && kMostGradient % 64 == 0 && 255ull * 4 * kMostGradient + 128 <= 1ull << 32);
 
 bool aligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 bool is_type(int type) { return type == INT4LINEAR_OUT_F32 || type == INT4LINEAR_OUT_F16 || type == INT4LINEAR_OUT_BF16; }
@@ -226,7 +228,7 @@ int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, co
                                      size_t work_bytes, int m, int n, int k, void *stream_v)
 {
     Checks ok;
-    ok.sizes(m, n, k).that(m <= kMostK - 64 && n <= kMostK - 64 && k <= kMostK - 64, INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(m, n, k).that(m <= kMostGradient && n <= kMostGradient && k <= kMostGradient, INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(!dw_d || dw_type == INT4LINEAR_OUT_F32 || dw_type == INT4LINEAR_OUT_BF16, INT4LINEAR_ERR_UNSUPPORTED);
     const bool want_dx = dx_d && m > 0 && k > 0, want_dw = dw_d && n > 0 && k > 0, want_sums = dbias_d && n > 0;
     if (!ok || (!want_dx && !want_dw && !want_sums))
@@ -284,7 +286,7 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
                                     int k, void *stream_v)
 {
     Checks ok;
-    ok.sizes(m, n, k).that(m <= kMostK - 64 && n <= kMostK - 64 && k <= kMostK - 64, INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(m, n, k).that(m <= kMostGradient && n <= kMostGradient && k <= kMostGradient, INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(is_activation(activation), INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(!dwg_d || dw_type == INT4LINEAR_OUT_F32 || dw_type == INT4LINEAR_OUT_BF16, INT4LINEAR_ERR_UNSUPPORTED);
     ok.that(!dwg_d == !dwu_d, INT4LINEAR_ERR_NULL);

@@ -52,3 +52,16 @@ def test_a_workspace_may_be_an_address_with_its_size():
     assert api._work(work, None) == (work.data_ptr(), work.numel()) and api._work(work, 256) == (work.data_ptr(), 256)
     with pytest.raises(lib.Int4LinearError, match="status 7"):
         linear(work, work_bytes=need - 1)
+
+
+def test_sizes_beyond_a_tiles_offsets_are_refused():
+    """A product's k to 2^22, every size of a gradient to 2^22 - 64: there the offset of a tile's last row still fits 32 bits."""
+    A, most = 4096, (1 << 22) - 64
+    assert 255 * 4 * most + 128 <= 1 << 32 < 255 * 4 * (most + 64 * 300)
+    with pytest.raises(lib.Int4LinearError, match="status 5"):
+        lib.mxfp4_linear(A, A, A, A, None, A, "f32", 1, 1, (1 << 22) + 1, stream=0)
+    for sizes, status in (((most, 1, 1), 7), ((1, most, 1), 7), ((1, 1, most), 7), ((most + 1, 1, 1), 5), ((1, most + 1, 1), 5), ((1, 1, most + 1), 5)):
+        with pytest.raises(lib.Int4LinearError, match=f"status {status}"):
+            lib.mxfp4_linear_backward(A, A, A, A, A, A, A, "f32", A, A, *sizes, work_bytes=0, stream=0)
+        with pytest.raises(lib.Int4LinearError, match=f"status {status}"):
+            lib.mxfp4_gated_backward(A, A, A, A, A, A, A, A, A, A, "f32", A, *sizes, work_bytes=0, stream=0)
