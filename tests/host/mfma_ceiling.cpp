@@ -1,16 +1,16 @@
 // What the matrix pipes sustain with nothing else going on: loops of nothing but MFMAs on
-// operands held in registers, for the two instructions the library's large-shape kernels issue
-// (v_mfma_i32_32x32x32_i8 and v_mfma_f32_32x32x64_f8f6f4 with FP6 E2M3 operands), on operand
-// data of several kinds, among them every exact encoding of signed 4-bit values that the FP6 / BF6
+// operands held in registers, for the instructions the library's large-shape kernels issue
+// (v_mfma_i32_32x32x32_i8 and v_mfma_f32_32x32x64_f8f6f4 with FP6 E2M3 operands; for MXFP4 layers the latter with E2M1 operands
+// and block scales, and v_mfma_f32_32x32x16_bf16), on operand data of several kinds, among them every exact encoding of signed 4-bit values that the FP6 / BF6
 // formats offer (the one the FP6 kernel uses, n/8 in E2M3, draws the least power of them).  The rate depends on the data: at the device's power limit the clock
 // drops as more operand bits toggle, so "peak" is reached on zeros only.  Each line gives the
 // throughput, the shader clock observed while the loop ran (cycle counter against the constant
 // 100 MHz counter) and the share of the launch's cycles the matrix pipes were busy (32 cycles
-// per MFMA of either kind, two waves per SIMD; launch gaps included).  The figures are what a GEMM kernel's rate can be read
+// per MFMA of any kind, two waves per SIMD; launch gaps included).  The figures are what a GEMM kernel's rate can be read
 // against; the reference has no counterpart (its README quotes no peak, README.md:57-62).
 //
 //   mfma_ceiling [--iters N]
-//   prints lines:  [MFMA] <int8|fp6|bf6> <data> <TOPS> TOPS <GHz> GHz <busy %>
+//   prints lines:  [MFMA] <int8|fp6|bf6|fp4|bf16> <data> <TOPS> TOPS <GHz> GHz <busy %>
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -33,6 +33,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 __device__ unsigned mix(unsigned x)
 {
@@ -43,8 +44,17 @@ __device__ unsigned mix(unsigned x)
 enum Data {
     kZeros = 0, kRandom = 1, kNibbleTimes16 = 2, kSignExtendedS4 = 3,
     // Exact codes of uniform s4 values n: E2M3 n/8 (the FP6 kernel's), n/4, n/2; E3M2 n and n/16.
-    kS4Codes = 4, kS4CodesQuarter = 5, kS4CodesHalf = 6, kBf6CodesOne = 7, kBf6CodesSixteenth = 8
+    kS4Codes = 4, kS4CodesQuarter = 5, kS4CodesHalf = 6, kBf6CodesOne = 7, kBf6CodesSixteenth = 8,
+    kNormal = 9  // normal deviates, as E2M1 in blocks whose largest value is between 4 and 8, or as bfloat16
 };
+
+constexpr int kE2m1 = 4, kBf16 = 16;  // FMT of the loops on MXFP4 layers' operands (kBf16 is none of the field's values)
+
+__device__ float normal(unsigned r)
+{
+    const float u = ((mix(r) >> 8) + 1) * 0x1p-24f, v = (mix(r + 0x9E3779B9u) >> 8) * 0x1p-24f;
+    return sqrtf(-2.0f * logf(u)) * cosf(6.2831853f * v);
+}
 
 // The magnitude bits (exponent and mantissa) of |n| = mg in the given exact encoding.
 __device__ unsigned s4_magnitude_code(int data, unsigned mg)
@@ -88,8 +98,28 @@ __device__ v8i fp6_operand(int data, unsigned seed)
     return (v8i){(int)w[0], (int)w[1], (int)w[2], (int)w[3], (int)w[4], (int)w[5], 0, 0};
 }
 
+// 16 bytes of E2M1 codes or of bfloat16 values.
+__device__ v8i normal_operand(int fmt, int data, unsigned seed)
+{
+    unsigned w[4] = {0, 0, 0, 0};
+    if (data == kNormal)
+        for (int e = 0; e < (fmt == kE2m1 ? 32 : 8); ++e) {
+            const float f = normal(seed * 64 + e);
+            if (fmt == kE2m1) {
+                const float a = fabsf(f) * 2.3f;  // the largest of 32 is 2.1 on average
+                const unsigned code = a < .25f ? 0 : a < .75f ? 1 : a < 1.25f ? 2 : a < 1.75f ? 3 : a < 2.5f ? 4 : a < 3.5f ? 5 : a < 5.0f ? 6 : 7;
+                w[e / 8] |= (code | (f < 0 ? 8u : 0u)) << (4 * (e % 8));
+            } else {
+                w[e / 2] |= (__builtin_bit_cast(unsigned, f) >> 16) << (16 * (e % 2));
+            }
+        }
+    return (v8i){(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+}
+
+__device__ v8bf first8(const v8i &v) { return __builtin_bit_cast(v8bf, (v4i){v[0], v[1], v[2], v[3]}); }
+
 // cycles[0] = shader cycles, cycles[1] = 100 MHz ticks of the loop, as seen by wave 0 of block 0
-// FMT: the instruction's operand format field (2 = E2M3, 3 = E3M2)
+// FMT: the instruction's operand format field (2 = E2M3, 3 = E3M2, kE2m1), or kBf16
 template <bool FP6, int FMT = 2>
 __global__ __launch_bounds__(512) void mfma_loop(int *out, long long *cycles, int iters, int data)
 {
@@ -100,12 +130,20 @@ __global__ __launch_bounds__(512) void mfma_loop(int *out, long long *cycles, in
         v16f acc[8];
         for (int i = 0; i < 8; ++i) for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
         v8i a[4], b[4];
-        for (int i = 0; i < 4; ++i) { a[i] = fp6_operand(data, seed + 1000 * i); b[i] = fp6_operand(data, seed + 77 + 1000 * i); }
+        for (int i = 0; i < 4; ++i) {
+            a[i] = FMT < kE2m1 ? fp6_operand(data, seed + 1000 * i) : normal_operand(FMT, data, seed + 1000 * i);
+            b[i] = FMT < kE2m1 ? fp6_operand(data, seed + 77 + 1000 * i) : normal_operand(FMT, data, seed + 77 + 1000 * i);
+        }
+        const int scale = FMT == kE2m1 ? 0x7F7F7F7F : 0;
         c0 = __builtin_readcyclecounter(); r0 = __builtin_amdgcn_s_memrealtime();
         for (int it = 0; it < iters; ++it) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                acc[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 3], b[(i + (i >> 2)) & 3], acc[i], FMT, FMT, 0, 0, 0, 0);
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (FMT == kBf16)
+                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(first8(a[i & 3]), first8(b[(i + (i >> 2)) & 3]), acc[i], 0, 0, 0);
+                else
+                    acc[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 3], b[(i + (i >> 2)) & 3], acc[i], FMT, FMT, 0, scale, 0, scale);
+            }
         }
         c1 = __builtin_readcyclecounter(); r1 = __builtin_amdgcn_s_memrealtime();
         for (int i = 0; i < 8; ++i) for (int j = 0; j < 16; ++j) sum += (int)acc[i][j];
@@ -148,7 +186,7 @@ void run(const char *kind, const char *name, int data, int iters, int cus, int *
     HIP_OK(hipEventElapsedTime(&ms, e0, e1));
     long long cyc[2];
     HIP_OK(hipMemcpy(cyc, cycles_d, sizeof(cyc), hipMemcpyDeviceToHost));
-    const double mac_per_mfma = FP6 ? 32.0 * 32 * 64 : 32.0 * 32 * 32;
+    const double mac_per_mfma = 32.0 * 32 * (!FP6 ? 32 : FMT == kBf16 ? 16 : 64);
     const double ops = 2.0 * mac_per_mfma * 8 * iters * 8.0 * cus * launches;  // 8 MFMAs x 8 waves per workgroup
     const double ghz = (double)cyc[0] / ((double)cyc[1] * 10e-9) / 1e9;
     // two waves per SIMD, 8 * iters MFMAs each, 32 cycles per MFMA, over a launch's share of the
@@ -188,6 +226,10 @@ int main(int argc, char **argv)
     run<true>("fp6", "s4-codes n/2 (E2M3)", kS4CodesHalf, iters, cus, out, cycles);
     run<true, 3>("bf6", "s4-codes n (E3M2)", kBf6CodesOne, iters, cus, out, cycles);
     run<true, 3>("bf6", "s4-codes n/16 (E3M2)", kBf6CodesSixteenth, iters, cus, out, cycles);
+    run<true, kE2m1>("fp4", "zeros, scaled", kZeros, iters, cus, out, cycles);
+    run<true, kE2m1>("fp4", "normal, scaled", kNormal, iters, cus, out, cycles);
+    run<true, kBf16>("bf16", "zeros", kZeros, iters, cus, out, cycles);
+    run<true, kBf16>("bf16", "normal", kNormal, iters, cus, out, cycles);
     run<false>("int8", "zeros-again", kZeros, iters, cus, out, cycles);
     return 0;
 }

@@ -154,3 +154,12 @@ def test_int8_ablation_reports_every_build(gpu):
     assert len(rows) == 13 and rows[0][0] == "whole kernel", r.stdout
     assert all(float(us) > 0 and float(tops) > 0 for _, us, tops in rows), r.stdout
     assert r.stdout.count("[SPREAD]") == 2, r.stdout
+
+
+@pytest.mark.gpu
+def test_mfma_ceiling_reports_rates_of_the_mxfp4_layers_operands(gpu):
+    r = subprocess.run([str(_binary("mfma_ceiling")), "--iters", "500"], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+    rows = re.findall(r"\[MFMA\] (fp4|bf16) .*? ([\d.]+) TOPS +([\d.]+) GHz", r.stdout)
+    assert [kind for kind, _, _ in rows] == ["fp4", "fp4", "bf16", "bf16"], r.stdout
+    assert all(float(t) > 500 and 0.5 < float(g) < 3.0 for _, t, g in rows), r.stdout
