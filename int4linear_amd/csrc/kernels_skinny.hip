@@ -113,11 +113,7 @@ __device__ __forceinline__ unsigned uniform(unsigned v) { return (unsigned)__bui
 __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p)
 {
     const unsigned long long v = (unsigned long long)p;
-    unsigned long long s = (unsigned long long)uniform((unsigned)v) | ((unsigned long long)uniform((unsigned)(v >> 32)) << 32);
-    // The hardware lets a load read a scalar register up to five instructions after a vector instruction (the
-    // readfirstlane) wrote it without waiting; the compiler keeps them apart for its own loads, not for those above.
-    asm volatile("s_nop 4" : "+s"(s));
-    return (const uint8_t *)s;
+    return (const uint8_t *)((unsigned long long)uniform((unsigned)v) | ((unsigned long long)uniform((unsigned)(v >> 32)) << 32));
 }
 
 // f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
@@ -340,8 +336,13 @@ __device__ __forceinline__ void skinny_body(const uint8_t *X, const uint8_t *W, 
     constexpr std::integral_constant<int, T> kAllTiles{};
     // Issue order: the first tile of W (in the first pass it is on its way already), X, the
     // rest of W.
-    if (pass > 0)
+    if (pass > 0) {
+        // The hardware lets a load read a scalar register up to five instructions after a vector instruction (the base's
+        // readfirstlane) wrote it without waiting; the compiler keeps them apart for its own loads, not for those above.  The other
+        // loads on this base come later than that in every build (tests/test_device_code.py reads them).
+        asm volatile("s_nop 4" : : "s"(wbase));
         issue_w(kZero, kZero, kOne);
+    }
     // With the first loads on their way: the sums start at zero, which everybody has to have
     // seen before anybody adds to them.  (Meeting here, where every wave is about to wait for
     // memory anyway, measured better than meeting in front of the first addition.)
