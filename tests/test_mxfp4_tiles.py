@@ -174,10 +174,11 @@ def test_gated_backward(gpu, m, n, k, few):
 
 
 @pytest.mark.gpu
-def test_results_repeat_whatever_slice_arrives_first(gpu):
-    """The grouped products of a small backward pass meet through counters that are atomic; what they add up, and in which order, is
-    not left to them: the same bits from call to call, with other work on the device and on any stream."""
-    m, n, k = 130, 300, 1100
+@pytest.mark.parametrize("m, n, k", [(70, 900, 520), (2500, 40, 72)])
+def test_results_repeat_whatever_slice_arrives_first(gpu, m, n, k):
+    """The products of a small backward pass whose sums are long (dx over 2 n, the weights' over m) are made in slices that meet through
+    atomic counters; what is added up, and in which order, is not left to them: the same bits from call to call, with other work on
+    the device and on any stream."""
     (xq, _), (gq, _), (uq, _) = gated_operands(m, n, k)
     dh = torch.randn(m, n, generator=torch.Generator("cuda").manual_seed(1), device="cuda").bfloat16()
     first, busy = None, torch.randn(2048, 2048, device="cuda")
