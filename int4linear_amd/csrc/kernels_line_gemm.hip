@@ -838,7 +838,17 @@ LineOperands operands(const MxMatrix &x, const MxMatrix &w0, const MxMatrix &w1,
             x.rows, w0.rows, (k + kLineFp4 - 1) / kLineFp4};
 }
 
-constexpr int kSkinnyRows = 32;  // up to here the weight-streaming kernel
+// Up to here the weight-streaming kernel.  us streaming and on tiles, weights from HBM (from the caches streaming takes up to a fifth
+// less, tiles up to a third):
+//   rows of x            4           16          17          32          48
+//   4096 x 4096          4.7, 7.7    5.3, 8.1    5.8, 8.1    6.6, 8.7    8.8, 9.2
+//   4096 x 14336         7.9, 18.8   10.9, 20.5  12.0, 20.6  14.6, 22.2  23.1, 23.8
+//   8192 x 8192          10.2, 13.4  10.6, 13.5  11.4, 13.6  13.1, 14.7  21.6, 15.4
+//   14336 x 4096         8.7, 8.8    9.7, 9.2    10.6, 9.3   12.6, 9.9   19.0, 10.4
+//   14336 x 4096, gated  14.0, 15.3  15.7, 15.6  16.7, 15.7  18.9, 16.1  29.9, 16.6
+// Weights that give the device few tiles are streamed faster up to 48 rows, those that fill it up to 16: one line for both costs the
+// second up to a quarter at 32 rows.
+constexpr int kSkinnyRows = 32;
 
 // f(type, columns) with the output type of a call and the epilogue's form for rows of n elements.
 template <class F>
@@ -994,8 +1004,9 @@ constexpr int kLeastSlice = 6;
 hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const SliceSpace &space, const DeviceInfo &dev,
                                 hipStream_t stream)
 {
-    // Together up to three rounds of tiles of 64 x 64 (us apart and together: 700 x 2000 x 1000, gated, 1200 tiles 60, 54; 1000 x 2000 x 2000,
-    // linear, 1536 tiles 51, 48; 2048^3, 2048 tiles 66, 70): beyond that each fills the device alone, on larger tiles.  Long k is cut into slices as far as they go.  (Backward pass of a gated layer, 257 x 1400 x 1000, and of a linear one,
+    // Together up to three rounds of tiles of 64 x 64 (us apart and together: 257 x 1400 x 1000, gated, 784 tiles 39, 32.6; 700 x 2000 x 1000, gated,
+    // 1200 tiles 53.2, 52.5; 1600 x 2048 x 1536, linear, 1368 tiles 50.4, 46.1; 1000 x 2000 x 2000, linear, 1536 tiles 42.7, 43.7; 2048^3, 2048 tiles
+    // 60, 66): beyond that each fills the device alone, on larger tiles.  Long k is cut into slices as far as they go.  (Backward pass of a gated layer, 257 x 1400 x 1000, and of a linear one,
     // 130 x 1001 x 515: a launch for each product and operand 39 and 27 us, grouped 33 and 14, with slices 29 and 14: the
     // gated products 21 us, with dx in four slices 17.)
     long tiles = 0;

@@ -223,7 +223,7 @@ hipError_t launch_rows(const SkinnyArgs &g, int n, hipStream_t stream)
 }
 
 // Fragments of w per workgroup: more of them read x less often, fewer make more workgroups.  One as long as two would
-// leave CUs without a workgroup.  (us with 1, 2, 4: 14336 x 4096, 1 row 9.0, 8.3, 8.7; 16 rows 11.4, 9.8, 9.5; 32 rows 17.1,
+// leave CUs without a workgroup.  (us, weights from HBM, with 1, 2, 4: 14336 x 4096, 1 row 9.0, 8.3, 8.7; 16 rows 11.4, 9.8, 9.5; 32 rows 17.1,
 // 12.9, 11.7; 8192 x 8192, 1 row 10.4, 9.9, 12.4; 4096 x 4096, 1 row 4.8, 5.2, 7.3.)  The gated block has two of each, and with
 // few rows the smaller x in return: 14336 x 4096, 1 row 14.0, 14.3; 8 rows 15.1, 14.9; 16 rows 16.8, 15.9; 32 rows 22.4, 19.0.
 bool two_fragments(int n) { return n >= 2 * kRows * 256; }

@@ -19,7 +19,7 @@ constexpr LineTileCost kLineTiles[] = {{256, 256, {131072, 147456}, 175, 175, 11
 constexpr int line_tiles_per_cu(const LineTileCost &t, bool fp4) { return 160 * 1024 / t.lds[fp4]; }
 
 // The tile that makes a product of m x n (columns of b) in `stages` stages quickest by these costs; the last is too narrow for a pair of
-// matrices b.  Measured, us by tile, 4-bit operands:
+// matrices b.  Measured, us by tile, bfloat16 results, operands in the caches; 4-bit operands:
 //   512 x 4096 x 11008   64, 32.9, 23.6, 29.8        333 x 11008 x 4999   36, 21.2, 27.8, 27.1
 //   2048 x 4096 x 4096   33, 25.6, 34.5, 44.7        128 x 14336 x 4096   26, 14.4, 10.3, 12.3
 //   64 x 4096 x 4096     23, 10.1, 8.6, 7.5          200 x 4096 x 14336   -, 37.7, 24.1, 20.4
