@@ -55,8 +55,8 @@ enum {
     INT4LINEAR_ERR_NO_DEVICE = 6,   /* no gfx950 device is visible                       */
     INT4LINEAR_ERR_SCRATCH = 7,     /* int4linear_gemm_s4s4s32_static: the only fast kernel
                                        for the shape needs more scratch memory than
-                                       INT4LINEAR_STATIC_SCRATCH_BYTES; the MXFP4 gradients:
-                                       work_bytes is too small                           */
+                                       INT4LINEAR_STATIC_SCRATCH_BYTES; the gradients
+                                       (MXFP4, 8 bits, norm): work_bytes is too small    */
     INT4LINEAR_ERR_NOT_INITIALISED = 8 /* first call on this device while its stream is being
                                        captured: call int4linear_init() before capturing */
 };
@@ -264,6 +264,75 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
                                     const void *wu_codes_d, const void *wu_scales_d, int activation,
                                     void *dx_d, void *dwg_d, void *dwu_d, int dw_type, void *work_d,
                                     size_t work_bytes, int m, int n, int k, void *stream);
+
+/*
+ * Linear layers in 8 bits: whole numbers with a scale for each row, a token of X or an output channel of W.  (The reference has
+ * no counterpart; its operands are 4-bit and carry no scales.)
+ *
+ * A rows x k matrix is two device arrays:
+ *   codes   8-bit whole numbers, row-major, 16-byte aligned, every row padded with zeros to a multiple of 128 bytes
+ *           (int4linear_int8_code_bytes is the array's size, 0 for a negative one);
+ *   scales  rows floats.  A value is code * scale.
+ * Rows beyond 2^30, a product's k beyond 2^17 - 1 (its sums are exact in 32 bits) and a gradient's sizes beyond 2^22 - 64 are
+ * refused with INT4LINEAR_ERR_UNSUPPORTED.  Like the MXFP4 calls these are asynchronous on `stream`, allocate nothing, take no locks,
+ * do not touch the library's workspace, and may be captured into a graph once the device is set up.
+ */
+size_t int4linear_int8_code_bytes(int rows, int k);
+
+/* x_d (rows x k of `type`, `ld` >= k elements between rows, aligned to its element) -> 8 bits, row by row: the scale is
+ * max(max |x| / 127, 2^-100), a float, and a code the whole number nearest to x / scale, ties to the even one.  A row with an
+ * infinity or a NaN becomes NaN (scale NaN, codes 0).  The padding of codes is written too. */
+int int4linear_int8_quantize(const void *x_d, int type, size_t ld, void *codes_d, float *scales_d, int rows, int k, void *stream);
+/* The way back: y_d (rows x k of `type`, `ld` >= k elements between rows). */
+int int4linear_int8_dequantize(const void *codes_d, const float *scales_d, void *y_d, int type, size_t ld, int rows, int k, void *stream);
+
+/* Y[m x n] = X[m x k] W[n x k]^T + bias: exact sums of the codes' products, (float)sum * x's scale * w's scale + bias in float, rounded
+ * once to out_type; y_d contiguous, 16-byte aligned.  bias_d: n floats or NULL.  k == 0 gives the bias.  Any codes are taken,
+ * -128 among them. */
+int int4linear_int8_linear(const void *x_codes_d, const float *x_scales_d, const void *w_codes_d, const float *w_scales_d,
+                           const float *bias_d, void *y_d, int out_type, int m, int n, int k, void *stream);
+
+/* Its gradients at the values that X and W stand for, as those of int4linear_mxfp4_linear_backward (arguments and workspace
+ * likewise; its bytes depend on dw_type):
+ *   dx (m x k, bfloat16) = dy W,  dw (n x k, dw_type) = dy^T X,  dbias (n floats) = column sums of dy.
+ * A value has more bits than bfloat16, which the products take: dx and a bfloat16 dw are sums of terms with W and X rounded to
+ * bfloat16, which adds as much to their errors as half of their own rounding does; where dw_type is INT4LINEAR_OUT_F32 X is taken as
+ * the sum of two bfloat16 (2^-16 of a term is lost at most), and the product takes twice the time. */
+size_t int4linear_int8_linear_backward_bytes(int m, int n, int k, int dw_type);
+int int4linear_int8_linear_backward(const void *dy_d, const void *x_codes_d, const float *x_scales_d, const void *w_codes_d,
+                                    const float *w_scales_d, void *dx_d, void *dw_d, int dw_type, float *dbias_d, void *work_d,
+                                    size_t work_bytes, int m, int n, int k, void *stream);
+
+/*
+ * The norm in front of such layers: y = (x - mean) / sqrt(variance + eps) * gamma + beta, mean and variance (of all n, not n - 1)
+ * over a row.  (The reference has no counterpart.)  x_d is rows x n of `type`, `ld` >= n elements between rows, aligned to its element;
+ * gamma_d and beta_d are n floats each or NULL (1 and 0); eps >= 0 and finite, else INT4LINEAR_ERR_UNSUPPORTED, as are more than 2^30
+ * rows and n beyond 2^22.  Sums and statistics are held in float: a row whose squares (of x - mean) add up to more
+ * than a float holds gives beta.  A row with an infinity or a NaN becomes NaN.
+ *   int4linear_layer_norm        y_d is rows x n of out_type, ld_y >= n elements between rows, aligned to its element; it may be x_d
+ *                                where types and distances of rows are the same;
+ *   int4linear_layer_norm_int8   y in 8 bits, quantised from its float value: the operand of int4linear_int8_linear;
+ *   int4linear_layer_norm_mxfp4  y in MXFP4, likewise: the operand of the MXFP4 layers.
+ * Calls are asynchronous, allocate nothing, and may be captured, like those above.
+ */
+int int4linear_layer_norm(const void *x_d, int type, size_t ld, const float *gamma_d, const float *beta_d, float eps, void *y_d,
+                          int out_type, size_t ld_y, int rows, int n, void *stream);
+int int4linear_layer_norm_int8(const void *x_d, int type, size_t ld, const float *gamma_d, const float *beta_d, float eps, void *codes_d,
+                               float *scales_d, int rows, int n, void *stream);
+int int4linear_layer_norm_mxfp4(const void *x_d, int type, size_t ld, const float *gamma_d, const float *beta_d, float eps, void *codes_d,
+                                void *scales_d, int rows, int n, void *stream);
+
+/* Gradients of int4linear_layer_norm from dy_d (rows x n of dy_type, ld_dy elements between rows); mean and variance are computed
+ * again from x, so the forward pass has nothing to keep.  With h = (x - mean) / sqrt(variance + eps) and g = dy gamma:
+ *   dx (of x's type, ld_dx elements between rows) = (g - mean(g) - h mean(g h)) / sqrt(variance + eps),
+ *   dgamma (n floats) = sum over rows of dy h,  dbeta (n floats) = sum over rows of dy.
+ * dx_d, dgamma_d and dbeta_d may each be NULL (not wanted).  work_d: a 256-byte aligned device buffer of at least
+ * int4linear_layer_norm_backward_bytes(rows, n) bytes, else INT4LINEAR_ERR_SCRATCH; what it holds before does not matter, and two calls
+ * that may overlap need one each.  Results are the same bits from call to call, whichever of them are wanted. */
+size_t int4linear_layer_norm_backward_bytes(int rows, int n);
+int int4linear_layer_norm_backward(const void *dy_d, int dy_type, size_t ld_dy, const void *x_d, int type, size_t ld, const float *gamma_d,
+                                   float eps, void *dx_d, size_t ld_dx, float *dgamma_d, float *dbeta_d, void *work_d, size_t work_bytes,
+                                   int rows, int n, void *stream);
 
 /* Bytes of internal workspace INT4LINEAR_KERNEL_AUTO would use for a shape on the current
  * device (0 when the chosen kernel needs none).  Sets the device up if that has not

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_size_t, c_void_p
 from pathlib import Path
 
 # INT4LINEAR_LIBRARY overrides the in-tree location (e.g. to try a differently built copy).
@@ -48,6 +48,23 @@ C_ABI = [
     ("int4linear_mxfp4_gated_backward_bytes", c_size_t, [c_int, c_int, c_int]),
     ("int4linear_mxfp4_gated_backward", c_int,
      [c_void_p] * 7 + [c_int] + [c_void_p] * 3 + [c_int, c_void_p, c_size_t] + [c_int] * 3 + [c_void_p]),
+    ("int4linear_int8_code_bytes", c_size_t, [c_int, c_int]),
+    ("int4linear_int8_quantize", c_int, [c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    ("int4linear_int8_dequantize", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_int, c_int, c_void_p]),
+    ("int4linear_int8_linear", c_int, [c_void_p] * 6 + [c_int] * 4 + [c_void_p]),
+    ("int4linear_int8_linear_backward_bytes", c_size_t, [c_int] * 4),
+    ("int4linear_int8_linear_backward", c_int,
+     [c_void_p] * 7 + [c_int, c_void_p, c_void_p, c_size_t] + [c_int] * 3 + [c_void_p]),
+    ("int4linear_layer_norm", c_int,
+     [c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_float, c_void_p, c_int, c_size_t, c_int, c_int, c_void_p]),
+    ("int4linear_layer_norm_int8", c_int,
+     [c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    ("int4linear_layer_norm_mxfp4", c_int,
+     [c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    ("int4linear_layer_norm_backward_bytes", c_size_t, [c_int, c_int]),
+    ("int4linear_layer_norm_backward", c_int,
+     [c_void_p, c_int, c_size_t, c_void_p, c_int, c_size_t, c_void_p, c_float, c_void_p, c_size_t] + [c_void_p] * 3 +
+     [c_size_t, c_int, c_int, c_void_p]),
     ("int4linear_workspace_bytes", c_size_t, [c_int, c_int, c_int]),
     ("int4linear_set_workspace_limit", None, [c_size_t]),
     ("int4linear_release_workspace", c_int, []),

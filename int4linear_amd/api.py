@@ -266,6 +266,111 @@ def mxfp4_gated_backward(dh_d, x_codes_d, x_scales_d, wg_codes_d, wg_scales_d, w
                                                    OUT_TYPES[dw_type], *_work(work_d, work_bytes), m, n, k, stream))
 
 
+def int8_code_bytes(rows: int, k: int) -> int:
+    """Bytes of a rows x k matrix's codes in 8 bits (a row: a multiple of 128); its scales are rows float32."""
+    return int(_lib.load().int4linear_int8_code_bytes(rows, k))
+
+
+def int8_quantize(x_d, codes_d, scales_d, rows: int, k: int, *, in_type: str = "bf16", ld: int | None = None,
+                  stream: int | None = None) -> None:
+    """x_d (rows x k of in_type "f32", "f16" or "bf16", ld elements between rows, k if None) -> 8 bits with a scale a row."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_int8_quantize(_ptr(x_d), OUT_TYPES[in_type], k if ld is None else ld, _ptr(codes_d),
+                                            _ptr(scales_d), rows, k, stream))
+
+
+def int8_dequantize(codes_d, scales_d, y_d, rows: int, k: int, *, out_type: str = "bf16", ld: int | None = None,
+                    stream: int | None = None) -> None:
+    """8 bits -> y_d (rows x k of out_type, ld elements between rows, k if None)."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_int8_dequantize(_ptr(codes_d), _ptr(scales_d), _ptr(y_d), OUT_TYPES[out_type],
+                                              k if ld is None else ld, rows, k, stream))
+
+
+def int8_linear(x_codes_d, x_scales_d, w_codes_d, w_scales_d, bias_d, y_d, out_type: str, m: int, n: int, k: int, *,
+                stream: int | None = None) -> None:
+    """Y (m x n of out_type) = X * W^T + bias for 8-bit operands; bias_d (n float32) may be None."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_int8_linear(_ptr(x_codes_d), _ptr(x_scales_d), _ptr(w_codes_d), _ptr(w_scales_d),
+                                          _ptr(bias_d), _ptr(y_d), OUT_TYPES[out_type], m, n, k, stream))
+
+
+def int8_linear_backward_bytes(m: int, n: int, k: int, dw_type: str) -> int:
+    """Bytes of workspace int8_linear_backward needs."""
+    return int(_lib.load().int4linear_int8_linear_backward_bytes(m, n, k, OUT_TYPES[dw_type]))
+
+
+def int8_linear_backward(dy_d, x_codes_d, x_scales_d, w_codes_d, w_scales_d, dx_d, dw_d, dw_type: str, dbias_d, work_d,
+                         m: int, n: int, k: int, *, work_bytes: int | None = None, stream: int | None = None) -> None:
+    """dx (bfloat16) = dy W, dw (dw_type "bf16" or "f32") = dy^T X, dbias (float32) = column sums of dy
+    (bfloat16); dx_d, dw_d and dbias_d may each be None.  work_d: a tensor of at least
+    int8_linear_backward_bytes(m, n, k, dw_type) bytes, or a device address with its work_bytes."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_int8_linear_backward(_ptr(dy_d), _ptr(x_codes_d), _ptr(x_scales_d), _ptr(w_codes_d),
+                                                   _ptr(w_scales_d), _ptr(dx_d), _ptr(dw_d), OUT_TYPES[dw_type],
+                                                   _ptr(dbias_d), *_work(work_d, work_bytes), m, n, k, stream))
+
+
+def layer_norm(x_d, gamma_d, beta_d, y_d, rows: int, n: int, *, eps: float = 1e-5, in_type: str = "bf16",
+               out_type: str = "bf16", ld: int | None = None, ld_y: int | None = None, stream: int | None = None) -> None:
+    """y_d (rows x n of out_type) = (x - mean) / sqrt(variance + eps) * gamma + beta, row by row of x_d (rows x n of
+    in_type); gamma_d and beta_d (n float32) may each be None.  ld, ld_y: elements between rows, n if None."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_layer_norm(_ptr(x_d), OUT_TYPES[in_type], n if ld is None else ld, _ptr(gamma_d),
+                                         _ptr(beta_d), eps, _ptr(y_d), OUT_TYPES[out_type], n if ld_y is None else ld_y,
+                                         rows, n, stream))
+
+
+def layer_norm_int8(x_d, gamma_d, beta_d, codes_d, scales_d, rows: int, n: int, *, eps: float = 1e-5,
+                    in_type: str = "bf16", ld: int | None = None, stream: int | None = None) -> None:
+    """layer_norm with the result in 8 bits, the form int8_linear takes."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_layer_norm_int8(_ptr(x_d), OUT_TYPES[in_type], n if ld is None else ld, _ptr(gamma_d),
+                                              _ptr(beta_d), eps, _ptr(codes_d), _ptr(scales_d), rows, n, stream))
+
+
+def layer_norm_mxfp4(x_d, gamma_d, beta_d, codes_d, scales_d, rows: int, n: int, *, eps: float = 1e-5,
+                     in_type: str = "bf16", ld: int | None = None, stream: int | None = None) -> None:
+    """layer_norm with the result in MXFP4, the form the mxfp4 layers take."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_layer_norm_mxfp4(_ptr(x_d), OUT_TYPES[in_type], n if ld is None else ld, _ptr(gamma_d),
+                                               _ptr(beta_d), eps, _ptr(codes_d), _ptr(scales_d), rows, n, stream))
+
+
+def layer_norm_backward_bytes(rows: int, n: int) -> int:
+    """Bytes of workspace layer_norm_backward needs."""
+    return int(_lib.load().int4linear_layer_norm_backward_bytes(rows, n))
+
+
+def layer_norm_backward(dy_d, x_d, gamma_d, dx_d, dgamma_d, dbeta_d, work_d, rows: int, n: int, *, eps: float = 1e-5,
+                        dy_type: str = "bf16", in_type: str = "bf16", ld_dy: int | None = None, ld: int | None = None,
+                        ld_dx: int | None = None, work_bytes: int | None = None, stream: int | None = None) -> None:
+    """Gradients of layer_norm from dy_d (rows x n of dy_type): dx_d (of x_d's in_type), dgamma_d and dbeta_d (n
+    float32); each of the three may be None.  work_d: a tensor of at least layer_norm_backward_bytes(rows, n) bytes, or a
+    device address with its work_bytes."""
+    lib = _lib.load()
+    if stream is None:
+        stream = _current_stream()
+    _lib.check(lib.int4linear_layer_norm_backward(_ptr(dy_d), OUT_TYPES[dy_type], n if ld_dy is None else ld_dy, _ptr(x_d),
+                                                  OUT_TYPES[in_type], n if ld is None else ld, _ptr(gamma_d), eps,
+                                                  _ptr(dx_d), n if ld_dx is None else ld_dx, _ptr(dgamma_d), _ptr(dbeta_d),
+                                                  *_work(work_d, work_bytes), rows, n, stream))
+
+
 def workspace_bytes(m: int, n: int, k: int) -> int:
     """Internal workspace the automatic dispatch would use for this shape."""
     return int(_lib.load().int4linear_workspace_bytes(m, n, k))

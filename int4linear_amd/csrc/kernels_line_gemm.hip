@@ -1,12 +1,14 @@
 // GEMM over lines of 128 bytes: MXFP4 operands (256 k per line, block scales applied by the matrix
-// instruction) and bfloat16 operands (64 k per line), y = a b^T.
+// instruction), 8-bit whole numbers (128 k per line, rows' scales applied to the sums) and bfloat16 operands (64 k per
+// line), y = a b^T.
 //
-// Both element types share one kernel, because their matrix instructions take the same bytes from
-// a lane: v_mfma_scale_f32_32x32x64_f8f6f4 on 4-bit operands and v_mfma_f32_32x32x16_bf16 both
-// read 16 bytes of row lane % 32, and both run 32 cycles.  A stage is one line of every row of the tile; lane
+// The element types share one kernel, because their matrix instructions take the same bytes from
+// a lane: v_mfma_scale_f32_32x32x64_f8f6f4 on 4-bit operands, v_mfma_i32_32x32x32_i8 and v_mfma_f32_32x32x16_bf16 all
+// read 16 bytes of row lane % 32, and all run 32 cycles.  A stage is one line of every row of the tile; lane
 // group lane / 32 takes chunk (16 bytes) 4 * (lane / 32) + j of its rows in step j = 0 .. 3, for a and b
 // alike, which is all that a sum over k asks for.  With 4-bit operands a chunk is one block of 32, and the
 // scales of the four chunks that a lane sees in a stage are the four bytes of one aligned dword.
+#include "int8.h"
 #include "line_tiles.h"
 #include "mxfp4.h"
 #include "mxfp4_epilogue.h"
@@ -23,6 +25,7 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
@@ -30,6 +33,11 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 constexpr int kFrag = 32;
+
+// What the operands hold.
+enum Values : int { kBf16Values, kFp4Values, kInt8Values };
+template <int VALUES>
+using Sums = std::conditional_t<VALUES == kInt8Values, v16i, v16f>;
 
 // The operands.  A row is `stages` lines, `stride` bytes from the next, and with 4-bit values its scales, scale_stride
 // bytes from the next, for a and b alike.  The gated block's two matrices b have as many rows each.
@@ -135,6 +143,84 @@ struct PlainEpilogue {
                 for (int t = 0; t < 16; ++t)
                     v[t] = acc[j][i][t] + add[t];
                 store_block<OUT, COLUMNS>(y, ld, m, n, row + kFrag * j, c, lane, v);
+            }
+        }
+    }
+};
+
+// y = sums * x's scale of the row * w's scale of the column + bias, rounded once to OUT.  The sums are whole numbers below 2^31; as floats
+// they are off by 2^-24 of themselves at most.
+template <int OUT, bool COLUMNS>
+struct Int8Epilogue {
+    static constexpr bool kPair = false, kColumns = COLUMNS;
+    void *y;
+    const float *bias, *x_scales, *w_scales;
+    size_t ld;
+    int m, n;
+
+    // Elements 8 (t / 4) + t % 4 of v from `first` on, of which there are `count` (those behind: the last again).
+    static __device__ __forceinline__ void sixteen(const float *v, int first, int count, float (&out)[16])
+    {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = first + 8 * q;
+            if (at + 4 <= count) {
+                __builtin_memcpy(&out[4 * q], v + at, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    out[4 * q + e] = v[min(at + e, count - 1)];
+            }
+        }
+    }
+
+    template <int FM, int FN>
+    __device__ __forceinline__ void operator()(v16i (&acc)[FM][FN], int row, int col, int lane) const
+    {
+        const int one = lane & 31, four = 4 * (lane >> 5);
+        if constexpr (COLUMNS) {
+            float ws[FN], add[FN];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                const int c = min(col + kFrag * i + one, n - 1);
+                ws[i] = w_scales[c];
+                add[i] = bias ? bias[c] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                float xs[16];
+                sixteen(x_scales, row + kFrag * j + four, m, xs);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    float v[16];
+#pragma unroll
+                    for (int t = 0; t < 16; ++t)
+                        v[t] = (float)acc[j][i][t] * xs[t] * ws[i] + add[i];
+                    store_block<OUT, COLUMNS>(y, ld, m, n, row + kFrag * j, col + kFrag * i, lane, v);
+                }
+            }
+        } else {
+            float xs[FM];
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+                xs[j] = x_scales[min(row + kFrag * j + one, m - 1)];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                float ws[16], add[16];
+                sixteen(w_scales, col + kFrag * i + four, n, ws);
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+                    add[t] = 0.0f;
+                if (bias)
+                    sixteen(bias, col + kFrag * i + four, n, add);
+#pragma unroll
+                for (int j = 0; j < FM; ++j) {
+                    float v[16];
+#pragma unroll
+                    for (int t = 0; t < 16; ++t)
+                        v[t] = (float)acc[j][i][t] * xs[j] * ws[t] + add[t];
+                    store_block<OUT, COLUMNS>(y, ld, m, n, row + kFrag * j, col + kFrag * i, lane, v);
+                }
             }
         }
     }
@@ -358,6 +444,7 @@ __device__ __forceinline__ void tile_coords(int v, int total, int tiles_m, int t
 
 // Marks a value as used at this point of the program without generating code.
 __device__ __forceinline__ void pin(const v16f &v) { asm volatile("" ::"v"(v)); }
+__device__ __forceinline__ void pin(const v16i &v) { asm volatile("" ::"v"(v)); }
 
 // Sums without a single term: y = bias.
 template <int OUT>
@@ -384,9 +471,10 @@ hipError_t fill_rows(void *y, const float *bias, size_t m, size_t n, hipStream_t
 // instructions; while a step's instructions run, those of the step AHEAD further on are read from LDS into another register
 // set.  Before a stage's AHEAD last steps every read of the stage has been made: there the waves meet, the next stage must
 // have landed (younger ones stay in flight), and the stage's buffer is given to the loads of the stage STAGES further on.
-template <bool FP4, class C, class Ep>
+template <int VALUES, class C, class Ep>
 __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, int tiles_n, const Ep &ep, int first, int by)
 {
+    constexpr bool FP4 = VALUES == kFp4Values;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -397,13 +485,13 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
     const int stages = o.stages;
     constexpr int kTileN = Ep::kPair ? C::BN / 2 : C::BN;  // columns of y
 
-    v16f acc[C::FM][C::FN];
+    Sums<VALUES> acc[C::FM][C::FN];
     auto clear = [&] {
 #pragma unroll
         for (int j = 0; j < C::FM; ++j)
 #pragma unroll
             for (int i = 0; i < C::FN; ++i)
-                acc[j][i] = (v16f)0.0f;
+                acc[j][i] = (Sums<VALUES>)0;
     };
     auto finish = [&](int it) {
         int tm, tn;
@@ -587,6 +675,11 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
                         acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_a, wide_b, acc[j][i], 4, 4, J, sa[0][j], J, sb[0][i]);
                     else
                         acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_b, wide_a, acc[j][i], 4, 4, J, sb[0][i], J, sa[0][j]);
+                } else if constexpr (VALUES == kInt8Values) {
+                    if constexpr (Ep::kColumns)
+                        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[p][j], fb[p][i], acc[j][i], 0, 0, 0);
+                    else
+                        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[p][i], fa[p][j], acc[j][i], 0, 0, 0);
                 } else {
                     const v8bf wide_a = __builtin_bit_cast(v8bf, fa[p][j]), wide_b = __builtin_bit_cast(v8bf, fb[p][i]);
                     if constexpr (Ep::kColumns)
@@ -664,10 +757,10 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <bool FP4, class C, class Ep>
+template <int VALUES, class C, class Ep>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void line_gemm_kernel(LineOperands o, int tiles_m, int tiles_n, Ep ep)
 {
-    line_gemm<FP4, C>(o, tiles_m, tiles_n, ep, blockIdx.x, gridDim.x);
+    line_gemm<VALUES, C>(o, tiles_m, tiles_n, ep, blockIdx.x, gridDim.x);
 }
 
 // Up to three products in one launch, by blockIdx.z: those of a small layer's backward pass, each of which would leave
@@ -778,7 +871,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_group_kernel(LineGrou
         ep.m = o.a_rows;
         const SliceEpilogue<decltype(ep)> shared{ep, g.partial + (size_t)(g.first[z] + tile * slices) * 64 * 64,
                                                  g.arrivals + (g.first[z] + tile * slices) * C::NWAVES, slice, slices};
-        line_gemm<false, C>(o, g.tiles_m[z], g.tiles_n[z], shared, tile, tiles);
+        line_gemm<kBf16Values, C>(o, g.tiles_m[z], g.tiles_n[z], shared, tile, tiles);
     };
     if (z == g.count - 1)
         run(ep_x);
@@ -795,13 +888,13 @@ using Tile64 = LineTile<2, 2, 1, 1, 4, 4, 2, 4>;  // (too narrow for pairs of bl
 template <class C, bool FP4>
 constexpr int per_cu = 160 * 1024 / C::template LDS<FP4>;
 
-template <bool FP4, class C, class Ep>
+template <int VALUES, class C, class Ep>
 hipError_t launch_tile(const LineOperands &o, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
     const int bn = Ep::kPair ? C::BN / 2 : C::BN;
     const int tiles_m = (o.a_rows + C::BM - 1) / C::BM, tiles_n = (n + bn - 1) / bn;
-    const int groups = min(tiles_m * tiles_n, max(1, dev.cu_count * per_cu<C, FP4>));
-    line_gemm_kernel<FP4, C, Ep><<<groups, C::THREADS, C::template LDS<FP4>, stream>>>(o, tiles_m, tiles_n, ep);
+    const int groups = min(tiles_m * tiles_n, max(1, dev.cu_count * per_cu<C, VALUES == kFp4Values>));
+    line_gemm_kernel<VALUES, C, Ep><<<groups, C::THREADS, C::template LDS<VALUES == kFp4Values>, stream>>>(o, tiles_m, tiles_n, ep);
     return hipGetLastError();
 }
 
@@ -814,21 +907,21 @@ static_assert(described_by<Tile256>(kLineTiles[0]) && described_by<Tile128>(kLin
               described_by<Tile64>(kLineTiles[3]));
 
 // n: columns of the product that have to be covered.
-template <bool FP4, class Ep>
+template <int VALUES, class Ep>
 hipError_t launch(const LineOperands &o, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
-    switch (quickest_tile(FP4, o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev.cu_count)) {
+    switch (quickest_tile(VALUES == kFp4Values, o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev.cu_count)) {
     case 0:
-        return launch_tile<FP4, Tile256>(o, n, ep, dev, stream);
+        return launch_tile<VALUES, Tile256>(o, n, ep, dev, stream);
     case 1:
-        return launch_tile<FP4, Tile128>(o, n, ep, dev, stream);
+        return launch_tile<VALUES, Tile128>(o, n, ep, dev, stream);
     case 2:
-        return launch_tile<FP4, Tile64x128>(o, n, ep, dev, stream);
+        return launch_tile<VALUES, Tile64x128>(o, n, ep, dev, stream);
     default:
         if constexpr (Ep::kPair)
             return hipErrorInvalidValue;
         else
-            return launch_tile<FP4, Tile64>(o, n, ep, dev, stream);
+            return launch_tile<VALUES, Tile64>(o, n, ep, dev, stream);
     }
 }
 
@@ -864,14 +957,14 @@ hipError_t by_type(int out, int n, F &&f)
 }  // namespace
 
 // Lets the kernels of an epilogue have their LDS.
-template <bool FP4, class Ep>
+template <int VALUES, class Ep>
 static hipError_t allow_lds()
 {
     hipError_t e = hipSuccess;
     auto allow = [&](auto tile) {
         using C = decltype(tile);
         if (e == hipSuccess)
-            e = hipFuncSetAttribute((const void *)line_gemm_kernel<FP4, C, Ep>, hipFuncAttributeMaxDynamicSharedMemorySize, C::template LDS<FP4>);
+            e = hipFuncSetAttribute((const void *)line_gemm_kernel<VALUES, C, Ep>, hipFuncAttributeMaxDynamicSharedMemorySize, C::template LDS<VALUES == kFp4Values>);
     };
     allow(Tile256{});
     allow(Tile128{});
@@ -898,14 +991,17 @@ hipError_t line_gemm_init(const DeviceInfo &)
                        allow_group_lds<Rows16, Rows16>})
         if (e == hipSuccess)
             e = allow();
-    for (auto allow : {allow_lds<true, PlainEpilogue<kOutF32, true>>, allow_lds<true, PlainEpilogue<kOutF16, true>>,
-                       allow_lds<true, PlainEpilogue<kOutF16, false>>, allow_lds<true, PlainEpilogue<kOutBF16, true>>,
-                       allow_lds<true, PlainEpilogue<kOutBF16, false>>, allow_lds<true, GatedEpilogue<kOutF32, true>>,
-                       allow_lds<true, GatedEpilogue<kOutF16, true>>, allow_lds<true, GatedEpilogue<kOutF16, false>>,
-                       allow_lds<true, GatedEpilogue<kOutBF16, true>>, allow_lds<true, GatedEpilogue<kOutBF16, false>>,
-                       allow_lds<true, GatedMxEpilogue>, allow_lds<true, GradientEpilogue>,
-                       allow_lds<false, PlainEpilogue<kOutF32, true>>, allow_lds<false, PlainEpilogue<kOutBF16, true>>,
-                       allow_lds<false, PlainEpilogue<kOutBF16, false>>})
+    for (auto allow : {allow_lds<kFp4Values, PlainEpilogue<kOutF32, true>>, allow_lds<kFp4Values, PlainEpilogue<kOutF16, true>>,
+                       allow_lds<kFp4Values, PlainEpilogue<kOutF16, false>>, allow_lds<kFp4Values, PlainEpilogue<kOutBF16, true>>,
+                       allow_lds<kFp4Values, PlainEpilogue<kOutBF16, false>>, allow_lds<kFp4Values, GatedEpilogue<kOutF32, true>>,
+                       allow_lds<kFp4Values, GatedEpilogue<kOutF16, true>>, allow_lds<kFp4Values, GatedEpilogue<kOutF16, false>>,
+                       allow_lds<kFp4Values, GatedEpilogue<kOutBF16, true>>, allow_lds<kFp4Values, GatedEpilogue<kOutBF16, false>>,
+                       allow_lds<kFp4Values, GatedMxEpilogue>, allow_lds<kFp4Values, GradientEpilogue>,
+                       allow_lds<kInt8Values, Int8Epilogue<kOutF32, true>>, allow_lds<kInt8Values, Int8Epilogue<kOutF16, true>>,
+                       allow_lds<kInt8Values, Int8Epilogue<kOutF16, false>>, allow_lds<kInt8Values, Int8Epilogue<kOutBF16, true>>,
+                       allow_lds<kInt8Values, Int8Epilogue<kOutBF16, false>>,
+                       allow_lds<kBf16Values, PlainEpilogue<kOutF32, true>>, allow_lds<kBf16Values, PlainEpilogue<kOutBF16, true>>,
+                       allow_lds<kBf16Values, PlainEpilogue<kOutBF16, false>>})
         if (e == hipSuccess)
             e = allow();
     return e;
@@ -921,7 +1017,21 @@ hipError_t launch_mx_linear(const MxMatrix &x, const MxMatrix &w, const float *b
         if (k == 0)
             return fill_rows<OUT>(y, bias, (size_t)x.rows, (size_t)w.rows, stream);
         const PlainEpilogue<OUT, decltype(columns)::value> ep{y, bias, (size_t)w.rows, x.rows, w.rows};
-        return launch<true>(operands(x, w, w, k), w.rows, ep, dev, stream);
+        return launch<kFp4Values>(operands(x, w, w, k), w.rows, ep, dev, stream);
+    });
+}
+
+hipError_t launch_int8_linear(const Int8Matrix &x, const Int8Matrix &w, const float *bias, void *y, int out, int k, const DeviceInfo &dev,
+                              hipStream_t stream)
+{
+    return by_type(out, w.rows, [&](auto type, auto columns) {
+        constexpr int OUT = decltype(type)::value;
+        if (k == 0)
+            return fill_rows<OUT>(y, bias, (size_t)x.rows, (size_t)w.rows, stream);
+        const LineOperands o{(const uint8_t *)x.codes, (const uint8_t *)w.codes, (const uint8_t *)w.codes, nullptr, nullptr, nullptr,
+                             (unsigned)int8_code_stride(k), 0, x.rows, w.rows, (k + kLineInt8 - 1) / kLineInt8};
+        const Int8Epilogue<OUT, decltype(columns)::value> ep{y, bias, x.scales, w.scales, (size_t)w.rows, x.rows, w.rows};
+        return launch<kInt8Values>(o, w.rows, ep, dev, stream);
     });
 }
 
@@ -935,7 +1045,7 @@ hipError_t launch_mx_gated(const MxMatrix &x, const MxMatrix &wg, const MxMatrix
         if (k == 0)
             return fill_rows<OUT>(h, nullptr, (size_t)x.rows, (size_t)wg.rows, stream);
         const GatedEpilogue<OUT, decltype(columns)::value> ep{h, (size_t)wg.rows, x.rows, wg.rows, act};
-        return launch<true>(operands(x, wg, wu, k), wg.rows, ep, dev, stream);
+        return launch<kFp4Values>(operands(x, wg, wu, k), wg.rows, ep, dev, stream);
     });
 }
 
@@ -951,7 +1061,7 @@ hipError_t launch_mx_gated_quantized(const MxMatrix &x, const MxMatrix &wg, cons
         return launch_mx_gated_quantized_skinny(x, wg, wu, act, codes, scales, k, stream);
     const GatedMxEpilogue ep{codes, scales, mx_code_stride(n), mx_scale_stride(n), x.rows, n, act};
     // (the grid covers the padding at the end of h's rows)
-    return launch<true>(operands(x, wg, wu, k), (int)(mx_code_stride(n) * 2), ep, dev, stream);
+    return launch<kFp4Values>(operands(x, wg, wu, k), (int)(mx_code_stride(n) * 2), ep, dev, stream);
 }
 
 hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, const MxMatrix &wu, Activation act, const uint16_t *dh,
@@ -959,7 +1069,7 @@ hipError_t launch_mx_gated_gradients(const MxMatrix &x, const MxMatrix &wg, cons
                                      hipStream_t stream)
 {
     const GradientEpilogue ep{(const __bf16 *)dh, (__bf16 *)d, (__bf16 *)dt, ld_n, ld_m, x.rows, wg.rows, act, wg.rows % 4 == 0};
-    return launch<true>(operands(x, wg, wu, k), wg.rows, ep, dev, stream);
+    return launch<kFp4Values>(operands(x, wg, wu, k), wg.rows, ep, dev, stream);
 }
 
 static LineOperands operands(const Bf16Product &p)
@@ -981,9 +1091,9 @@ static hipError_t launch_bf16(const Bf16Product &p, const DeviceInfo &dev, hipSt
         return p.out == kOutF32 ? fill_rows<kOutF32>(p.y, nullptr, (size_t)p.m, (size_t)p.n, stream)
                                 : fill_rows<kOutBF16>(p.y, nullptr, (size_t)p.m, (size_t)p.n, stream);
     if (p.out == kOutF32)
-        return launch<false>(operands(p), p.n, epilogue<kOutF32, true>(p), dev, stream);
-    return p.n % 8 ? launch<false>(operands(p), p.n, epilogue<kOutBF16, true>(p), dev, stream)
-                   : launch<false>(operands(p), p.n, epilogue<kOutBF16, false>(p), dev, stream);
+        return launch<kBf16Values>(operands(p), p.n, epilogue<kOutF32, true>(p), dev, stream);
+    return p.n % 8 ? launch<kBf16Values>(operands(p), p.n, epilogue<kOutBF16, true>(p), dev, stream)
+                   : launch<kBf16Values>(operands(p), p.n, epilogue<kOutBF16, false>(p), dev, stream);
 }
 
 template <class EpW, class EpX>

@@ -9,6 +9,7 @@
 // 1, so the result follows from the formula bit by bit.  floor(log2) is the exponent field: a
 // denormal maximum has the field 0 and meets the lower bound.  A block that holds an infinity or a NaN gets
 // the scale code 255 and stands for 32 NaNs.
+#include "int8.h"
 #include "mxfp4.h"
 #include "mxfp4_epilogue.h"
 
@@ -18,7 +19,9 @@ namespace int4linear {
 
 namespace {
 
+typedef int v2i __attribute__((ext_vector_type(2)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
 constexpr int kSegment = 512;  // k that one wave converts at a time: 8 per lane
@@ -204,21 +207,63 @@ __device__ __forceinline__ void store_transposed(const v4u (&rows)[8], uint16_t 
 }
 
 template <int DOWN>
+__device__ __forceinline__ void transpose_int8(const Transposed &t, int k)
+{
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = (blockIdx.x * DOWN + wave / kTilesAcross) * kTile, c0 = (blockIdx.y * kTilesAcross + wave % kTilesAcross) * kTile;
+    if (r0 >= t.of.q.rows || c0 >= k)
+        return;
+    const int row = r0 + (lane & 7) * 8, col = c0 + (lane >> 3) * 8;
+    const size_t stride = int8_code_stride(k);
+    v2i codes[8];
+    float scales[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        codes[r] = (v2i)0;
+        scales[r] = 0.0f;
+        if (row + r < t.of.q.rows) {
+            codes[r] = *(const v2i *)(t.of.q.codes + (size_t)(row + r) * stride + col);
+            scales[r] = t.of.row_scales[row + r];
+        }
+    }
+    v4u rows[8], rest[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            v2bf two, left;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = 2 * p + e;
+                const float v = (float)(int8_t)(codes[r][c / 4] >> 8 * (c % 4)) * scales[r];
+                two[e] = (__bf16)v;
+                left[e] = (__bf16)(v - (float)two[e]);
+            }
+            rows[r][p] = __builtin_bit_cast(unsigned, two);
+            rest[r][p] = __builtin_bit_cast(unsigned, left);
+        }
+    store_transposed(rows, t.dst + (size_t)c0 * t.ld + r0, t.ld, k - c0);
+    if (t.rest)
+        store_transposed(rest, t.rest + (size_t)c0 * t.ld + r0, t.ld, k - c0);
+}
+
+template <int DOWN>
 __device__ __forceinline__ void transpose_matrix(const Transposed &t, int k, size_t code_stride, size_t scale_stride)
 {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r0 = (blockIdx.x * DOWN + wave / kTilesAcross) * kTile, c0 = (blockIdx.y * kTilesAcross + wave % kTilesAcross) * kTile;
-    if (r0 >= t.q.rows || c0 >= k)
+    if (r0 >= t.of.q.rows || c0 >= k)
         return;
     const int row = r0 + (lane & 7) * 8, col = c0 + (lane >> 3) * 8;
     unsigned codes[8], scales[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         codes[r] = scales[r] = 0;
-        if (row + r < t.q.rows) {
-            codes[r] = *(const unsigned *)(t.q.codes + (size_t)(row + r) * code_stride + col / 2);
-            scales[r] = t.q.scales[(size_t)(row + r) * scale_stride + col / kMxBlock];
+        if (row + r < t.of.q.rows) {
+            codes[r] = *(const unsigned *)(t.of.q.codes + (size_t)(row + r) * code_stride + col / 2);
+            scales[r] = t.of.q.scales[(size_t)(row + r) * scale_stride + col / kMxBlock];
         }
     }
     v4u rows[8];
@@ -285,6 +330,8 @@ __device__ __forceinline__ void transpose_dy(const Prepared &p)
     }
     if (p.transposed)
         store_transposed(rows, p.transposed + (size_t)c0 * p.ld_t + r0, p.ld_t, p.cols - c0);
+    if (p.transposed_again)
+        store_transposed(rows, p.transposed_again + (size_t)c0 * p.ld_t + r0, p.ld_t, p.cols - c0);
     if (p.partial) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -302,14 +349,17 @@ __device__ __forceinline__ void transpose_dy(const Prepared &p)
 }
 
 // blockIdx.z: one of the matrices, or dy behind them.  A workgroup takes DOWN x kTilesAcross tiles.
-template <int DOWN>
+template <int DOWN, bool INT8>
 __global__ __launch_bounds__(DOWN *kTilesAcross * 64) void prepare_kernel(Prepared p, size_t code_stride, size_t scale_stride)
 {
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
         for (int i = threadIdx.x; i < p.zero_count; i += DOWN * kTilesAcross * 64)
             p.zeros[i] = 0;
     if ((int)blockIdx.z < p.matrices)
-        transpose_matrix<DOWN>(p.matrix[blockIdx.z], p.k, code_stride, scale_stride);
+        if constexpr (INT8)
+            transpose_int8<DOWN>(p.matrix[blockIdx.z], p.k);
+        else
+            transpose_matrix<DOWN>(p.matrix[blockIdx.z], p.k, code_stride, scale_stride);
     else
         transpose_dy<DOWN>(p);
 }
@@ -396,7 +446,7 @@ hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
 {
     int rows = p.dy ? p.rows : 0, cols = p.dy ? p.cols : 0;
     for (int i = 0; i < p.matrices; ++i) {
-        rows = max(rows, p.matrix[i].q.rows);
+        rows = max(rows, p.matrix[i].of.q.rows);
         cols = max(cols, p.k);
     }
     if (rows == 0 || cols == 0)
@@ -404,7 +454,10 @@ hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
     auto run = [&](auto down) {
         constexpr int DOWN = decltype(down)::value, kSide = DOWN * kTile, kWide = kTilesAcross * kTile;
         const dim3 grid((unsigned)((rows + kSide - 1) / kSide), (unsigned)((cols + kWide - 1) / kWide), (unsigned)(p.matrices + (p.dy != nullptr)));
-        prepare_kernel<DOWN><<<grid, DOWN * kTilesAcross * 64, 0, stream>>>(p, mx_code_stride(p.k), mx_scale_stride(p.k));
+        if (p.int8)
+            prepare_kernel<DOWN, true><<<grid, DOWN * kTilesAcross * 64, 0, stream>>>(p, 0, 0);
+        else
+            prepare_kernel<DOWN, false><<<grid, DOWN * kTilesAcross * 64, 0, stream>>>(p, mx_code_stride(p.k), mx_scale_stride(p.k));
     };
     if ((long)rows * cols >= kLargeTranspose)
         run(std::integral_constant<int, 4>{});

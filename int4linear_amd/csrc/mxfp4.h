@@ -18,6 +18,7 @@ namespace int4linear {
 constexpr int kMxBlock = 32;      // values that share a scale
 constexpr int kLineBytes = 128;   // codes of 256 k
 constexpr int kLineFp4 = 256;     // k in a line of 4-bit values
+constexpr int kLineInt8 = 128;    // k in a line of 8-bit values
 constexpr int kLineBf16 = 64;     // k in a line of bfloat16
 
 inline size_t mx_code_stride(int k) { return ((size_t)k + 255) / 256 * 128; }
@@ -42,17 +43,25 @@ hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld,
 // dst[c * ld + r] = q[r][c] in bfloat16 for c < k, r going on to the next multiple of 64 with zeros; and of dy (rows x cols
 // bfloat16, contiguous), where they are not null, the transpose (cols x ld_t, zeros behind the rows), a copy whose rows
 // are padded with zeros (rows x ld_p), and every column's sum over 64 rows at a time (partial: ceil(rows / 64) x cols).
-struct Transposed {
+// With `int8` the matrices are codes of 8 bits with a scale for each row (rows padded to 128 bytes), whose products are rounded to
+// bfloat16, and where `rest` is not null what the rounding took away, rounded too, goes there (the same ld).
+struct BackwardOperand {
     MxMatrix q;
+    const float *row_scales = nullptr;
+};
+struct Transposed {
+    BackwardOperand of;
     uint16_t *dst;
     size_t ld;
+    uint16_t *rest;
 };
 struct Prepared {
     Transposed matrix[3];
     int matrices, k;
+    bool int8;
     const uint16_t *dy;
     int rows, cols;
-    uint16_t *transposed, *padded;
+    uint16_t *transposed, *transposed_again, *padded;  // (the transpose a second time, the same ld)
     size_t ld_t, ld_p;
     float *partial;
     unsigned *zeros;  // words to be cleared
