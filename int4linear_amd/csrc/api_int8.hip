@@ -45,7 +45,7 @@ int layer_norm(RowPass p, void *stream)
     p.norm = true;
     DeviceInfo info;
     const int st = api_begin((hipStream_t)stream, &info);
-    return st != INT4LINEAR_OK ? st : api_status(launch_rows(p, (hipStream_t)stream));
+    return st != INT4LINEAR_OK ? st : api_status(launch_rows(p, info, (hipStream_t)stream));
 }
 
 }  // namespace
@@ -77,7 +77,7 @@ int int4linear_int8_quantize(const void *x_d, int type, size_t ld, void *codes_d
     p.result = kRowInt8;
     p.y = codes_d;
     p.scales = scales_d;
-    return api_status(launch_rows(p, (hipStream_t)stream));
+    return api_status(launch_rows(p, info, (hipStream_t)stream));
 }
 
 int int4linear_int8_dequantize(const void *codes_d, const float *scales_d, void *y_d, int type, size_t ld, int rows, int k, void *stream)
@@ -119,7 +119,7 @@ int int4linear_int8_linear(const void *x_codes_d, const float *x_scales_d, const
 
 size_t int4linear_int8_linear_backward_bytes(int m, int n, int k, int dw_type)
 {
-    return linear_backward_bytes(m, n, k, dw_type == INT4LINEAR_OUT_F32);
+    return linear_backward_bytes(m, n, k, dw_type == INT4LINEAR_OUT_F32 ? kPieces : 1);
 }
 
 int int4linear_int8_linear_backward(const void *dy_d, const void *x_codes_d, const float *x_scales_d, const void *w_codes_d,

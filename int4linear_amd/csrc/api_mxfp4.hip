@@ -136,7 +136,7 @@ int int4linear_mxfp4_gated_quantized(const void *x_codes_d, const void *x_scales
                                                 (uint8_t *)h_scales_d, k, info, (hipStream_t)stream));
 }
 
-size_t int4linear_mxfp4_linear_backward_bytes(int m, int n, int k) { return linear_backward_bytes(m, n, k, false); }
+size_t int4linear_mxfp4_linear_backward_bytes(int m, int n, int k) { return linear_backward_bytes(m, n, k, 1); }
 
 int int4linear_mxfp4_linear_backward(const void *dy_d, const void *x_codes_d, const void *x_scales_d, const void *w_codes_d,
                                      const void *w_scales_d, void *dx_d, void *dw_d, int dw_type, float *dbias_d, void *work_d,
@@ -187,10 +187,10 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
     prepared.zeros = p.slices.arrivals;
     prepared.zero_count = m > 0 && n > 0 && k > 0 ? kMostSlices * 4 : 0;
     if (want_dw && m > 0)
-        prepared.matrix[prepared.matrices++] = {{x}, p.x_t, p.ld_m, nullptr};
+        prepared.matrix[prepared.matrices++] = {{x}, p.x_t, p.ld_m, 0};
     if (want_dx && n > 0) {
-        prepared.matrix[prepared.matrices++] = {{wg}, p.w_t, 2 * p.ld_n, nullptr};
-        prepared.matrix[prepared.matrices++] = {{wu}, p.w_t + p.ld_n, 2 * p.ld_n, nullptr};
+        prepared.matrix[prepared.matrices++] = {{wg}, p.w_t, 2 * p.ld_n, 0};
+        prepared.matrix[prepared.matrices++] = {{wu}, p.w_t + p.ld_n, 2 * p.ld_n, 0};
     }
     if (e == hipSuccess)
         e = launch_prepare(prepared, stream);

@@ -45,7 +45,7 @@ struct RowPass {
     size_t ld_y;
     void *scales;        // floats (kRowInt8), bytes (kRowMx)
 };
-hipError_t launch_rows(const RowPass &p, hipStream_t stream);
+hipError_t launch_rows(const RowPass &p, const DeviceInfo &dev, hipStream_t stream);
 
 // Gradients of the norm: dx (of `type`) from dy (of dy_type), and the sums over rows dgamma of dy * (normalised x), dbeta of dy;
 // each may be null.  work: layer_norm_work_bytes(), 256-byte aligned.

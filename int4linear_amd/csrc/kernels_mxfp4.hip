@@ -227,25 +227,29 @@ __device__ __forceinline__ void transpose_int8(const Transposed &t, int k)
             scales[r] = t.of.row_scales[row + r];
         }
     }
-    v4u rows[8], rest[8];
+    float v[8][8];
 #pragma unroll
     for (int r = 0; r < 8; ++r)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            v2bf two, left;
+        for (int c = 0; c < 8; ++c)
+            v[r][c] = (float)(int8_t)(codes[r][c / 4] >> 8 * (c % 4)) * scales[r];
+    uint16_t *dst = t.dst + (size_t)c0 * t.ld + r0;
+    for (int pieces = t.apart ? 3 : 1;;) {
+        v4u rows[8];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = 2 * p + e;
-                const float v = (float)(int8_t)(codes[r][c / 4] >> 8 * (c % 4)) * scales[r];
-                two[e] = (__bf16)v;
-                left[e] = (__bf16)(v - (float)two[e]);
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const v2bf two = {(__bf16)v[r][2 * p], (__bf16)v[r][2 * p + 1]};
+                v[r][2 * p] -= (float)two[0];
+                v[r][2 * p + 1] -= (float)two[1];
+                rows[r][p] = __builtin_bit_cast(unsigned, two);
             }
-            rows[r][p] = __builtin_bit_cast(unsigned, two);
-            rest[r][p] = __builtin_bit_cast(unsigned, left);
-        }
-    store_transposed(rows, t.dst + (size_t)c0 * t.ld + r0, t.ld, k - c0);
-    if (t.rest)
-        store_transposed(rest, t.rest + (size_t)c0 * t.ld + r0, t.ld, k - c0);
+        store_transposed(rows, dst, t.ld, k - c0);
+        if (--pieces == 0)
+            break;
+        dst += t.apart;
+    }
 }
 
 template <int DOWN>
@@ -328,10 +332,11 @@ __device__ __forceinline__ void transpose_dy(const Prepared &p)
             if (row + r < p.rows)
                 *(v4u *)(p.padded + (size_t)(row + r) * p.ld_p + col) = rows[r];
     }
-    if (p.transposed)
+    if (p.transposed) {
         store_transposed(rows, p.transposed + (size_t)c0 * p.ld_t + r0, p.ld_t, p.cols - c0);
-    if (p.transposed_again)
-        store_transposed(rows, p.transposed_again + (size_t)c0 * p.ld_t + r0, p.ld_t, p.cols - c0);
+        for (int i = 1; i < p.copies; ++i)
+            store_transposed(rows, p.transposed + (size_t)c0 * p.ld_t + p.ld_t / p.copies * i + r0, p.ld_t, p.cols - c0);
+    }
     if (p.partial) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {

@@ -16,7 +16,8 @@ template <int TYPE>
 using Element = OutElement<TYPE>;
 
 struct BackwardStatistics {
-    float shift, delta, r, mean_g, mean_gh;
+    RowStatistics of;
+    float mean_g, mean_gh;
 };
 
 struct WorkParts {
@@ -41,6 +42,7 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward 
     constexpr int kWaves = kThreads / 64;
     __shared__ float room[3][2 * kWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const float over_n = 1.0f / (float)p.n;
     for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const Element<TYPE> *x = (const Element<TYPE> *)p.x + (size_t)row * p.ld;
         const Element<DY> *dy = (const Element<DY> *)p.dy + (size_t)row * p.ld_dy;
@@ -53,7 +55,7 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward 
                 sum[0] += v[e];
         }
         group_all<Add>(sum, room[0], wave, kWaves);
-        const float shift = sum[0] / (float)p.n;
+        const float shift = row_shift(sum[0], over_n);
         float two[2] = {};
         for (int c0 = threadIdx.x * 8; c0 < p.n; c0 += kThreads * 8) {
             load8(x, c0, p.n, v);
@@ -61,11 +63,11 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward 
             for (int e = 0; e < 8; ++e) {
                 const float d = c0 + e < p.n ? v[e] - shift : 0.0f;
                 two[0] += d;
-                two[1] += d * d;
+                two[1] = fmaf(d, d, two[1]);
             }
         }
         group_all<Add>(two, room[1], wave, kWaves);
-        const RowStatistics s = RowStatistics::from(shift, two[0], two[1], p.n, p.eps);
+        const RowStatistics s = RowStatistics::from(shift, two[0], two[1], over_n, p.eps);
         float means[2] = {};
         for (int c0 = threadIdx.x * 8; c0 < p.n; c0 += kThreads * 8) {
             load8(x, c0, p.n, v);
@@ -77,13 +79,13 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward 
                 const float a = p.gamma ? g[e] * w[e] : g[e];
                 if (c0 + e < p.n) {
                     means[0] += a;
-                    means[1] += a * s.normalised(v[e]);
+                    means[1] = fmaf(a, s.normalised(v[e] - shift), means[1]);
                 }
             }
         }
         group_all<Add>(means, room[2], wave, kWaves);
         if (threadIdx.x == 0)
-            to[row] = {s.shift, s.delta, s.r, means[0] / (float)p.n, means[1] / (float)p.n};
+            to[row] = {s, means[0] * over_n, means[1] * over_n};
     }
 }
 
@@ -99,26 +101,178 @@ __global__ __launch_bounds__(kThreads) void norm_columns_kernel(NormBackward p, 
     for (int row = first; row < last; ++row) {
         const BackwardStatistics s = of[row];
         const float g = (float)((const Element<DY> *)p.dy)[(size_t)row * p.ld_dy + c];
-        const float h = (((float)((const Element<TYPE> *)p.x)[(size_t)row * p.ld + c] - s.shift) - s.delta) * s.r;
-        dgamma += g * h;
+        const float h = s.of.normalised((float)((const Element<TYPE> *)p.x)[(size_t)row * p.ld + c] - s.of.shift);
+        dgamma = fmaf(g, h, dgamma);
         dbeta += g;
         if (p.dx)
-            ((Element<TYPE> *)p.dx)[(size_t)row * p.ld_dx + c] = (Element<TYPE>)(s.r * (g * w - s.mean_g - h * s.mean_gh));
+            ((Element<TYPE> *)p.dx)[(size_t)row * p.ld_dx + c] = (Element<TYPE>)(s.of.r * (g * w - s.mean_g - h * s.mean_gh));
     }
     float *to = partial + (size_t)blockIdx.y * 2 * p.n + c;
     to[0] = dgamma;
     to[p.n] = dbeta;
 }
 
-// dgamma and dbeta from the strips' sums, in their order.
-__global__ __launch_bounds__(kThreads) void norm_sums_kernel(const float *partial, int strips, int n, float *dgamma, float *dbeta)
+// (128 registers for each of 1024 threads hold eight columns a lane, 256 for each of 512 four times as many.)
+template <int C>
+constexpr int most_threads = C == 1 ? 1024 : 512;
+
+// Rows that fit registers, read once.  WAVES waves share a row, C times eight columns a lane; a workgroup takes blockDim.y rows at a
+// time and stays: gamma and the columns' sums are in registers, the next rows' values on their way while these rows' sums are made.
+// A row's four sums are made in two meetings, since g h summed over the row is r (sum of g d) + c (sum of g) with d = x - shift.  At
+// the end the groups of a workgroup add their columns' sums up in LDS, one after another.
+template <int TYPE, int DY, int WAVES, int C>
+__global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBackward p, float *partial)
 {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= 2 * n)
+    constexpr int kAcross = WAVES * 64 * 8;
+    extern __shared__ float columns[];  // n, where there is more than one group
+    __shared__ float rooms[2][most_threads<C> / 64 * 5];
+    using X = Element<TYPE>;
+    using D = Element<DY>;
+    const int group = threadIdx.y, groups = blockDim.y, first = threadIdx.x * 8;
+    const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const float over_n = 1.0f / (float)p.n;
+    Eight<X> in_x[C];
+    Eight<D> in_dy[C];
+    float gamma[C][8], dgamma[C][8] = {}, dbeta[C][8] = {};
+    auto fetch = [&](int row) {
+        const X *x = (const X *)p.x + (size_t)row * p.ld;
+        const D *dy = (const D *)p.dy + (size_t)row * p.ld_dy;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            fetch8(x, first + i * kAcross, p.n, in_x[i]);
+            fetch8(dy, first + i * kAcross, p.n, in_dy[i]);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        in_x[i] = (Eight<X>)(X)0.0f;
+        in_dy[i] = (Eight<D>)(D)0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            gamma[i][e] = 1.0f;
+        if (p.gamma)
+            load8(p.gamma, first + i * kAcross, p.n, gamma[i]);
+    }
+    const int by = gridDim.x * groups;
+    int row = blockIdx.x * groups + group;
+    if (row < p.rows)
+        fetch(row);
+    // (every group makes as many turns, for their meetings; one without a row has zeros)
+    int turn = 0;
+    for (int base = blockIdx.x * groups; base < p.rows; base += by, row += by, turn ^= 1) {
+        float x[C][8], dy[C][8];
+        const bool there = row < p.rows;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            widen8<X>(in_x[i], x[i]);
+            widen8<D>(in_dy[i], dy[i]);
+        }
+        if (!there) {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[i][e] = dy[i][e] = 0.0f;
+        }
+        if (row + by < p.rows)
+            fetch(row + by);
+        float *room = rooms[turn] + group * WAVES * 5;
+        float sum[1] = {}, four[4] = {};
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                sum[0] += x[i][e];
+        group_all<Add>(sum, room, wave, WAVES);
+        const float shift = row_shift(sum[0], over_n);
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[i][e] -= shift;
+            behind8(first + i * kAcross, p.n, 0.0f, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float g = dy[i][e] * gamma[i][e];
+                four[0] += x[i][e];
+                four[1] = fmaf(x[i][e], x[i][e], four[1]);
+                four[2] += g;
+                four[3] = fmaf(g, x[i][e], four[3]);
+            }
+        }
+        group_all<Add>(four, room + WAVES, wave, WAVES);
+        const RowStatistics s = RowStatistics::from(shift, four[0], four[1], over_n, p.eps);
+        const float mean_g = four[2] * over_n, mean_gh = fmaf(s.r, four[3], s.c * four[2]) * over_n;
+        const float less = -s.r * mean_g, along = -s.r * mean_gh;
+        X *dx = (X *)p.dx + (size_t)row * p.ld_dx;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            float out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float h = s.normalised(x[i][e]), g = dy[i][e] * gamma[i][e];
+                out[e] = fmaf(h, along, fmaf(g, s.r, less));
+                if (there) {
+                    dgamma[i][e] = fmaf(dy[i][e], h, dgamma[i][e]);
+                    dbeta[i][e] += dy[i][e];
+                }
+            }
+            if (there && p.dx && first + i * kAcross < p.n)
+                store8(dx, first + i * kAcross, p.n, out);
+        }
+    }
+    if (!partial)
         return;
+    auto add_groups = [&](float(&sums)[C][8]) {
+        for (int turn = groups - 1; turn >= 0; --turn) {
+            __syncthreads();
+            if (group != turn)
+                continue;
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int c = first + i * kAcross + e;
+                    if (c >= p.n)
+                        continue;
+                    if (turn < groups - 1)
+                        sums[i][e] += columns[c];
+                    if (turn > 0)
+                        columns[c] = sums[i][e];
+                }
+        }
+    };
+    if (groups > 1) {
+        add_groups(dgamma);
+        add_groups(dbeta);
+    }
+    if (group == 0) {
+        float *to = partial + (size_t)blockIdx.x * 2 * p.n;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            store8(to, first + i * kAcross, p.n, dgamma[i]);
+            store8(to + p.n, first + i * kAcross, p.n, dbeta[i]);
+        }
+    }
+}
+
+// dgamma and dbeta from the strips' sums: 64 columns to a workgroup, a wave to every sixteenth strip; the waves' sums in their order.
+__global__ __launch_bounds__(1024) void norm_sums_kernel(const float *partial, int strips, int n, float *dgamma, float *dbeta)
+{
+    __shared__ float part[1024];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
     float sum = 0.0f;
-    for (int s = 0; s < strips; ++s)
-        sum += partial[(size_t)s * 2 * n + c];
+    if (c < 2 * n) {
+#pragma unroll 16
+        for (int s = wave; s < strips; s += 16)
+            sum += partial[(size_t)s * 2 * n + c];
+    }
+    part[threadIdx.x] = sum;
+    __syncthreads();
+    if (wave != 0 || c >= 2 * n)
+        return;
+    for (int w = 1; w < 16; ++w)
+        sum += part[w * 64 + threadIdx.x];
     if (c < n) {
         if (dgamma)
             dgamma[c] = sum;
@@ -128,34 +282,62 @@ __global__ __launch_bounds__(kThreads) void norm_sums_kernel(const float *partia
 }
 
 template <int TYPE, int DY>
-hipError_t launch(const NormBackward &p, hipStream_t stream)
+hipError_t launch(const NormBackward &p, const DeviceInfo &dev, hipStream_t stream)
 {
     const WorkParts w = parts(p.work, p.rows, p.n);
+    const int cus = min(dev.cu_count > 0 ? dev.cu_count : kStrips, kStrips);
+    int strips = 0;
+    auto run = [&](auto waves, auto c) {
+        constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value;
+        const int groups = min((p.rows + cus - 1) / cus, most_threads<C> / 64 / WAVES);
+        strips = min((p.rows + groups - 1) / groups, cus);
+        norm_backward_kernel<TYPE, DY, WAVES, C><<<strips, dim3(WAVES * 64, (unsigned)groups), groups > 1 ? p.n * sizeof(float) : 0, stream>>>(
+            p, p.dgamma || p.dbeta ? w.partial : nullptr);
+    };
+#define I4L_RUN(WAVES, C) run(std::integral_constant<int, WAVES>{}, std::integral_constant<int, C>{})
     if (p.rows > 0) {
-        norm_statistics_kernel<TYPE, DY><<<min(p.rows, 1 << 20), kThreads, 0, stream>>>(p, w.rows);
-        const int strips = strips_of(p.rows), per = (p.rows + strips - 1) / strips;
-        norm_columns_kernel<TYPE, DY><<<dim3((unsigned)((p.n + kThreads - 1) / kThreads), (unsigned)strips), kThreads, 0, stream>>>(p, w.rows, w.partial, per);
+        if (p.n <= 512)
+            I4L_RUN(1, 1);
+        else if (p.n <= 1024)
+            I4L_RUN(2, 1);
+        else if (p.n <= 2048)
+            I4L_RUN(4, 1);
+        else if (p.n <= 4096)
+            I4L_RUN(8, 1);
+        else if (p.n <= 8192)
+            I4L_RUN(16, 1);
+        else if (p.n <= 16384)
+            I4L_RUN(8, 4);
+        else {
+            strips = strips_of(p.rows);
+            norm_statistics_kernel<TYPE, DY><<<min(p.rows, 1 << 20), kThreads, 0, stream>>>(p, w.rows);
+            norm_columns_kernel<TYPE, DY><<<dim3((unsigned)((p.n + kThreads - 1) / kThreads), (unsigned)strips), kThreads, 0, stream>>>(
+                p, w.rows, w.partial, (p.rows + strips - 1) / strips);
+        }
     }
+#undef I4L_RUN
     if (p.dgamma || p.dbeta)
-        norm_sums_kernel<<<(2 * p.n + kThreads - 1) / kThreads, kThreads, 0, stream>>>(w.partial, strips_of(p.rows), p.n, p.dgamma, p.dbeta);
+        norm_sums_kernel<<<(2 * p.n + 63) / 64, 1024, 0, stream>>>(w.partial, strips, p.n, p.dgamma, p.dbeta);
     return hipGetLastError();
 }
 
 template <int TYPE>
-hipError_t by_dy(const NormBackward &p, hipStream_t stream)
+hipError_t by_dy(const NormBackward &p, const DeviceInfo &dev, hipStream_t stream)
 {
-    return p.dy_type == kOutF32   ? launch<TYPE, kOutF32>(p, stream)
-           : p.dy_type == kOutF16 ? launch<TYPE, kOutF16>(p, stream)
-                                  : launch<TYPE, kOutBF16>(p, stream);
+    return p.dy_type == kOutF32   ? launch<TYPE, kOutF32>(p, dev, stream)
+           : p.dy_type == kOutF16 ? launch<TYPE, kOutF16>(p, dev, stream)
+                                  : launch<TYPE, kOutBF16>(p, dev, stream);
 }
 
 }  // namespace
 
 size_t layer_norm_work_bytes(int rows, int n) { return parts(nullptr, rows, n).bytes; }
 
-hipError_t launch_norm_backward(const NormBackward &p, const DeviceInfo &, hipStream_t stream)
+hipError_t launch_norm_backward(const NormBackward &p, const DeviceInfo &dev, hipStream_t stream)
 {
-    return p.type == kOutF32 ? by_dy<kOutF32>(p, stream) : p.type == kOutF16 ? by_dy<kOutF16>(p, stream) : by_dy<kOutBF16>(p, stream);
+    return p.type == kOutF32   ? by_dy<kOutF32>(p, dev, stream)
+           : p.type == kOutF16 ? by_dy<kOutF16>(p, dev, stream)
+                               : by_dy<kOutBF16>(p, dev, stream);
 }
 
 }  // namespace int4linear

@@ -9,6 +9,8 @@ namespace int4linear {
 namespace {
 
 constexpr int kThreads = 256;
+// Fewer rows than this are spread over more waves each.
+constexpr int kFewRows = 1024;
 
 template <int TYPE>
 using Element = OutElement<TYPE>;
@@ -50,26 +52,51 @@ struct RowWriter {
     }
 };
 
-// (x - mean) r gamma + beta of eight columns; what is behind the row's end stays 0.
-__device__ __forceinline__ void normalise8(const RowPass &p, const RowStatistics &s, int c0, float (&v)[8])
+// h gamma + beta of eight columns from d = x - shift; what is behind the row's end becomes 0.
+__device__ __forceinline__ void normalise8(const RowStatistics &s, int c0, int n, const float (&g)[8], const float (&b)[8], float (&v)[8])
 {
-    float g[8], b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        v[e] = fmaf(s.normalised(v[e]), g[e], b[e]);
+    behind8(c0, n, 0.0f, v);
+}
+
+// Columns c0 .. of gamma and beta.
+__device__ __forceinline__ void load_affine(const RowPass &p, int c0, float (&g)[8], float (&b)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        g[e] = 1.0f;
+        b[e] = 0.0f;
+    }
     if (p.gamma)
         load8(p.gamma, c0, p.n, g);
     if (p.beta)
         load8(p.beta, c0, p.n, b);
+}
+
+__device__ __forceinline__ void largest8(const float (&v)[8], unsigned &big)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        big = max(big, __builtin_bit_cast(unsigned, v[e]) & 0x7FFFFFFFu);
+}
+
+// Eight d = x - shift, and their share of the row's sums.
+__device__ __forceinline__ void centre8(float shift, int c0, int n, float (&v)[8], float (&two)[2])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        v[e] -= shift;
+    behind8(c0, n, 0.0f, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        float y = s.normalised(v[e]);
-        if (p.gamma)
-            y *= g[e];
-        if (p.beta)
-            y += b[e];
-        v[e] = c0 + e < p.n ? y : 0.0f;
+        two[0] += v[e];
+        two[1] = fmaf(v[e], v[e], two[1]);
     }
 }
 
-// A workgroup takes a row at a time and reads it again in every pass, from the caches.
+// Rows of any length: a workgroup takes a row at a time and reads it again in every pass, from the caches.
 template <int TYPE, int RESULT, bool NORM>
 __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t code_stride, size_t scale_stride)
 {
@@ -77,10 +104,26 @@ __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t co
     __shared__ float room[3][2 * kWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const RowWriter<RESULT> writer{p, code_stride, scale_stride};
+    const float over_n = 1.0f / (float)p.n;
     for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const Element<TYPE> *x = (const Element<TYPE> *)p.x + (size_t)row * p.ld;
         RowStatistics s{};
         float v[8];
+        // A pass over the row as it leaves: f(first column, eight values).  (Whole quads of lanes, for MXFP4's blocks.)
+        auto pass = [&](int columns, auto &&f) {
+            for (int c0 = threadIdx.x * 8; c0 < columns; c0 += kThreads * 8) {
+                load8(x, c0, p.n, v);
+                if constexpr (NORM) {
+                    float g[8], b[8];
+                    load_affine(p, c0, g, b);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        v[e] -= s.shift;
+                    normalise8(s, c0, p.n, g, b, v);
+                }
+                f(c0, v);
+            }
+        };
         if constexpr (NORM) {
             float sum[1] = {};
             for (int c0 = threadIdx.x * 8; c0 < p.n; c0 += kThreads * 8) {
@@ -90,62 +133,153 @@ __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t co
                     sum[0] += v[e];
             }
             group_all<Add>(sum, room[0], wave, kWaves);
-            const float shift = sum[0] / (float)p.n;
+            const float shift = row_shift(sum[0], over_n);
             float two[2] = {};
             for (int c0 = threadIdx.x * 8; c0 < p.n; c0 += kThreads * 8) {
                 load8(x, c0, p.n, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float d = c0 + e < p.n ? v[e] - shift : 0.0f;
-                    two[0] += d;
-                    two[1] += d * d;
-                }
+                centre8(shift, c0, p.n, v, two);
             }
             group_all<Add>(two, room[1], wave, kWaves);
-            s = RowStatistics::from(shift, two[0], two[1], p.n, p.eps);
+            s = RowStatistics::from(shift, two[0], two[1], over_n, p.eps);
         }
         RowScale scale{};
         if constexpr (RESULT == kRowInt8) {
             unsigned big[1] = {};
-            for (int c0 = threadIdx.x * 8; c0 < p.n; c0 += kThreads * 8) {
-                load8(x, c0, p.n, v);
-                if constexpr (NORM)
-                    normalise8(p, s, c0, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    big[0] = max(big[0], __builtin_bit_cast(unsigned, v[e]) & 0x7FFFFFFFu);
-            }
+            pass(p.n, [&](int, const float(&w)[8]) { largest8(w, big[0]); });
             group_all<Larger>(big, (unsigned *)room[2], wave, kWaves);
             scale = RowScale::of(big[0]);
         }
-        // (whole quads of lanes, for MXFP4's blocks)
-        for (int c0 = threadIdx.x * 8; c0 < writer.columns(p.n); c0 += kThreads * 8) {
-            load8(x, c0, p.n, v);
-            if constexpr (NORM)
-                normalise8(p, s, c0, v);
-            writer.write(row, c0, v, scale);
-        }
+        pass(writer.columns(p.n), [&](int c0, const float(&w)[8]) { writer.write(row, c0, w, scale); });
         if constexpr (!NORM)
             __syncthreads();  // (else the room of one row is used again behind two further meetings)
     }
 }
 
-template <int TYPE, int RESULT, bool NORM>
-hipError_t launch(const RowPass &p, hipStream_t stream)
+// The same with a row in registers, read once: WAVES waves share it (1: a wave has a row to itself, four rows to a workgroup), a lane
+// holds C times eight values, those of chunk i * 64 * WAVES + (its number in the group).  Workgroups stay: gamma and beta are read
+// once, and the next row's values are on their way while this one's sums are made.  (STAYS = false, for rows that leave no registers
+// for either: a row after the other.)
+template <int WAVES, int C>
+constexpr int waves_per_simd = C <= 2 ? 4 : C <= 4 ? 3 : 2;
+
+template <int TYPE, int RESULT, bool NORM, int WAVES, int C, bool STAYS>
+__global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd<WAVES, C>)) void row_kernel(RowPass p, size_t code_stride, size_t scale_stride)
 {
-    const size_t codes = RESULT == kRowInt8 ? int8_code_stride(p.n) : mx_code_stride(p.n);
-    row_loop_kernel<TYPE, RESULT, NORM><<<min(p.rows, 1 << 20), kThreads, 0, stream>>>(p, codes, mx_scale_stride(p.n));
+    constexpr int kAcross = WAVES * 64 * 8, kRows = WAVES == 1 ? kThreads / 64 : 1;
+    __shared__ float room[2][3][2 * WAVES];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int in_row = WAVES == 1 ? 0 : wave, first = (WAVES == 1 ? threadIdx.x & 63 : threadIdx.x) * 8;
+    const RowWriter<RESULT> writer{p, code_stride, scale_stride};
+    const float over_n = 1.0f / (float)p.n;
+    Eight<Element<TYPE>> in[C];
+    auto fetch = [&](int row) {
+        const Element<TYPE> *x = (const Element<TYPE> *)p.x + (size_t)row * p.ld;
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            fetch8(x, first + i * kAcross, p.n, in[i]);
+    };
+    int row = blockIdx.x * kRows + (WAVES == 1 ? wave : 0), turn = 0;
+    if (row >= p.rows)
+        return;
+    fetch(row);
+    float g[C][8], b[C][8];
+    if constexpr (NORM && STAYS)
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            load_affine(p, first + i * kAcross, g[i], b[i]);
+    for (;; turn ^= 1) {
+        const int next = row + gridDim.x * kRows;
+        float v[C][8];
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            widen8<Element<TYPE>>(in[i], v[i]);
+        if (STAYS && next < p.rows)
+            fetch(next);
+        if constexpr (NORM) {
+            float sum[1] = {}, two[2] = {};
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    sum[0] += v[i][e];
+            group_all<Add>(sum, room[turn][0], in_row, WAVES);
+            const float shift = row_shift(sum[0], over_n);
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                centre8(shift, first + i * kAcross, p.n, v[i], two);
+            group_all<Add>(two, room[turn][1], in_row, WAVES);
+            const RowStatistics s = RowStatistics::from(shift, two[0], two[1], over_n, p.eps);
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int c0 = first + i * kAcross;
+                if constexpr (!STAYS)
+                    load_affine(p, c0, g[0], b[0]);
+                normalise8(s, c0, p.n, g[STAYS ? i : 0], b[STAYS ? i : 0], v[i]);
+            }
+        }
+        RowScale scale{};
+        if constexpr (RESULT == kRowInt8) {
+            unsigned big[1] = {};
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                largest8(v[i], big[0]);
+            group_all<Larger>(big, (unsigned *)room[turn][2], in_row, WAVES);
+            scale = RowScale::of(big[0]);
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (first + i * kAcross < writer.columns(p.n))
+                writer.write(row, first + i * kAcross, v[i], scale);
+        row = next;
+        if (row >= p.rows)
+            break;
+        if constexpr (!STAYS)
+            fetch(row);
+    }
+}
+
+template <int TYPE, int RESULT, bool NORM>
+hipError_t launch(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
+{
+    const size_t codes = RESULT == kRowInt8 ? int8_code_stride(p.n) : mx_code_stride(p.n), scales = mx_scale_stride(p.n);
+    const int cus = dev.cu_count > 0 ? dev.cu_count : 256;
+    auto run = [&](auto waves, auto c, auto stays) {
+        constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value, kRows = WAVES == 1 ? kThreads / 64 : 1;
+        constexpr bool STAYS = decltype(stays)::value;
+        constexpr int kPlaces = 4 * waves_per_simd<WAVES, C> / (WAVES == 1 ? kThreads / 64 : WAVES);  // workgroups of a CU
+        const int groups = min((p.rows + kRows - 1) / kRows, cus * kPlaces);
+        row_kernel<TYPE, RESULT, NORM, WAVES, C, STAYS><<<groups, WAVES == 1 ? kThreads : WAVES * 64, 0, stream>>>(p, codes, scales);
+        return hipGetLastError();
+    };
+    using std::integral_constant;
+#define I4L_RUN(WAVES, C, STAYS) run(integral_constant<int, WAVES>{}, integral_constant<int, C>{}, std::bool_constant<STAYS>{})
+    // (floats take twice the registers on their way: no more than two eights of them to a lane)
+    const bool wide = p.rows < kFewRows || TYPE == kOutF32;
+    if (p.n <= 512)
+        return I4L_RUN(1, 1, true);
+    if (p.n <= 1024)
+        return I4L_RUN(1, 2, true);
+    if (p.n <= 2048)
+        return wide ? I4L_RUN(4, 1, true) : I4L_RUN(1, 4, true);
+    if (p.n <= 4096)
+        return p.rows < kFewRows ? I4L_RUN(8, 1, true) : I4L_RUN(4, 2, true);
+    if (p.n <= 8192)
+        return wide ? I4L_RUN(8, 2, true) : I4L_RUN(4, 4, true);
+    if (p.n <= 16384)
+        return wide ? I4L_RUN(16, 2, true) : I4L_RUN(8, 4, true);
+#undef I4L_RUN
+    row_loop_kernel<TYPE, RESULT, NORM><<<min(p.rows, 1 << 20), kThreads, 0, stream>>>(p, codes, scales);
     return hipGetLastError();
 }
 
 template <int TYPE>
-hipError_t by_result(const RowPass &p, hipStream_t stream)
+hipError_t by_result(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
 {
     if (!p.norm)
-        return launch<TYPE, kRowInt8, false>(p, stream);
+        return launch<TYPE, kRowInt8, false>(p, dev, stream);
     if (p.result == kRowTyped)
-        return launch<TYPE, kRowTyped, true>(p, stream);
-    return p.result == kRowInt8 ? launch<TYPE, kRowInt8, true>(p, stream) : launch<TYPE, kRowMx, true>(p, stream);
+        return launch<TYPE, kRowTyped, true>(p, dev, stream);
+    return p.result == kRowInt8 ? launch<TYPE, kRowInt8, true>(p, dev, stream) : launch<TYPE, kRowMx, true>(p, dev, stream);
 }
 
 // A thread takes eight values at a time.
@@ -176,11 +310,11 @@ hipError_t dequantize(const Int8Matrix &q, void *y, size_t ld, int k, hipStream_
 
 }  // namespace
 
-hipError_t launch_rows(const RowPass &p, hipStream_t stream)
+hipError_t launch_rows(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
 {
-    return p.type == kOutF32   ? by_result<kOutF32>(p, stream)
-           : p.type == kOutF16 ? by_result<kOutF16>(p, stream)
-                               : by_result<kOutBF16>(p, stream);
+    return p.type == kOutF32   ? by_result<kOutF32>(p, dev, stream)
+           : p.type == kOutF16 ? by_result<kOutF16>(p, dev, stream)
+                               : by_result<kOutBF16>(p, dev, stream);
 }
 
 hipError_t launch_int8_dequantize(const Int8Matrix &q, void *y, int type, size_t ld, int k, hipStream_t stream)

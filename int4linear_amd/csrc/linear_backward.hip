@@ -21,15 +21,15 @@ struct LinearBackwardParts {
     size_t ld_m, ld_n, bytes;
 };
 
-LinearBackwardParts linear_backward_parts(void *work, int m, int n, int k, bool split)
+LinearBackwardParts linear_backward_parts(void *work, int m, int n, int k, int pieces)
 {
     Parts p{(uint8_t *)work};
     LinearBackwardParts r{};
     r.ld_m = up((size_t)m, 64);
     r.ld_n = up((size_t)n, 64);
-    r.dy_t = p.take<uint16_t>((size_t)n * r.ld_m * (split ? 2 : 1));
+    r.dy_t = p.take<uint16_t>((size_t)n * r.ld_m * pieces);
     r.dy_padded = p.take<uint16_t>(n % 64 ? (size_t)m * r.ld_n : 0);
-    r.x_t = p.take<uint16_t>((size_t)k * r.ld_m * (split ? 2 : 1));
+    r.x_t = p.take<uint16_t>((size_t)k * r.ld_m * pieces);
     r.w_t = p.take<uint16_t>((size_t)k * r.ld_n);
     r.sums = p.take<float>((size_t)n * (r.ld_m / 64));
     r.slices = slice_space(p, m > 0 && n > 0 && k > 0);
@@ -39,9 +39,9 @@ LinearBackwardParts linear_backward_parts(void *work, int m, int n, int k, bool 
 
 }  // namespace
 
-size_t linear_backward_bytes(int m, int n, int k, bool split)
+size_t linear_backward_bytes(int m, int n, int k, int pieces)
 {
-    return m < 0 || n < 0 || k < 0 ? 0 : linear_backward_parts(nullptr, m, n, k, split).bytes;
+    return m < 0 || n < 0 || k < 0 ? 0 : linear_backward_parts(nullptr, m, n, k, pieces).bytes;
 }
 
 int linear_backward(const void *dy, const BackwardOperand &x, const BackwardOperand &w, bool int8, void *dx, void *dw, int dw_type,
@@ -65,8 +65,11 @@ int linear_backward(const void *dy, const BackwardOperand &x, const BackwardOper
         check(x);
     if (want_dx)
         check(w);
-    const bool split = int8 && dw && dw_type == INT4LINEAR_OUT_F32;
-    const LinearBackwardParts p = linear_backward_parts(work, m, n, k, split);
+    const int pieces = int8 && dw && dw_type == INT4LINEAR_OUT_F32 ? kPieces : 1;
+    ok.that(pieces == 1 || m <= kMostInPieces, INT4LINEAR_ERR_UNSUPPORTED);
+    if (!ok)
+        return ok.status;
+    const LinearBackwardParts p = linear_backward_parts(work, m, n, k, pieces);
     ok.array(work, 256, p.bytes > 0).that(work_bytes >= p.bytes, INT4LINEAR_ERR_SCRATCH);
     if (!ok)
         return ok.status;
@@ -75,22 +78,22 @@ int linear_backward(const void *dy, const BackwardOperand &x, const BackwardOper
     if (st != INT4LINEAR_OK)
         return st;
     const bool ragged = n % 64 != 0;
-    const size_t ld_sum = p.ld_m * (split ? 2 : 1);  // of what dw sums over
+    const size_t ld_sum = p.ld_m * pieces;  // of what dw sums over
     Prepared prepared{};
     prepared.k = k;
     prepared.int8 = int8;
     prepared.zeros = p.slices.arrivals;
     prepared.zero_count = m > 0 && n > 0 && k > 0 ? kMostSlices * 4 : 0;
     if (want_dw && m > 0)
-        prepared.matrix[prepared.matrices++] = {x, p.x_t, ld_sum, split ? p.x_t + p.ld_m : nullptr};
+        prepared.matrix[prepared.matrices++] = {x, p.x_t, ld_sum, pieces > 1 ? p.ld_m : 0};
     if (want_dx && n > 0)
-        prepared.matrix[prepared.matrices++] = {w, p.w_t, p.ld_n, nullptr};
+        prepared.matrix[prepared.matrices++] = {w, p.w_t, p.ld_n, 0};
     if (m > 0 && n > 0 && (want_dw || want_sums || ragged)) {
         prepared.dy = (const uint16_t *)dy;
         prepared.rows = m;
         prepared.cols = n;
         prepared.transposed = want_dw ? p.dy_t : nullptr;
-        prepared.transposed_again = want_dw && split ? p.dy_t + p.ld_m : nullptr;
+        prepared.copies = pieces;
         prepared.ld_t = ld_sum;
         prepared.padded = want_dx && ragged ? p.dy_padded : nullptr;
         prepared.ld_p = p.ld_n;
@@ -98,7 +101,7 @@ int linear_backward(const void *dy, const BackwardOperand &x, const BackwardOper
     }
     hipError_t e = launch_prepare(prepared, stream);
     const Bf16Product products[] = {
-        {p.dy_t, n, p.x_t, k, ld_sum, split && m > 0 ? (int)ld_sum : m, want_dw ? dw : nullptr, dw_type},
+        {p.dy_t, n, p.x_t, k, ld_sum, pieces > 1 && m > 0 ? (int)ld_sum : m, want_dw ? dw : nullptr, dw_type},
         {ragged ? p.dy_padded : (const uint16_t *)dy, m, p.w_t, k, p.ld_n, n, want_dx ? dx : nullptr, kOutBF16}};
     const ColumnSums sums{want_sums ? dbias : nullptr, p.sums, (int)(p.ld_m / 64), n};
     if (e == hipSuccess)

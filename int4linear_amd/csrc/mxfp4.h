@@ -44,7 +44,8 @@ hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld,
 // bfloat16, contiguous), where they are not null, the transpose (cols x ld_t, zeros behind the rows), a copy whose rows
 // are padded with zeros (rows x ld_p), and every column's sum over 64 rows at a time (partial: ceil(rows / 64) x cols).
 // With `int8` the matrices are codes of 8 bits with a scale for each row (rows padded to 128 bytes), whose products are rounded to
-// bfloat16, and where `rest` is not null what the rounding took away, rounded too, goes there (the same ld).
+// bfloat16; where `apart` is not 0 what the rounding took away, rounded too, goes that many elements further on, and what is left of
+// that as far again.
 struct BackwardOperand {
     MxMatrix q;
     const float *row_scales = nullptr;
@@ -52,8 +53,7 @@ struct BackwardOperand {
 struct Transposed {
     BackwardOperand of;
     uint16_t *dst;
-    size_t ld;
-    uint16_t *rest;
+    size_t ld, apart;
 };
 struct Prepared {
     Transposed matrix[3];
@@ -61,7 +61,8 @@ struct Prepared {
     bool int8;
     const uint16_t *dy;
     int rows, cols;
-    uint16_t *transposed, *transposed_again, *padded;  // (the transpose a second time, the same ld)
+    uint16_t *transposed, *padded;
+    int copies;  // of the transpose, side by side: ld_t / copies elements between them
     size_t ld_t, ld_p;
     float *partial;
     unsigned *zeros;  // words to be cleared

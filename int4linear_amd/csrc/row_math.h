@@ -7,24 +7,49 @@ namespace int4linear {
 
 typedef int row_v2i __attribute__((ext_vector_type(2)));
 
-// Values c0 .. c0 + 7 of a row of n as floats, zeros behind its end.  (16 bytes of 16-bit types at once, aligned to the element
+// Values c0 .. c0 + 7 of a row of n as they are, zeros behind its end.  (16 bytes of 16-bit types at once, aligned to the element
 // only: the hardware splits those that are not aligned to more.)
 template <class T>
-__device__ __forceinline__ void load8(const T *row, int c0, int n, float (&v)[8])
+using Eight = T __attribute__((ext_vector_type(8)));
+
+template <class T>
+__device__ __forceinline__ void fetch8(const T *row, int c0, int n, Eight<T> &in)
 {
-    typedef T v8t __attribute__((ext_vector_type(8)));
-    v8t in = (v8t)(T)0.0f;
+    in = (Eight<T>)(T)0.0f;
     if (c0 + 8 <= n) {
-        __builtin_memcpy(&in, row + c0, sizeof(v8t));
+        __builtin_memcpy(&in, row + c0, sizeof(in));
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (c0 + e < n)
                 in[e] = row[c0 + e];
     }
+}
+
+template <class T>
+__device__ __forceinline__ void widen8(const Eight<T> &in, float (&v)[8])
+{
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         v[e] = (float)in[e];
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T *row, int c0, int n, float (&v)[8])
+{
+    Eight<T> in;
+    fetch8(row, c0, n, in);
+    widen8<T>(in, v);
+}
+
+// What is behind the row's end set to `value`.
+__device__ __forceinline__ void behind8(int c0, int n, float value, float (&v)[8])
+{
+    if (c0 + 8 > n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = c0 + e < n ? v[e] : value;
+    }
 }
 
 // The other way, rounded to T.
@@ -108,18 +133,29 @@ __device__ __forceinline__ void group_all(T (&v)[N], T *room, int wave, int wave
     }
 }
 
-// A row's mean is `shift` + `delta` with shift a first sum's (rounded) mean, so that what is squared and summed next is centred: the
+// What all values of a row are centred on.  It has to be one number: left in sight, the product would be merged with some of the
+// differences that take it and not with others, and so be rounded for these alone.
+__device__ __forceinline__ float row_shift(float sum, float over_n)
+{
+    float shift = sum * over_n;
+    asm("" : "+v"(shift));
+    return shift;
+}
+
+// A row's mean is `shift` + delta with shift a first sum's (rounded) mean, so that what is squared and summed next is centred: the
 // variance is the mean of (x - shift)^2 less delta^2, a correction of the first sum's rounding and no cancellation.
+// h = (x - mean) / sqrt(variance + eps) is d r + c with d = x - shift, one rounding.
 struct RowStatistics {
-    float shift, delta, r;  // r = 1 / sqrt(variance + eps)
-    __device__ static RowStatistics from(float shift, float sum, float squares, int n, float eps)
+    float shift, r, c;
+    __device__ static RowStatistics from(float shift, float sum, float squares, float over_n, float eps)
     {
-        const float delta = sum / (float)n;
-        const float variance = fmaxf(squares / (float)n - delta * delta, 0.0f);
+        const float delta = sum * over_n;
+        const float variance = fmaxf(squares * over_n - delta * delta, 0.0f);
         // (fmaxf takes a NaN away: rows with infinities or NaNs become NaN)
-        return {shift, delta, 1.0f / sqrtf((squares == squares ? variance : squares) + eps)};
+        const float r = rsqrtf((squares == squares ? variance : squares) + eps);
+        return {shift, r, -delta * r};
     }
-    __device__ __forceinline__ float normalised(float x) const { return ((x - shift) - delta) * r; }
+    __device__ __forceinline__ float normalised(float d) const { return fmaf(d, r, c); }
 };
 
 // The 8-bit format's scale of a row whose largest magnitude has the bits `big` (NaN above infinity above all numbers), and what
@@ -137,30 +173,36 @@ struct RowScale {
 
 // v / scale to the nearest whole number, ties to the even one, decided exactly: the product with the rounded inverse is within
 // 1e-4 of the quotient, and what is left of v is exact in one fused operation.  Beyond half a scale the neighbour is nearer, at
-// half a scale the even one is taken.
+// half a scale the even one is taken.  (Added to 1.5 * 2^23 a number is rounded to a whole one, whose low byte is then the code.)
 __device__ __forceinline__ void encode_int8(const float (&v)[8], const RowScale &s, row_v2i &codes)
 {
-    float q[8], left[8], most = 0.0f;
+    constexpr float kWhole = 12582912.0f;
+    float t[8], left[8], most = 0.0f;
     const float half = 0.5f * s.scale;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        q[e] = rintf(v[e] * s.inverse);
-        left[e] = fmaf(-q[e], s.scale, v[e]);
+        t[e] = fmaf(v[e], s.inverse, kWhole);
+        left[e] = fmaf(kWhole - t[e], s.scale, v[e]);
         most = fmaxf(most, fabsf(left[e]));
     }
     if (most >= half) {  // rare
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float a = fabsf(left[e]);
-            const bool odd = ((int)q[e] & 1) != 0;
+            const bool odd = (__builtin_bit_cast(unsigned, t[e]) & 1u) != 0;
             if (a > half || (a == half && odd))
-                q[e] += left[e] > 0.0f ? 1.0f : -1.0f;
+                t[e] += left[e] > 0.0f ? 1.0f : -1.0f;
         }
     }
-    unsigned bytes[2] = {};
+    unsigned bytes[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        bytes[e / 4] |= ((unsigned)(int)q[e] & 0xFFu) << (8 * (e % 4));
+    for (int w = 0; w < 2; ++w) {
+        unsigned two[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            two[h] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, t[4 * w + 2 * h + 1]), __builtin_bit_cast(unsigned, t[4 * w + 2 * h]), 0x0C0C0400u);
+        bytes[w] = two[0] | two[1] << 16;
+    }
     codes = s.scale == s.scale ? (row_v2i){(int)bytes[0], (int)bytes[1]} : (row_v2i)0;
 }
 

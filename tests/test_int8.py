@@ -63,7 +63,10 @@ def test_refusals_of_the_gradients():
     most = (1 << 22) - 64
     for sizes, status in (((most, 1, 1), SCRATCH), ((1, most, 1), SCRATCH), ((1, 1, most), SCRATCH), ((most + 1, 1, 1), UNSUPPORTED),
                           ((1, most + 1, 1), UNSUPPORTED), ((1, 1, most + 1), UNSUPPORTED)):
-        assert b(A, A, A, A, A, A, A, 1, A, A, 0, *sizes, None) == status
+        assert b(A, A, A, A, A, A, A, 3, A, A, 0, *sizes, None) == status
+    for m, status in ((1 << 21, SCRATCH), ((1 << 21) + 1, UNSUPPORTED)):  # in three pieces
+        assert b(A, A, A, A, A, A, A, 1, A, A, 0, m, 1, 1, None) == status
+        assert b(A, A, A, A, A, A, None, 1, A, A, 0, m, 1, 1, None) == SCRATCH
 
 
 @pytest.mark.parametrize("wrong", [b"sixteen bytes...", "text", [1, 2], 4096.0])
@@ -264,11 +267,11 @@ def test_linear_backward(gpu, m, n, k, dw_type):
     torch.cuda.synchronize()
     assert untouched(raw) and untouched(raw_x) and untouched(raw_w) and untouched(raw_b)
     d = dy.double()
-    # float sums of n (m) terms, each with one factor rounded to bfloat16 or to the sum of two
+    # float sums of n (m) terms, each with one factor rounded to bfloat16 or, in three pieces of a float, 3 m of them
     size_x, size_w = d.abs() @ w.abs(), d.abs().T @ x.abs()
     got_x, got_w, got_b = dx.view(torch.bfloat16).view(m, k), dw.view(ref.DTYPE[dw_type]).view(n, k), db.view(torch.float32)
     ref.check(got_x, d @ w, (2.0**-8 + n * 2.0**-23) * size_x, "bf16")
-    ref.check(got_w, d.T @ x, ((2.0**-8 if dw_type == "bf16" else 2.0**-16) * 1.01 + 2 * m * 2.0**-23) * size_w, dw_type)
+    ref.check(got_w, d.T @ x, ((2.0**-8 if dw_type == "bf16" else 2.0**-24) + 3 * m * 2.0**-23) * size_w, dw_type)
     ref.check(got_b, d.sum(0), m * 2.0**-23 * d.abs().sum(0), "f32")
     # any of them alone: the same bits
     for which in range(3):
@@ -279,17 +282,16 @@ def test_linear_backward(gpu, m, n, k, dw_type):
 
 @pytest.mark.gpu
 def test_gradients_as_floats_keep_the_values_bits(gpu):
-    """One token with dy = 1: dw is X itself, to 2^-16; a scale with a bfloat16's bits gives it exactly."""
+    """One token with dy = 1: dw is X itself as a float, to the last bit."""
     k = 300
     codes = torch.randint(-128, 128, (1, 384), dtype=torch.int8, generator=torch.Generator().manual_seed(1)).cuda()
     codes[:, k:] = 0
     dy, work = torch.ones(1, 8, dtype=torch.bfloat16, device="cuda"), torch.empty(1 << 25, dtype=torch.uint8, device="cuda")
-    for scale, error in ((0.7310586, 2.0**-16), (0.75, 0.0)):
+    for scale in (0.7310586, 0.75):
         dw = torch.empty(8, k, device="cuda")
         s = torch.tensor([scale], device="cuda")
         lib.int8_linear_backward(dy, codes, s, None, None, None, dw, "f32", None, work, 1, 8, k)
-        want = ref.decode(codes, s, k).expand(8, k)
-        ref.check(dw, want, error * want.abs(), "f32")
+        assert torch.equal(dw, (codes[:, :k].float() * s).expand(8, k))
 
 
 @pytest.mark.gpu
