@@ -164,8 +164,8 @@ __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBack
         const bool there = row < p.rows;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            widen8<X>(in_x[i], x[i]);
-            widen8<D>(in_dy[i], dy[i]);
+            widen8<X>(in_x[i], first + i * kAcross, p.n, x[i]);
+            widen8<D>(in_dy[i], first + i * kAcross, p.n, dy[i]);
         }
         if (!there) {
 #pragma unroll
@@ -301,11 +301,11 @@ hipError_t launch(const NormBackward &p, const DeviceInfo &dev, hipStream_t stre
         else if (p.n <= 1024)
             I4L_RUN(2, 1);
         else if (p.n <= 2048)
-            I4L_RUN(4, 1);
+            I4L_RUN(2, 2);
         else if (p.n <= 4096)
-            I4L_RUN(8, 1);
+            I4L_RUN(4, 2);
         else if (p.n <= 8192)
-            I4L_RUN(16, 1);
+            I4L_RUN(8, 2);
         else if (p.n <= 16384)
             I4L_RUN(8, 4);
         else {

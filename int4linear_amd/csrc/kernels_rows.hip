@@ -192,8 +192,8 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
         float v[C][8];
 #pragma unroll
         for (int i = 0; i < C; ++i)
-            widen8<Element<TYPE>>(in[i], v[i]);
-        if (STAYS && next < p.rows)
+            widen8<Element<TYPE>>(in[i], first + i * kAcross, p.n, v[i]);
+        if (NORM && STAYS && next < p.rows)
             fetch(next);
         if constexpr (NORM) {
             float sum[1] = {}, two[2] = {};
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
         row = next;
         if (row >= p.rows)
             break;
-        if constexpr (!STAYS)
+        if constexpr (!NORM || !STAYS)
             fetch(row);
     }
 }
@@ -247,7 +247,8 @@ hipError_t launch(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
         constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value, kRows = WAVES == 1 ? kThreads / 64 : 1;
         constexpr bool STAYS = decltype(stays)::value;
         constexpr int kPlaces = 4 * waves_per_simd<WAVES, C> / (WAVES == 1 ? kThreads / 64 : WAVES);  // workgroups of a CU
-        const int groups = min((p.rows + kRows - 1) / kRows, cus * kPlaces);
+        // (without gamma and beta there is nothing to stay for: 8192 x 14336 63 us, and 71 where workgroups stay)
+        const int groups = min((p.rows + kRows - 1) / kRows, NORM ? cus * kPlaces : 1 << 20);
         row_kernel<TYPE, RESULT, NORM, WAVES, C, STAYS><<<groups, WAVES == 1 ? kThreads : WAVES * 64, 0, stream>>>(p, codes, scales);
         return hipGetLastError();
     };

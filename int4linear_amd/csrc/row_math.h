@@ -7,8 +7,9 @@ namespace int4linear {
 
 typedef int row_v2i __attribute__((ext_vector_type(2)));
 
-// Values c0 .. c0 + 7 of a row of n as they are, zeros behind its end.  (16 bytes of 16-bit types at once, aligned to the element
-// only: the hardware splits those that are not aligned to more.)
+// Eight values of a row of n for columns c0 .. c0 + 7, on their way to a lane: at the row's end the row's last eight, to be brought to
+// their places when they are used (a load that has not been waited for cannot be).  16 bytes of 16-bit types at once, aligned to the
+// element only: the hardware splits those that are not aligned to more.
 template <class T>
 using Eight = T __attribute__((ext_vector_type(8)));
 
@@ -16,22 +17,32 @@ template <class T>
 __device__ __forceinline__ void fetch8(const T *row, int c0, int n, Eight<T> &in)
 {
     in = (Eight<T>)(T)0.0f;
-    if (c0 + 8 <= n) {
-        __builtin_memcpy(&in, row + c0, sizeof(in));
-    } else {
+    if (n >= 8) {
+        if (c0 < n)
+            __builtin_memcpy(&in, row + min(c0, n - 8), sizeof(in));
+    } else if (c0 == 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c0 + e < n)
-                in[e] = row[c0 + e];
+        for (int e = 0; e < 7; ++e)
+            if (e < n)
+                in[e] = row[e];
     }
 }
 
+// As floats, zeros behind the row's end.
 template <class T>
-__device__ __forceinline__ void widen8(const Eight<T> &in, float (&v)[8])
+__device__ __forceinline__ void widen8(const Eight<T> &in, int c0, int n, float (&v)[8])
 {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         v[e] = (float)in[e];
+    if (c0 + 8 > n && n >= 8) {
+        const int over = c0 + 8 - n;  // (behind the end: zeros in any order)
+#pragma unroll
+        for (int by = 4; by > 0; by /= 2)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = over & by ? (e + by < 8 ? v[e + by] : 0.0f) : v[e];
+    }
 }
 
 template <class T>
@@ -39,7 +50,7 @@ __device__ __forceinline__ void load8(const T *row, int c0, int n, float (&v)[8]
 {
     Eight<T> in;
     fetch8(row, c0, n, in);
-    widen8<T>(in, v);
+    widen8<T>(in, c0, n, v);
 }
 
 // What is behind the row's end set to `value`.
@@ -52,22 +63,30 @@ __device__ __forceinline__ void behind8(int c0, int n, float value, float (&v)[8
     }
 }
 
-// The other way, rounded to T.
+// The other way, rounded to T; what is left at the row's end in four, two and one.
 template <class T>
 __device__ __forceinline__ void store8(T *row, int c0, int n, const float (&v)[8])
 {
-    typedef T v8t __attribute__((ext_vector_type(8)));
-    v8t out;
+    typedef T Four __attribute__((ext_vector_type(4)));
+    typedef T Two __attribute__((ext_vector_type(2)));
+    Eight<T> out;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         out[e] = (T)v[e];
     if (c0 + 8 <= n) {
-        __builtin_memcpy(row + c0, &out, sizeof(v8t));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c0 + e < n)
-                row[c0 + e] = out[e];
+        __builtin_memcpy(row + c0, &out, sizeof(out));
+    } else if (c0 < n) {
+        const int left = n - c0;
+        T *to = row + c0;
+        const Four four = {out[0], out[1], out[2], out[3]};
+        const Two two = left & 4 ? (Two){out[4], out[5]} : (Two){out[0], out[1]};
+        const T one = left & 4 ? (left & 2 ? out[6] : out[4]) : (left & 2 ? out[2] : out[0]);
+        if (left & 4)
+            __builtin_memcpy(to, &four, sizeof(four));
+        if (left & 2)
+            __builtin_memcpy(to + (left & 4), &two, sizeof(two));
+        if (left & 1)
+            to[left & 6] = one;
     }
 }
 
