@@ -21,7 +21,8 @@ LIB_PATH = LIB_DIR / "libint4linear.so"
 
 HIP_SOURCES = ["api.hip", "kernels_simple.hip", "kernels_mfma.hip", "kernels_grid.hip", "kernels_fp6.hip", "kernels_fp6_grid.hip",
                "kernels_skinny.hip", "kernels_skinny_any.hip", "api_mxfp4.hip", "kernels_mxfp4.hip", "kernels_line_gemm.hip",
-               "kernels_mxfp4_skinny.hip", "linear_backward.hip", "api_int8.hip", "kernels_rows.hip", "kernels_norm_backward.hip"]
+               "kernels_mxfp4_skinny.hip", "linear_backward.hip", "api_int8.hip", "kernels_rows.hip", "kernels_norm_backward.hip",
+               "kernels_int8_skinny.hip"]
 CXX_SOURCES = ["packer_host.cpp"]
 
 # Packed-FP32 VALU forms are switched off for every device compile of this project.
@@ -44,6 +45,7 @@ HIP_FLAGS = [
 EXTRA_HIP_FLAGS = {
     "kernels_skinny.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
     "kernels_skinny_any.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
+    "kernels_int8_skinny.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
     "kernels_mxfp4_skinny.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
 }
 

@@ -1,6 +1,7 @@
 // C ABI of libint4linear.so, shape dispatch, and the reference's C++-linkage shims.
 #include "../../include/int4linear.h"
 #include "kernels.h"
+#include "int8.h"
 #include "mxfp4.h"
 
 #include <atomic>
@@ -87,6 +88,8 @@ hipError_t set_up_device(PerDevice &pd, int dev)
         err = skinny_init(pd.info);
     if (err == hipSuccess)
         err = line_gemm_init(pd.info);
+    if (err == hipSuccess)
+        err = int8_skinny_init();
     if (err == hipSuccess)  // `dev` is current here: the addresses are this device's copies
         err = hipGetSymbolAddress((void **)&pd.scratch, HIP_SYMBOL(scratch));
     if (err == hipSuccess)

@@ -25,6 +25,11 @@ struct Int8Matrix {
 hipError_t launch_int8_linear(const Int8Matrix &x, const Int8Matrix &w, const float *bias, void *y, int out, int k, const DeviceInfo &dev,
                               hipStream_t stream);
 
+// The same for up to 64 rows of x (k > 0): w is streamed (kernels_int8_skinny.hip).
+hipError_t int8_skinny_init();
+bool int8_skinny_preferred(int m, int n);
+hipError_t launch_int8_skinny(const Int8Matrix &x, const Int8Matrix &w, const float *bias, void *y, int out, int k, hipStream_t stream);
+
 // y (rows x k of `type`, ld elements between rows) = what q stands for.
 hipError_t launch_int8_dequantize(const Int8Matrix &q, void *y, int type, size_t ld, int k, hipStream_t stream);
 

@@ -1024,6 +1024,8 @@ hipError_t launch_mx_linear(const MxMatrix &x, const MxMatrix &w, const float *b
 hipError_t launch_int8_linear(const Int8Matrix &x, const Int8Matrix &w, const float *bias, void *y, int out, int k, const DeviceInfo &dev,
                               hipStream_t stream)
 {
+    if (k > 0 && int8_skinny_preferred(x.rows, w.rows))
+        return launch_int8_skinny(x, w, bias, y, out, k, stream);
     return by_type(out, w.rows, [&](auto type, auto columns) {
         constexpr int OUT = decltype(type)::value;
         if (k == 0)
