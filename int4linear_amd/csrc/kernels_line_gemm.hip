@@ -158,12 +158,20 @@ struct Int8Epilogue {
     size_t ld;
     int m, n;
 
-    // Elements 8 (t / 4) + t % 4 of v from `first` on, of which there are `count` (those behind: the last again).
-    static __device__ __forceinline__ void sixteen(const float *v, int first, int count, float (&out)[16])
+    // The elements of v that belong to a lane's 16 results of a block that begins at element `from` of `count`: from + 8 (t / 4) +
+    // 4 (lane / 32) + t % 4.  (Columns of this form come in fours of which all are there or none: loaded without a question for each,
+    // which would cost more than the loads.)
+    static __device__ __forceinline__ void of_columns(const float *v, int from, int count, int lane, float (&out)[16])
+    {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            __builtin_memcpy(&out[4 * q], v + (unsigned)min(from + 8 * q + 4 * (lane >> 5), count - 4), 16);
+    }
+    static __device__ __forceinline__ void of_rows(const float *v, int from, int count, int lane, float (&out)[16])
     {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int at = first + 8 * q;
+            const int at = from + 8 * q + 4 * (lane >> 5);
             if (at + 4 <= count) {
                 __builtin_memcpy(&out[4 * q], v + at, 16);
             } else {
@@ -177,7 +185,7 @@ struct Int8Epilogue {
     template <int FM, int FN>
     __device__ __forceinline__ void operator()(v16i (&acc)[FM][FN], int row, int col, int lane) const
     {
-        const int one = lane & 31, four = 4 * (lane >> 5);
+        const int one = lane & 31;
         if constexpr (COLUMNS) {
             float ws[FN], add[FN];
 #pragma unroll
@@ -189,7 +197,7 @@ struct Int8Epilogue {
 #pragma unroll
             for (int j = 0; j < FM; ++j) {
                 float xs[16];
-                sixteen(x_scales, row + kFrag * j + four, m, xs);
+                of_rows(x_scales, row + kFrag * j, m, lane, xs);
 #pragma unroll
                 for (int i = 0; i < FN; ++i) {
                     float v[16];
@@ -200,27 +208,37 @@ struct Int8Epilogue {
                 }
             }
         } else {
+            // (Two blocks side by side are a line of 16-bit results: its halves leave one after the other, where there are registers for it.  With a column of blocks after
+            // the other 8192 x 8192 x 2048 takes 155 us, so 151.)
+            constexpr int kSide = FN > 2 ? 2 : 1;
             float xs[FM];
 #pragma unroll
             for (int j = 0; j < FM; ++j)
                 xs[j] = x_scales[min(row + kFrag * j + one, m - 1)];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                float ws[16], add[16];
-                sixteen(w_scales, col + kFrag * i + four, n, ws);
+            for (int i = 0; i < FN; i += kSide) {
+                __builtin_amdgcn_sched_barrier(0);  // (or the scales of all columns are fetched first, into registers that are not there)
+                float ws[kSide][16];
 #pragma unroll
-                for (int t = 0; t < 16; ++t)
-                    add[t] = 0.0f;
-                if (bias)
-                    sixteen(bias, col + kFrag * i + four, n, add);
+                for (int p = 0; p < kSide; ++p)
+                    of_columns(w_scales, col + kFrag * (i + p), n, lane, ws[p]);
 #pragma unroll
-                for (int j = 0; j < FM; ++j) {
-                    float v[16];
+                for (int j = 0; j < FM; ++j)
 #pragma unroll
-                    for (int t = 0; t < 16; ++t)
-                        v[t] = (float)acc[j][i][t] * xs[j] * ws[t] + add[t];
-                    store_block<OUT, COLUMNS>(y, ld, m, n, row + kFrag * j, col + kFrag * i, lane, v);
-                }
+                    for (int p = 0; p < kSide; ++p) {
+                        float v[16];
+#pragma unroll
+                        for (int t = 0; t < 16; ++t)
+                            v[t] = (float)acc[j][i + p][t] * xs[j] * ws[p][t];
+                        if (bias) {
+                            float add[16];
+                            of_columns(bias, col + kFrag * (i + p), n, lane, add);
+#pragma unroll
+                            for (int t = 0; t < 16; ++t)
+                                v[t] += add[t];
+                        }
+                        store_block<OUT, COLUMNS>(y, ld, m, n, row + kFrag * j, col + kFrag * (i + p), lane, v);
+                    }
             }
         }
     }
@@ -694,7 +712,9 @@ __device__ __forceinline__ void line_gemm(const LineOperands &o, int tiles_m, in
             }(), ...);
         }(std::make_integer_sequence<int, C::SLOTS>{});
     };
-    constexpr int kReadsPerSlot = (kReads + C::SLOTS - 1) / C::SLOTS;
+    // (The 256 x 256 tile's reads, but with 4-bit operands, two behind an instruction: the sooner they are made the less the next step
+    // waits for the last.  8192^3 in 8 bits 464 us with one, 459 with two; 4-bit 291 and 295.)
+    constexpr int kReadsPerSlot = !FP4 && C::SLOTS == 8 ? 2 : (kReads + C::SLOTS - 1) / C::SLOTS;
     constexpr int kLoadsPerSlot = (kLoads + C::SLOTS - 1) / C::SLOTS;
 
 #pragma unroll
