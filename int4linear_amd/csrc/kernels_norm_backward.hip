@@ -35,7 +35,8 @@ WorkParts parts(void *work, int rows, int n)
     return {(float *)work, (BackwardStatistics *)((uint8_t *)work + partial), partial + statistics};
 }
 
-// Rows of any length: a workgroup finds a row's means, reading it three times ...
+// Rows of any length: a workgroup finds a row's means, reading it three times (2000 x 40000 bf16: 200 us, 2.4 TB/s with what is read
+// twice counted once) ...
 template <int TYPE, int DY>
 __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward p, BackwardStatistics *to)
 {
@@ -89,27 +90,75 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward 
     }
 }
 
-// ... and a thread walks a column of a strip of rows.
+// ... and a wave walks 512 columns of a strip of rows, eight a lane; a workgroup's waves take every fourth row each, and their sums are
+// added in order.
+constexpr int kColumns = 64 * 8;
+
 template <int TYPE, int DY>
 __global__ __launch_bounds__(kThreads) void norm_columns_kernel(NormBackward p, const BackwardStatistics *of, float *partial, int per_strip)
 {
-    const int c = blockIdx.x * kThreads + threadIdx.x, first = blockIdx.y * per_strip, last = min(first + per_strip, p.rows);
-    if (c >= p.n)
-        return;
-    const float w = p.gamma ? p.gamma[c] : 1.0f;
-    float dgamma = 0.0f, dbeta = 0.0f;
-    for (int row = first; row < last; ++row) {
-        const BackwardStatistics s = of[row];
-        const float g = (float)((const Element<DY> *)p.dy)[(size_t)row * p.ld_dy + c];
-        const float h = s.of.normalised((float)((const Element<TYPE> *)p.x)[(size_t)row * p.ld + c] - s.of.shift);
-        dgamma = fmaf(g, h, dgamma);
-        dbeta += g;
-        if (p.dx)
-            ((Element<TYPE> *)p.dx)[(size_t)row * p.ld_dx + c] = (Element<TYPE>)(s.of.r * (g * w - s.mean_g - h * s.mean_gh));
+    using X = Element<TYPE>;
+    using D = Element<DY>;
+    constexpr int kWaves = kThreads / 64, kAhead = 2;  // rows whose values are on their way together
+    __shared__ float sums[kWaves - 1][2][kColumns];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c0 = blockIdx.x * kColumns + lane * 8;
+    const int first = blockIdx.y * per_strip, last = min(first + per_strip, p.rows);
+    float gamma[8], dgamma[8] = {}, dbeta[8] = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        gamma[e] = 1.0f;
+    if (p.gamma)
+        load8(p.gamma, c0, p.n, gamma);
+    for (int at = first + wave; at < last; at += kWaves * kAhead) {
+        Eight<X> in_x[kAhead];
+        Eight<D> in_dy[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int row = min(at + u * kWaves, last - 1);
+            fetch8((const X *)p.x + (size_t)row * p.ld, c0, p.n, in_x[u]);
+            fetch8((const D *)p.dy + (size_t)row * p.ld_dy, c0, p.n, in_dy[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int row = at + u * kWaves;
+            if (row >= last)
+                break;
+            const BackwardStatistics s = of[row];
+            const float less = -s.of.r * s.mean_g, along = -s.of.r * s.mean_gh;
+            float x[8], dy[8], out[8];
+            widen8<X>(in_x[u], c0, p.n, x);
+            widen8<D>(in_dy[u], c0, p.n, dy);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float h = s.of.normalised(x[e] - s.of.shift);
+                out[e] = fmaf(h, along, fmaf(dy[e] * gamma[e], s.of.r, less));
+                dgamma[e] = fmaf(dy[e], h, dgamma[e]);
+                dbeta[e] += dy[e];
+            }
+            if (p.dx)
+                store8((X *)p.dx + (size_t)row * p.ld_dx, c0, p.n, out);
+        }
     }
-    float *to = partial + (size_t)blockIdx.y * 2 * p.n + c;
-    to[0] = dgamma;
-    to[p.n] = dbeta;
+    if (wave > 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sums[wave - 1][0][e * 64 + lane] = dgamma[e];
+            sums[wave - 1][1][e * 64 + lane] = dbeta[e];
+        }
+    }
+    __syncthreads();
+    if (wave > 0)
+        return;
+    for (int w = 0; w < kWaves - 1; ++w)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            dgamma[e] += sums[w][0][e * 64 + lane];
+            dbeta[e] += sums[w][1][e * 64 + lane];
+        }
+    float *to = partial + (size_t)blockIdx.y * 2 * p.n;
+    store8(to, c0, p.n, dgamma);
+    store8(to + p.n, c0, p.n, dbeta);
 }
 
 // (128 registers for each of 1024 threads hold eight columns a lane, 256 for each of 512 four times as many.)
@@ -309,9 +358,9 @@ hipError_t launch(const NormBackward &p, const DeviceInfo &dev, hipStream_t stre
         else if (p.n <= 16384)
             I4L_RUN(8, 4);
         else {
-            strips = strips_of(p.rows);
+            strips = min(strips_of(p.rows), 64);
             norm_statistics_kernel<TYPE, DY><<<min(p.rows, 1 << 20), kThreads, 0, stream>>>(p, w.rows);
-            norm_columns_kernel<TYPE, DY><<<dim3((unsigned)((p.n + kThreads - 1) / kThreads), (unsigned)strips), kThreads, 0, stream>>>(
+            norm_columns_kernel<TYPE, DY><<<dim3((unsigned)((p.n + kColumns - 1) / kColumns), (unsigned)strips), kThreads, 0, stream>>>(
                 p, w.rows, w.partial, (p.rows + strips - 1) / strips);
         }
     }
