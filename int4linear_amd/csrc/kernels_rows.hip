@@ -156,13 +156,14 @@ __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t co
 }
 
 // The same with a row in registers, read once: WAVES waves share it (1: a wave has a row to itself, four rows to a workgroup), a lane
-// holds C times eight values, those of chunk i * 64 * WAVES + (its number in the group).  Workgroups stay: gamma and beta are read
-// once, and the next row's values are on their way while this one's sums are made.  (STAYS = false, for rows that leave no registers
-// for either: a row after the other.)
+// holds C times eight values, those of chunk i * 64 * WAVES + (its number in the group).  With a norm workgroups stay: gamma and beta
+// are read once, and the next row's values are on their way while this one's sums are made (16384 x 8192 bf16 145 us a row after the
+// other, so 102 us = 5.2 TB/s, what a copy of 1 GiB runs at).  Without, there is nothing to stay for (8192 x 14336 62 us = 5.7 TB/s; 71
+// where workgroups stay).
 template <int WAVES, int C>
-constexpr int waves_per_simd = C <= 2 ? 4 : C <= 4 ? 3 : 2;
+constexpr int waves_per_simd = C <= 2 ? 4 : 3;
 
-template <int TYPE, int RESULT, bool NORM, int WAVES, int C, bool STAYS>
+template <int TYPE, int RESULT, bool NORM, int WAVES, int C>
 __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd<WAVES, C>)) void row_kernel(RowPass p, size_t code_stride, size_t scale_stride)
 {
     constexpr int kAcross = WAVES * 64 * 8, kRows = WAVES == 1 ? kThreads / 64 : 1;
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
         return;
     fetch(row);
     float g[C][8], b[C][8];
-    if constexpr (NORM && STAYS)
+    if constexpr (NORM)
 #pragma unroll
         for (int i = 0; i < C; ++i)
             load_affine(p, first + i * kAcross, g[i], b[i]);
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
 #pragma unroll
         for (int i = 0; i < C; ++i)
             widen8<Element<TYPE>>(in[i], first + i * kAcross, p.n, v[i]);
-        if (NORM && STAYS && next < p.rows)
+        if (next < p.rows)
             fetch(next);
         if constexpr (NORM) {
             float sum[1] = {}, two[2] = {};
@@ -210,12 +211,8 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
             group_all<Add>(two, room[turn][1], in_row, WAVES);
             const RowStatistics s = RowStatistics::from(shift, two[0], two[1], over_n, p.eps);
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                const int c0 = first + i * kAcross;
-                if constexpr (!STAYS)
-                    load_affine(p, c0, g[0], b[0]);
-                normalise8(s, c0, p.n, g[STAYS ? i : 0], b[STAYS ? i : 0], v[i]);
-            }
+            for (int i = 0; i < C; ++i)
+                normalise8(s, first + i * kAcross, p.n, g[i], b[i], v[i]);
         }
         RowScale scale{};
         if constexpr (RESULT == kRowInt8) {
@@ -233,41 +230,46 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
         row = next;
         if (row >= p.rows)
             break;
-        if constexpr (!NORM || !STAYS)
-            fetch(row);
     }
 }
 
+// us for 1000 x 4999 f32 by waves and eights a lane: 4, 4 15.4; 8, 2 13.3; 16, 1 15.5; for 4096 x 4096 bf16 into 8 bits: 4, 2 16.6; 8, 1
+// 20.5; for 65536 x 1024 bf16: 1, 2 52.
 template <int TYPE, int RESULT, bool NORM>
 hipError_t launch(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
 {
     const size_t codes = RESULT == kRowInt8 ? int8_code_stride(p.n) : mx_code_stride(p.n), scales = mx_scale_stride(p.n);
     const int cus = dev.cu_count > 0 ? dev.cu_count : 256;
-    auto run = [&](auto waves, auto c, auto stays) {
+    auto run = [&](auto waves, auto c) {
         constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value, kRows = WAVES == 1 ? kThreads / 64 : 1;
-        constexpr bool STAYS = decltype(stays)::value;
         constexpr int kPlaces = 4 * waves_per_simd<WAVES, C> / (WAVES == 1 ? kThreads / 64 : WAVES);  // workgroups of a CU
-        // (without gamma and beta there is nothing to stay for: 8192 x 14336 63 us, and 71 where workgroups stay)
         const int groups = min((p.rows + kRows - 1) / kRows, NORM ? cus * kPlaces : 1 << 20);
-        row_kernel<TYPE, RESULT, NORM, WAVES, C, STAYS><<<groups, WAVES == 1 ? kThreads : WAVES * 64, 0, stream>>>(p, codes, scales);
+        row_kernel<TYPE, RESULT, NORM, WAVES, C><<<groups, WAVES == 1 ? kThreads : WAVES * 64, 0, stream>>>(p, codes, scales);
         return hipGetLastError();
     };
-    using std::integral_constant;
-#define I4L_RUN(WAVES, C, STAYS) run(integral_constant<int, WAVES>{}, integral_constant<int, C>{}, std::bool_constant<STAYS>{})
-    // (floats take twice the registers on their way: no more than two eights of them to a lane)
-    const bool wide = p.rows < kFewRows || TYPE == kOutF32;
+#define I4L_RUN(WAVES, C) run(std::integral_constant<int, WAVES>{}, std::integral_constant<int, C>{})
     if (p.n <= 512)
-        return I4L_RUN(1, 1, true);
+        return I4L_RUN(1, 1);
     if (p.n <= 1024)
-        return I4L_RUN(1, 2, true);
+        return I4L_RUN(1, 2);
+    const bool few = p.rows < kFewRows;
+    // (floats take twice the registers on their way: no more than two eights of them to a lane)
+    if constexpr (TYPE != kOutF32) {
+        if (!few && p.n <= 2048)
+            return I4L_RUN(1, 4);
+        if (!few && p.n > 4096 && p.n <= 8192)
+            return I4L_RUN(4, 4);
+        if (!few && p.n > 8192 && p.n <= 16384)
+            return I4L_RUN(8, 4);
+    }
     if (p.n <= 2048)
-        return wide ? I4L_RUN(4, 1, true) : I4L_RUN(1, 4, true);
+        return I4L_RUN(4, 1);
     if (p.n <= 4096)
-        return p.rows < kFewRows ? I4L_RUN(8, 1, true) : I4L_RUN(4, 2, true);
+        return few ? I4L_RUN(8, 1) : I4L_RUN(4, 2);
     if (p.n <= 8192)
-        return wide ? I4L_RUN(8, 2, true) : I4L_RUN(4, 4, true);
+        return I4L_RUN(8, 2);
     if (p.n <= 16384)
-        return wide ? I4L_RUN(16, 2, true) : I4L_RUN(8, 4, true);
+        return I4L_RUN(16, 2);
 #undef I4L_RUN
     row_loop_kernel<TYPE, RESULT, NORM><<<min(p.rows, 1 << 20), kThreads, 0, stream>>>(p, codes, scales);
     return hipGetLastError();

@@ -22,9 +22,8 @@ __device__ __forceinline__ void fetch8(const T *row, int c0, int n, Eight<T> &in
             __builtin_memcpy(&in, row + min(c0, n - 8), sizeof(in));
     } else if (c0 == 0) {
 #pragma unroll
-        for (int e = 0; e < 7; ++e)
-            if (e < n)
-                in[e] = row[e];
+        for (int e = 0; e < 8; ++e)
+            in[e] = row[min(e, n - 1)];
     }
 }
 
@@ -35,13 +34,18 @@ __device__ __forceinline__ void widen8(const Eight<T> &in, int c0, int n, float 
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         v[e] = (float)in[e];
-    if (c0 + 8 > n && n >= 8) {
-        const int over = c0 + 8 - n;  // (behind the end: zeros in any order)
+    if (c0 + 8 > n) {
+        const int over = n >= 8 ? c0 + 8 - n : 0;  // (behind the end: zeros in any order)
 #pragma unroll
         for (int by = 4; by > 0; by /= 2)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 v[e] = over & by ? (e + by < 8 ? v[e + by] : 0.0f) : v[e];
+        if (n < 8) {
+#pragma unroll
+            for (int e = 1; e < 8; ++e)
+                v[e] = e < n ? v[e] : 0.0f;
+        }
     }
 }
 

@@ -198,7 +198,8 @@ def test_quantize_of_a_view_that_is_aligned_to_its_element_only(gpu):
 LINEAR = [(1, 1, 1), (1, 100, 64), (2, 33, 257), (5, 64, 512), (16, 130, 1000), (17, 256, 256), (31, 31, 31), (32, 500, 4096), (33, 129, 515),
           (64, 96, 768), (65, 200, 300), (128, 128, 256), (129, 257, 511), (200, 300, 1024), (257, 513, 640), (300, 700, 2050), (1, 8200, 300),
           (3, 8203, 2050), (16, 8200, 1300), (20, 8192, 5000), (48, 4100, 1000), (4250, 4504, 130), (2200, 4201, 400), (2, 5, 14336), (3, 130, 700),
-          (4, 301, 1300), (4, 8195, 2050), (7, 50, 1025), (33, 8193, 515), (49, 5000, 700), (50, 8192, 300), (64, 8192, 1300), (64, 8193, 520), (64, 31, 4000)]
+          (4, 301, 1300), (4, 8195, 2050), (7, 50, 1025), (33, 8193, 515), (49, 5000, 700), (50, 8192, 300), (64, 8192, 1300), (64, 8193, 520), (64, 31, 4000), (65, 1, 1), (70, 3, 129),
+          (66, 8, 128), (129, 12, 200), (65, 8193, 130), (100, 8200, 260)]
 
 
 def product(x, w, bias=None):
