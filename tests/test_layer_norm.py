@@ -388,3 +388,41 @@ def test_a_norm_and_its_layer(gpu, m, n, k):
         step()
         torch.cuda.synchronize()
         assert all(bool(a.any()) and torch.equal(a, b) for a, b in zip(replayed, outs))
+
+
+@pytest.mark.gpu
+def test_the_example_runs_and_its_gradients(gpu):
+    import importlib.util
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location("int8_norm_linear", Path(__file__).resolve().parent.parent / "examples" / "int8_norm_linear.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    tokens, hidden, out = 96, 128, 320
+    x = torch.randn(tokens, hidden, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) * 2 + 1
+    target = example.NormLinear(tokens, hidden, out, seed=2).forward(x).float()
+    layer = example.NormLinear(tokens, hidden, out)
+    assert all(math.isfinite(v) for v in example.train(layer, x, target, 5, 0.02))
+    # gradients at the values that the quantised operands stand for
+    layer.forward(x)
+    dy = torch.randn(tokens, out, device="cuda").bfloat16()
+    dx = layer.backward(x, dy)
+    h, w, d = ref.decode(*layer.hq, hidden), ref.decode(*layer.wq, hidden), dy.double()
+    dw, dbias, dgamma, dbeta = layer.grads
+    ref.check(layer.dh, d @ w, (2.0**-8 + out * 2.0**-23) * (d.abs() @ w.abs()), "bf16")
+    ref.check(dw, d.T @ h, (2.0**-24 + 3 * tokens * 2.0**-23) * (d.abs().T @ h.abs()), "f32")
+    ref.check(dbias, d.sum(0), tokens * 2.0**-23 * d.abs().sum(0), "f32")
+    for value, (want, e) in zip((dx, dgamma, dbeta), ref.norm_gradients(layer.dh, x, layer.gamma, EPS)):
+        ref.check(value, want, e, "f32")
+    # one token at a time from a graph, eager work between the replays
+    token = x[:1].clone()
+    want = [layer.forward(x[i : i + 1].contiguous()).clone() for i in range(4)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer.forward(token)
+    for i in range(4):
+        token.copy_(x[i : i + 1])
+        graph.replay()
+        assert torch.equal(y, want[i])
+        layer.forward(x)
+        torch.cuda.synchronize()
