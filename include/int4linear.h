@@ -272,7 +272,7 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
  * A rows x k matrix is two device arrays:
  *   codes   8-bit whole numbers, row-major, 16-byte aligned, every row padded with zeros to a multiple of 128 bytes
  *           (int4linear_int8_code_bytes is the array's size, 0 for a negative one);
- *   scales  rows floats.  A value is code * scale.
+ *   scales  rows floats.  A value is code * scale, a float.
  * Rows beyond 2^30, a product's k beyond 2^17 - 1 (its sums are exact in 32 bits) and a gradient's sizes beyond 2^22 - 64 are
  * refused with INT4LINEAR_ERR_UNSUPPORTED.  Like the MXFP4 calls these are asynchronous on `stream`, allocate nothing, take no locks,
  * do not touch the library's workspace, and may be captured into a graph once the device is set up.
@@ -283,7 +283,7 @@ size_t int4linear_int8_code_bytes(int rows, int k);
  * max(max |x| / 127, 2^-100), a float, and a code the whole number nearest to x / scale, ties to the even one.  A row with an
  * infinity or a NaN becomes NaN (scale NaN, codes 0).  The padding of codes is written too. */
 int int4linear_int8_quantize(const void *x_d, int type, size_t ld, void *codes_d, float *scales_d, int rows, int k, void *stream);
-/* The way back: y_d (rows x k of `type`, `ld` >= k elements between rows). */
+/* The way back: y_d (rows x k of `type`, `ld` >= k elements between rows), values rounded to `type`. */
 int int4linear_int8_dequantize(const void *codes_d, const float *scales_d, void *y_d, int type, size_t ld, int rows, int k, void *stream);
 
 /* Y[m x n] = X[m x k] W[n x k]^T + bias: exact sums of the codes' products, (float)sum * x's scale * w's scale + bias in float, rounded

@@ -165,19 +165,21 @@ __global__ __launch_bounds__(kThreads) void norm_columns_kernel(NormBackward p, 
 template <int C>
 constexpr int most_threads = C == 1 ? 1024 : 512;
 
-// Rows that fit registers, read once.  WAVES waves share a row, C times eight columns a lane; a workgroup takes blockDim.y rows at a
-// time and stays: gamma and the columns' sums are in registers, the next rows' values on their way while these rows' sums are made.
+// Rows that fit registers, read once.  WAVES waves share a row, C times eight columns a lane (or LANES lanes of one wave, eight columns
+// each, and the wave has 64 / LANES rows); a workgroup takes a row, or a wave's, for each of its blockDim.y groups at a time and stays: gamma and the columns' sums are in registers, the next rows' values on their way while these rows' sums are made.
 // A row's four sums are made in two meetings, since g h summed over the row is r (sum of g d) + c (sum of g) with d = x - shift.  At
-// the end the groups of a workgroup add their columns' sums up in LDS, one after another.
-template <int TYPE, int DY, int WAVES, int C>
+// the end the groups' columns' sums meet in LDS and are added in the groups' order.
+template <int TYPE, int DY, int WAVES, int C, int LANES>
 __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBackward p, float *partial)
 {
     constexpr int kAcross = WAVES * 64 * 8;
-    extern __shared__ float columns[];  // n, where there is more than one group
+    extern __shared__ float columns[];  // n for each group, where there is more than one (32 KiB at most)
     __shared__ float rooms[2][most_threads<C> / 64 * 5];
     using X = Element<TYPE>;
     using D = Element<DY>;
-    const int group = threadIdx.y, groups = blockDim.y, first = threadIdx.x * 8;
+    static_assert(LANES == 64 || (WAVES == 1 && C == 1));
+    constexpr int kRows = 64 / LANES;  // of a group
+    const int group = threadIdx.y, groups = blockDim.y, first = (LANES < 64 ? threadIdx.x % LANES : threadIdx.x) * 8;
     const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float over_n = 1.0f / (float)p.n;
     Eight<X> in_x[C];
@@ -202,13 +204,13 @@ __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBack
         if (p.gamma)
             load8(p.gamma, first + i * kAcross, p.n, gamma[i]);
     }
-    const int by = gridDim.x * groups;
-    int row = blockIdx.x * groups + group;
+    const int by = gridDim.x * groups * kRows;
+    int row = (blockIdx.x * groups + group) * kRows + (LANES < 64 ? (int)threadIdx.x / LANES : 0);
     if (row < p.rows)
         fetch(row);
     // (every group makes as many turns, for their meetings; one without a row has zeros)
     int turn = 0;
-    for (int base = blockIdx.x * groups; base < p.rows; base += by, row += by, turn ^= 1) {
+    for (int base = blockIdx.x * groups * kRows; base < p.rows; base += by, row += by, turn ^= 1) {
         float x[C][8], dy[C][8];
         const bool there = row < p.rows;
 #pragma unroll
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBack
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 sum[0] += x[i][e];
-        group_all<Add>(sum, room, wave, WAVES);
+        group_all<Add, LANES>(sum, room, wave, WAVES);
         const float shift = row_shift(sum[0], over_n);
 #pragma unroll
         for (int i = 0; i < C; ++i) {
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBack
                 four[3] = fmaf(g, x[i][e], four[3]);
             }
         }
-        group_all<Add>(four, room + WAVES, wave, WAVES);
+        group_all<Add, LANES>(four, room + WAVES, wave, WAVES);
         const RowStatistics s = RowStatistics::from(shift, four[0], four[1], over_n, p.eps);
         const float mean_g = four[2] * over_n, mean_gh = fmaf(s.r, four[3], s.c * four[2]) * over_n;
         const float less = -s.r * mean_g, along = -s.r * mean_gh;
@@ -272,37 +274,41 @@ __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBack
     }
     if (!partial)
         return;
-    auto add_groups = [&](float(&sums)[C][8]) {
-        for (int turn = groups - 1; turn >= 0; --turn) {
-            __syncthreads();
-            if (group != turn)
-                continue;
+    if constexpr (LANES < 64) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            dgamma[0][e] = across_all<LANES>(dgamma[0][e], Add{});
+            dbeta[0][e] = across_all<LANES>(dbeta[0][e], Add{});
+        }
+    }
+    float *to = partial + (size_t)blockIdx.x * 2 * p.n;
+    if (groups == 1) {
+        if (LANES == 64 || threadIdx.x < LANES) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                store8(to, first + i * kAcross, p.n, dgamma[i]);
+                store8(to + p.n, first + i * kAcross, p.n, dbeta[i]);
+            }
+        }
+        return;
+    }
+    auto add_groups = [&](const float(&sums)[C][8], float *result) {
+        if (LANES == 64 || threadIdx.x < LANES) {
 #pragma unroll
             for (int i = 0; i < C; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int c = first + i * kAcross + e;
-                    if (c >= p.n)
-                        continue;
-                    if (turn < groups - 1)
-                        sums[i][e] += columns[c];
-                    if (turn > 0)
-                        columns[c] = sums[i][e];
-                }
+                store8(columns + (size_t)group * p.n, first + i * kAcross, p.n, sums[i]);
         }
+        __syncthreads();
+        for (int c = group * WAVES * 64 + threadIdx.x; c < p.n; c += groups * WAVES * 64) {
+            float sum = columns[c];
+            for (int g = 1; g < groups; ++g)
+                sum += columns[g * p.n + c];
+            result[c] = sum;
+        }
+        __syncthreads();
     };
-    if (groups > 1) {
-        add_groups(dgamma);
-        add_groups(dbeta);
-    }
-    if (group == 0) {
-        float *to = partial + (size_t)blockIdx.x * 2 * p.n;
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            store8(to, first + i * kAcross, p.n, dgamma[i]);
-            store8(to + p.n, first + i * kAcross, p.n, dbeta[i]);
-        }
-    }
+    add_groups(dgamma, to);
+    add_groups(dbeta, to + p.n);
 }
 
 // dgamma and dbeta from the strips' sums: 64 columns to a workgroup, a wave to every sixteenth strip; the waves' sums in their order.
@@ -336,16 +342,24 @@ hipError_t launch(const NormBackward &p, const DeviceInfo &dev, hipStream_t stre
     const WorkParts w = parts(p.work, p.rows, p.n);
     const int cus = min(dev.cu_count > 0 ? dev.cu_count : kStrips, kStrips);
     int strips = 0;
-    auto run = [&](auto waves, auto c) {
-        constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value;
-        const int groups = min((p.rows + cus - 1) / cus, most_threads<C> / 64 / WAVES);
-        strips = min((p.rows + groups - 1) / groups, cus);
-        norm_backward_kernel<TYPE, DY, WAVES, C><<<strips, dim3(WAVES * 64, (unsigned)groups), groups > 1 ? p.n * sizeof(float) : 0, stream>>>(
+    auto run = [&](auto waves, auto c, auto lanes) {
+        constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value, LANES = decltype(lanes)::value, kRows = 64 / LANES;
+        const int waves_of_rows = (p.rows + kRows - 1) / kRows;
+        const int groups = min((waves_of_rows + cus - 1) / cus, most_threads<C> / 64 / WAVES);
+        strips = min((waves_of_rows + groups - 1) / groups, cus);
+        norm_backward_kernel<TYPE, DY, WAVES, C, LANES><<<strips, dim3(WAVES * 64, (unsigned)groups), groups > 1 ? groups * p.n * sizeof(float) : 0, stream>>>(
             p, p.dgamma || p.dbeta ? w.partial : nullptr);
     };
-#define I4L_RUN(WAVES, C) run(std::integral_constant<int, WAVES>{}, std::integral_constant<int, C>{})
+#define I4L_LANES(WAVES, C, LANES) run(std::integral_constant<int, WAVES>{}, std::integral_constant<int, C>{}, std::integral_constant<int, LANES>{})
+#define I4L_RUN(WAVES, C) I4L_LANES(WAVES, C, 64)
     if (p.rows > 0) {
-        if (p.n <= 512)
+        if (p.n <= 64)
+            I4L_LANES(1, 1, 8);
+        else if (p.n <= 128)
+            I4L_LANES(1, 1, 16);
+        else if (p.n <= 256)
+            I4L_LANES(1, 1, 32);
+        else if (p.n <= 512)
             I4L_RUN(1, 1);
         else if (p.n <= 1024)
             I4L_RUN(2, 1);
@@ -365,6 +379,7 @@ hipError_t launch(const NormBackward &p, const DeviceInfo &dev, hipStream_t stre
         }
     }
 #undef I4L_RUN
+#undef I4L_LANES
     if (p.dgamma || p.dbeta)
         norm_sums_kernel<<<(2 * p.n + 63) / 64, 1024, 0, stream>>>(w.partial, strips, p.n, p.dgamma, p.dbeta);
     return hipGetLastError();

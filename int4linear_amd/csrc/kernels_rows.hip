@@ -155,21 +155,22 @@ __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t co
     }
 }
 
-// The same with a row in registers, read once: WAVES waves share it (1: a wave has a row to itself, four rows to a workgroup), a lane
-// holds C times eight values, those of chunk i * 64 * WAVES + (its number in the group).  With a norm workgroups stay: gamma and beta
+// The same with a row in registers, read once: WAVES waves share it (1: LANES lanes of a wave have a row to themselves, a workgroup four
+// rows or more), a lane holds C times eight values, those of chunk i * 64 * WAVES + (its number in the group).  With a norm workgroups stay: gamma and beta
 // are read once, and the next row's values are on their way while this one's sums are made (16384 x 8192 bf16 145 us a row after the
 // other, so 102 us = 5.2 TB/s, what a copy of 1 GiB runs at).  Without, there is nothing to stay for (8192 x 14336 62 us = 5.7 TB/s; 71
 // where workgroups stay).
 template <int WAVES, int C>
 constexpr int waves_per_simd = C <= 2 ? 4 : 3;
 
-template <int TYPE, int RESULT, bool NORM, int WAVES, int C>
+template <int TYPE, int RESULT, bool NORM, int WAVES, int C, int LANES>
 __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd<WAVES, C>)) void row_kernel(RowPass p, size_t code_stride, size_t scale_stride)
 {
-    constexpr int kAcross = WAVES * 64 * 8, kRows = WAVES == 1 ? kThreads / 64 : 1;
+    static_assert(LANES == 64 || (WAVES == 1 && C == 1));
+    constexpr int kAcross = WAVES * 64 * 8, kRows = WAVES == 1 ? kThreads / LANES : 1;
     __shared__ float room[2][3][2 * WAVES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int in_row = WAVES == 1 ? 0 : wave, first = (WAVES == 1 ? threadIdx.x & 63 : threadIdx.x) * 8;
+    const int in_row = WAVES == 1 ? 0 : wave, first = (WAVES == 1 ? threadIdx.x % LANES : threadIdx.x) * 8;
     const RowWriter<RESULT> writer{p, code_stride, scale_stride};
     const float over_n = 1.0f / (float)p.n;
     Eight<Element<TYPE>> in[C];
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
         for (int i = 0; i < C; ++i)
             fetch8(x, first + i * kAcross, p.n, in[i]);
     };
-    int row = blockIdx.x * kRows + (WAVES == 1 ? wave : 0), turn = 0;
+    int row = blockIdx.x * kRows + (LANES < 64 ? (int)threadIdx.x / LANES : WAVES == 1 ? wave : 0), turn = 0;
     if (row >= p.rows)
         return;
     fetch(row);
@@ -203,12 +204,12 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     sum[0] += v[i][e];
-            group_all<Add>(sum, room[turn][0], in_row, WAVES);
+            group_all<Add, LANES>(sum, room[turn][0], in_row, WAVES);
             const float shift = row_shift(sum[0], over_n);
 #pragma unroll
             for (int i = 0; i < C; ++i)
                 centre8(shift, first + i * kAcross, p.n, v[i], two);
-            group_all<Add>(two, room[turn][1], in_row, WAVES);
+            group_all<Add, LANES>(two, room[turn][1], in_row, WAVES);
             const RowStatistics s = RowStatistics::from(shift, two[0], two[1], over_n, p.eps);
 #pragma unroll
             for (int i = 0; i < C; ++i)
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd
 #pragma unroll
             for (int i = 0; i < C; ++i)
                 largest8(v[i], big[0]);
-            group_all<Larger>(big, (unsigned *)room[turn][2], in_row, WAVES);
+            group_all<Larger, LANES>(big, (unsigned *)room[turn][2], in_row, WAVES);
             scale = RowScale::of(big[0]);
         }
 #pragma unroll
@@ -240,14 +241,26 @@ hipError_t launch(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
 {
     const size_t codes = RESULT == kRowInt8 ? int8_code_stride(p.n) : mx_code_stride(p.n), scales = mx_scale_stride(p.n);
     const int cus = dev.cu_count > 0 ? dev.cu_count : 256;
-    auto run = [&](auto waves, auto c) {
-        constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value, kRows = WAVES == 1 ? kThreads / 64 : 1;
+    auto run = [&](auto waves, auto c, auto lanes) {
+        constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value, LANES = decltype(lanes)::value, kRows = WAVES == 1 ? kThreads / LANES : 1;
         constexpr int kPlaces = 4 * waves_per_simd<WAVES, C> / (WAVES == 1 ? kThreads / 64 : WAVES);  // workgroups of a CU
         const int groups = min((p.rows + kRows - 1) / kRows, NORM ? cus * kPlaces : 1 << 20);
-        row_kernel<TYPE, RESULT, NORM, WAVES, C><<<groups, WAVES == 1 ? kThreads : WAVES * 64, 0, stream>>>(p, codes, scales);
+        row_kernel<TYPE, RESULT, NORM, WAVES, C, LANES><<<groups, WAVES == 1 ? kThreads : WAVES * 64, 0, stream>>>(p, codes, scales);
         return hipGetLastError();
     };
-#define I4L_RUN(WAVES, C) run(std::integral_constant<int, WAVES>{}, std::integral_constant<int, C>{})
+#define I4L_LANES(WAVES, C, LANES) run(std::integral_constant<int, WAVES>{}, std::integral_constant<int, C>{}, std::integral_constant<int, LANES>{})
+#define I4L_RUN(WAVES, C) I4L_LANES(WAVES, C, 64)
+    // Rows of a head's size: several to a wave, with lanes for the padding of 8-bit codes (that of MXFP4 reaches 512 columns).
+    if constexpr (RESULT == kRowTyped) {
+        if (p.n <= 64)
+            return I4L_LANES(1, 1, 8);
+    }
+    if constexpr (RESULT != kRowMx) {
+        if (p.n <= 128)
+            return I4L_LANES(1, 1, 16);
+        if (p.n <= 256)
+            return I4L_LANES(1, 1, 32);
+    }
     if (p.n <= 512)
         return I4L_RUN(1, 1);
     if (p.n <= 1024)
@@ -271,6 +284,7 @@ hipError_t launch(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
     if (p.n <= 16384)
         return I4L_RUN(16, 2);
 #undef I4L_RUN
+#undef I4L_LANES
     row_loop_kernel<TYPE, RESULT, NORM><<<min(p.rows, 1 << 20), kThreads, 0, stream>>>(p, codes, scales);
     return hipGetLastError();
 }
@@ -297,8 +311,10 @@ __global__ __launch_bounds__(kThreads) void int8_dequantize_kernel(Int8Matrix q,
         const float s = q.scales[row];
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 8; ++e) {
             v[e] = (float)(int8_t)(codes[e / 4] >> 8 * (e % 4)) * s;
+            asm("" : "+v"(v[e]));  // (a value is a float; in sight, the product would be rounded to float16 without that step)
+        }
         store8(y + row * ld, c0, k, v);
     }
 }

@@ -104,9 +104,9 @@ __device__ __forceinline__ void store8_as(int out, void *row, int c0, int n, con
         store8((__bf16 *)row, c0, n, v);
 }
 
-// Every lane's value combined with all others of the wave, the same bits in all of them: neighbours, pairs, quads and eights by
-// lane permutations, rows of 16 and halves of the wave by swaps.
-template <class T, class Op>
+// Every lane's value combined with those of the others of its LANES lanes (8, 16, 32 or the whole wave), the same bits in all of
+// them: neighbours, pairs, quads and eights by lane permutations, rows of 16 and halves of the wave by swaps.
+template <int LANES = 64, class T, class Op>
 __device__ __forceinline__ T wave_all(T v, Op op)
 {
     auto permuted = [](T x, auto ctrl) {
@@ -115,13 +115,38 @@ __device__ __forceinline__ T wave_all(T v, Op op)
     v = op(v, permuted(v, std::integral_constant<int, 0xB1>{}));   // lanes 1 0 3 2
     v = op(v, permuted(v, std::integral_constant<int, 0x4E>{}));   // lanes 2 3 0 1
     v = op(v, permuted(v, std::integral_constant<int, 0x141>{}));  // 7 .. 0
-    v = op(v, permuted(v, std::integral_constant<int, 0x140>{}));  // 15 .. 0
-    const unsigned a = __builtin_bit_cast(unsigned, v);
-    const auto rows = __builtin_amdgcn_permlane16_swap(a, a, false, false);
-    v = op(__builtin_bit_cast(T, (unsigned)rows[0]), __builtin_bit_cast(T, (unsigned)rows[1]));
-    const unsigned b = __builtin_bit_cast(unsigned, v);
-    const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return op(__builtin_bit_cast(T, (unsigned)halves[0]), __builtin_bit_cast(T, (unsigned)halves[1]));
+    if constexpr (LANES >= 16)
+        v = op(v, permuted(v, std::integral_constant<int, 0x140>{}));  // 15 .. 0
+    if constexpr (LANES >= 32) {
+        const unsigned a = __builtin_bit_cast(unsigned, v);
+        const auto rows = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+        v = op(__builtin_bit_cast(T, (unsigned)rows[0]), __builtin_bit_cast(T, (unsigned)rows[1]));
+    }
+    if constexpr (LANES == 64) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+        v = op(__builtin_bit_cast(T, (unsigned)halves[0]), __builtin_bit_cast(T, (unsigned)halves[1]));
+    }
+    return v;
+}
+
+// What lanes LANES apart hold, combined over the wave: the rest of wave_all.
+template <int LANES, class T, class Op>
+__device__ __forceinline__ T across_all(T v, Op op)
+{
+    if constexpr (LANES == 8)
+        v = op(v, __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xF, 0xF, true)));  // a row turned by 8
+    if constexpr (LANES <= 16) {
+        const unsigned a = __builtin_bit_cast(unsigned, v);
+        const auto rows = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+        v = op(__builtin_bit_cast(T, (unsigned)rows[0]), __builtin_bit_cast(T, (unsigned)rows[1]));
+    }
+    if constexpr (LANES <= 32) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        const auto halves = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+        v = op(__builtin_bit_cast(T, (unsigned)halves[0]), __builtin_bit_cast(T, (unsigned)halves[1]));
+    }
+    return v;
 }
 
 struct Add {
@@ -132,13 +157,13 @@ struct Larger {
 };
 
 // N values of every thread combined over the `waves` waves of a group, which all meet here.  `room` (N * waves words of LDS) may be
-// used again once the group has met for another time.
-template <class Op, class T, int N>
+// used again once the group has met for another time.  With one wave, over LANES of its lanes.
+template <class Op, int LANES = 64, class T, int N>
 __device__ __forceinline__ void group_all(T (&v)[N], T *room, int wave, int waves)
 {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-        v[i] = wave_all(v[i], Op{});
+        v[i] = wave_all<LANES>(v[i], Op{});
     if (waves == 1)
         return;
     if ((threadIdx.x & 63) == 0) {

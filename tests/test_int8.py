@@ -116,7 +116,7 @@ def matrix(seed, rows, k, scale=1.0):
     return (codes.cuda(), scales.cuda()), ref.decode(codes, scales, k)
 
 
-ROWS = [(1, 1, 1), (1, 31, 31), (2, 32, 40), (3, 33, 33), (5, 127, 128), (4, 128, 128), (7, 513, 515), (3, 1024, 1024), (6, 2049, 2060), (33, 1000, 1001),
+ROWS = [(1, 1, 1), (1, 31, 31), (300, 64, 64), (77, 129, 130), (50, 256, 256), (2, 32, 40), (3, 33, 33), (5, 127, 128), (4, 128, 128), (7, 513, 515), (3, 1024, 1024), (6, 2049, 2060), (33, 1000, 1001),
         (16, 4096, 4096), (130, 777, 784), (5, 8200, 8200), (3, 16384, 16384), (2, 32800, 32801), (2, 70001, 70001)]
 
 

@@ -108,7 +108,7 @@ def vectors(seed, n):
 
 
 #: rows, n: one lane's values, whole and ragged waves, rows of one wave, of several, of every number of eights a thread holds, and longer ones
-SIZES = [(1, 1), (3, 2), (2, 7), (5, 8), (4, 63), (7, 64), (9, 500), (3, 512), (6, 513), (5, 1000), (4, 1024), (3, 1030), (130, 777), (3, 2048), (2, 2050),
+SIZES = [(1, 1), (3, 2), (2, 7), (5, 8), (4, 63), (7, 64), (9, 500), (33, 65), (1000, 40), (70, 128), (19, 129), (5000, 3), (41, 200), (9, 256), (5, 257), (3, 512), (6, 513), (5, 1000), (4, 1024), (3, 1030), (130, 777), (3, 2048), (2, 2050),
          (16, 4096), (5, 4999), (3, 8192), (2, 8193), (2, 16384), (3, 16385), (2, 32768), (2, 32770), (3, 100001)]
 
 
@@ -223,7 +223,7 @@ def test_quantised_norms_are_the_norm_quantised(gpu, rows, n, kind):
 
 
 BACKWARD = [(1, 1), (2, 7), (3, 64), (17, 500), (5, 513), (257, 1000), (130, 2050), (64, 4096), (300, 4999), (19, 8193), (9, 16384), (6, 16390), (5, 32768),
-            (4, 40001), (1500, 72), (5000, 33), (1030, 1030)]
+            (4, 40001), (1500, 72), (5000, 33), (1030, 1030), (20000, 64), (7, 100), (3001, 128), (4500, 250), (100, 256), (5, 257)]
 
 
 @pytest.mark.gpu
