@@ -207,11 +207,11 @@ __device__ __forceinline__ void store_transposed(const v4u (&rows)[8], uint16_t 
 }
 
 template <int DOWN>
-__device__ __forceinline__ void transpose_int8(const Transposed &t, int k)
+__device__ __forceinline__ void transpose_int8(const Transposed &t, int k, int down, int across)
 {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r0 = (blockIdx.x * DOWN + wave / kTilesAcross) * kTile, c0 = (blockIdx.y * kTilesAcross + wave % kTilesAcross) * kTile;
+    const int r0 = (down * DOWN + wave / kTilesAcross) * kTile, c0 = (across * kTilesAcross + wave % kTilesAcross) * kTile;
     if (r0 >= t.of.q.rows || c0 >= k)
         return;
     const int row = r0 + (lane & 7) * 8, col = c0 + (lane >> 3) * 8;
@@ -253,11 +253,11 @@ __device__ __forceinline__ void transpose_int8(const Transposed &t, int k)
 }
 
 template <int DOWN>
-__device__ __forceinline__ void transpose_matrix(const Transposed &t, int k, size_t code_stride, size_t scale_stride)
+__device__ __forceinline__ void transpose_matrix(const Transposed &t, int k, size_t code_stride, size_t scale_stride, int down, int across)
 {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r0 = (blockIdx.x * DOWN + wave / kTilesAcross) * kTile, c0 = (blockIdx.y * kTilesAcross + wave % kTilesAcross) * kTile;
+    const int r0 = (down * DOWN + wave / kTilesAcross) * kTile, c0 = (across * kTilesAcross + wave % kTilesAcross) * kTile;
     if (r0 >= t.of.q.rows || c0 >= k)
         return;
     const int row = r0 + (lane & 7) * 8, col = c0 + (lane >> 3) * 8;
@@ -291,11 +291,11 @@ __device__ __forceinline__ float lanes(float v)
 }
 
 template <int DOWN>
-__device__ __forceinline__ void transpose_dy(const Prepared &p)
+__device__ __forceinline__ void transpose_dy(const Prepared &p, int down, int across)
 {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r0 = (blockIdx.x * DOWN + wave / kTilesAcross) * kTile, c0 = (blockIdx.y * kTilesAcross + wave % kTilesAcross) * kTile;
+    const int r0 = (down * DOWN + wave / kTilesAcross) * kTile, c0 = (across * kTilesAcross + wave % kTilesAcross) * kTile;
     if (r0 >= p.rows || c0 >= p.cols)
         return;
     const int row = r0 + (lane & 7) * 8, col = c0 + (lane >> 3) * 8;
@@ -353,20 +353,36 @@ __device__ __forceinline__ void transpose_dy(const Prepared &p)
     }
 }
 
-// blockIdx.z: one of the matrices, or dy behind them.  A workgroup takes DOWN x kTilesAcross tiles.
+// A workgroup takes DOWN x kTilesAcross tiles of one of the matrices, or of dy behind them: the first of each of these has number
+// first[i], and down[i] of them lie one below the other.  (A grid that is as long and as wide as the longest and the widest of them is mostly
+// empty workgroups where these differ.  Gradients of an 8-bit layer, us: 445 x 16320 x 2816 250, so 193; 64 x 8192 x 1024 57, 37; small ones
+// pay 0.4 for their number, 130 x 1001 x 515 14.1, 14.5.)
+struct PrepareGrid {
+    unsigned first[4], down[4], inverse[4];  // (first: of those that are not there, the number behind the last)
+    // inverse: the whole part of 2^32 / down, or the largest number: a quotient by it is the true one or one less
+};
+
 template <int DOWN, bool INT8>
-__global__ __launch_bounds__(DOWN *kTilesAcross * 64) void prepare_kernel(Prepared p, size_t code_stride, size_t scale_stride)
+__global__ __launch_bounds__(DOWN *kTilesAcross * 64) void prepare_kernel(Prepared p, PrepareGrid grid, size_t code_stride, size_t scale_stride)
 {
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+    if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < p.zero_count; i += DOWN * kTilesAcross * 64)
             p.zeros[i] = 0;
-    if ((int)blockIdx.z < p.matrices)
+    int which = 0;
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+        which += blockIdx.x >= grid.first[i];
+    const unsigned mine = blockIdx.x - grid.first[which], its_down = grid.down[which];
+    unsigned quotient = __umulhi(mine, grid.inverse[which]);
+    quotient += mine - quotient * its_down >= its_down;
+    const int across = (int)quotient, down = (int)(mine - quotient * its_down);
+    if (which < p.matrices)
         if constexpr (INT8)
-            transpose_int8<DOWN>(p.matrix[blockIdx.z], p.k);
+            transpose_int8<DOWN>(p.matrix[which], p.k, down, across);
         else
-            transpose_matrix<DOWN>(p.matrix[blockIdx.z], p.k, code_stride, scale_stride);
+            transpose_matrix<DOWN>(p.matrix[which], p.k, code_stride, scale_stride, down, across);
     else
-        transpose_dy<DOWN>(p);
+        transpose_dy<DOWN>(p, down, across);
 }
 
 // 64 columns per workgroup; the waves take every fourth row each, and their sums are added in order.
@@ -456,13 +472,24 @@ hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
     }
     if (rows == 0 || cols == 0)
         return hipSuccess;
-    auto run = [&](auto down) {
-        constexpr int DOWN = decltype(down)::value, kSide = DOWN * kTile, kWide = kTilesAcross * kTile;
-        const dim3 grid((unsigned)((rows + kSide - 1) / kSide), (unsigned)((cols + kWide - 1) / kWide), (unsigned)(p.matrices + (p.dy != nullptr)));
+    auto run = [&](auto tiles) {
+        constexpr int DOWN = decltype(tiles)::value, kSide = DOWN * kTile, kWide = kTilesAcross * kTile;
+        PrepareGrid grid{};
+        unsigned count = 0;
+        for (int i = 0; i < 4; ++i) {
+            grid.first[i] = count;
+            const bool is_dy = i == p.matrices && p.dy;
+            if (i < p.matrices || is_dy) {
+                const int its_rows = is_dy ? p.rows : p.matrix[i].of.q.rows, its_cols = is_dy ? p.cols : p.k;
+                grid.down[i] = (unsigned)((its_rows + kSide - 1) / kSide);
+                grid.inverse[i] = grid.down[i] > 1 ? (unsigned)((1ull << 32) / grid.down[i]) : ~0u;
+                count += grid.down[i] * (unsigned)((its_cols + kWide - 1) / kWide);
+            }
+        }
         if (p.int8)
-            prepare_kernel<DOWN, true><<<grid, DOWN * kTilesAcross * 64, 0, stream>>>(p, 0, 0);
+            prepare_kernel<DOWN, true><<<count, DOWN * kTilesAcross * 64, 0, stream>>>(p, grid, 0, 0);
         else
-            prepare_kernel<DOWN, false><<<grid, DOWN * kTilesAcross * 64, 0, stream>>>(p, mx_code_stride(p.k), mx_scale_stride(p.k));
+            prepare_kernel<DOWN, false><<<count, DOWN * kTilesAcross * 64, 0, stream>>>(p, grid, mx_code_stride(p.k), mx_scale_stride(p.k));
     };
     if ((long)rows * cols >= kLargeTranspose)
         run(std::integral_constant<int, 4>{});
