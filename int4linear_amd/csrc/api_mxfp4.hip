@@ -195,11 +195,12 @@ int int4linear_mxfp4_gated_backward(const void *dh_d, const void *x_codes_d, con
     if (e == hipSuccess)
         e = launch_prepare(prepared, stream);
     const Bf16Product products[] = {
-        {p.d_t, n, p.x_t, k, p.ld_m, m, want_dw ? dwg_d : nullptr, dw_type},
-        {p.d_t + (size_t)n * p.ld_m, n, p.x_t, k, p.ld_m, m, want_dw ? dwu_d : nullptr, dw_type},
-        {p.d, m, p.w_t, k, 2 * p.ld_n, (int)(n > 0 ? 2 * p.ld_n : 0), want_dx ? dx_d : nullptr, kOutBF16}};
+        {p.d_t, n, p.x_t, k, p.ld_m, m, want_dw ? dwg_d : nullptr, dw_type, m},
+        {p.d_t + (size_t)n * p.ld_m, n, p.x_t, k, p.ld_m, m, want_dw ? dwu_d : nullptr, dw_type, m},
+        {p.d, m, p.w_t, k, 2 * p.ld_n, (int)(n > 0 ? 2 * p.ld_n : 0), want_dx ? dx_d : nullptr, kOutBF16,
+         (int)(n > 0 ? 2 * p.ld_n : 0)}};
     if (e == hipSuccess)
-        e = launch_bf16_products(products, 3, ColumnSums{}, p.slices, info, stream);
+        e = launch_bf16_products(products, 3, false, ColumnSums{}, p.slices, info, stream);
     return api_status(e);
 }
 

@@ -1160,8 +1160,28 @@ constexpr int kMostTogether = 1536;
 // How long a slice of k is at least, in stages: meeting costs as much as about six.
 constexpr int kLeastSlice = 6;
 
-hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const SliceSpace &space, const DeviceInfo &dev,
-                                hipStream_t stream)
+// One product in slices of its sum, whose tile-slices have the numbers from `first` on.
+static hipError_t launch_sliced(const Bf16Product &p, int slices, int first, const SliceSpace &space, hipStream_t stream)
+{
+    LineGroup g{};
+    g.count = 2;  // (the last of a group has 16-bit results: one without tiles)
+    g.slices[1] = 1;
+    g.o[0] = operands(p);
+    g.y[0] = p.y;
+    g.tiles_m[0] = (p.m + 63) / 64;
+    g.tiles_n[0] = (p.n + 63) / 64;
+    g.slices[0] = slices;
+    g.first[0] = first;
+    g.partial = space.partial;
+    g.arrivals = space.arrivals;
+    if (p.out == kOutF32)
+        return launch_group(g, epilogue<kOutF32, true>(p), epilogue<kOutBF16, true>(p), stream);
+    return p.n % 8 ? launch_group(g, epilogue<kOutBF16, true>(p), epilogue<kOutBF16, true>(p), stream)
+                   : launch_group(g, epilogue<kOutBF16, false>(p), epilogue<kOutBF16, false>(p), stream);
+}
+
+hipError_t launch_bf16_products(const Bf16Product *p, int count, bool slices_alone, const ColumnSums &sums, const SliceSpace &space,
+                                const DeviceInfo &dev, hipStream_t stream)
 {
     // Together up to three rounds of tiles of 64 x 64 (us apart and together: 257 x 1400 x 1000, gated, 784 tiles 39, 32.6; 700 x 2000 x 1000, gated,
     // 1200 tiles 53.2, 52.5; 1600 x 2048 x 1536, linear, 1368 tiles 50.4, 46.1; 1000 x 2000 x 2000, linear, 1536 tiles 42.7, 43.7; 2048^3, 2048 tiles
@@ -1175,10 +1195,17 @@ hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSum
         together = together && p[i].k > 0 && p[i].n == p[0].n && (i == count - 1 || p[i].out == p[0].out);
     }
     if (!together || tiles > kMostTogether) {
+        // (Of one that has few tiles and long sums, the slices: 128 x 14336 x 4096 121 us, so 116.)
         hipError_t e = hipSuccess;
-        for (int i = 0; i < count && e == hipSuccess; ++i)
+        long used = 0;
+        for (int i = 0; i < count && e == hipSuccess; ++i) {
+            const int stages = (p[i].terms + kLineBf16 - 1) / kLineBf16;
+            const int slices = slices_alone ? quicker_slices(p[i].m, p[i].n, stages, kMostSlices - used, kLeastSlice, dev.cu_count) : 1;
             if (p[i].y)
-                e = launch_bf16(p[i], dev, stream);
+                e = slices > 1 ? launch_sliced(p[i], slices, (int)used, space, stream) : launch_bf16(p[i], dev, stream);
+            if (slices > 1)
+                used += slices * ((p[i].m + 63l) / 64) * ((p[i].n + 63l) / 64);
+        }
         return e == hipSuccess && sums.sums ? launch_column_sums(sums, stream) : e;
     }
     LineGroup g{};
@@ -1189,17 +1216,13 @@ hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSum
         g.tiles_m[i] = (p[i].m + 63) / 64;
         g.tiles_n[i] = (p[i].n + 63) / 64;
     }
-    int total = 0;
-    for (int least = kLeastSlice;; least += least / 4) {
-        total = 0;
-        for (int i = 0; i < count; ++i) {
-            g.slices[i] = min(max(g.o[i].stages / least, 1), 16);
-            g.first[i] = total;
-            total += g.tiles_m[i] * g.tiles_n[i] * g.slices[i];
-        }
-        if (total <= kMostSlices || total == tiles)
-            break;
+    int stages[3], tiles_of[3];
+    for (int i = 0; i < count; ++i) {
+        stages[i] = (p[i].terms + kLineBf16 - 1) / kLineBf16;
+        tiles_of[i] = g.tiles_m[i] * g.tiles_n[i];
     }
+    group_slices(count, tiles_of, stages, kLeastSlice, kMostSlices, slices_alone, (long)max(1, dev.cu_count) * per_cu<Tile64, false>, g.slices,
+                 g.first);
     bool any = false;
     for (int i = 0; i < count; ++i) {
         any = any || p[i].y;

@@ -26,28 +26,85 @@ constexpr int line_tiles_per_cu(const LineTileCost &t, bool fp4) { return 160 * 
 // and bfloat16 ones:
 //   1030 x 1990 x 2000   57, 29.3, 23.0, 22.8        1280 x 2048 x 4096   84, 40.9, 36.6, 37.1
 //   2048 x 2816 x 4096   92, 51.0, 58.9, 79.8        4096^3               116, 124, 160, 202
-inline int quickest_tile(bool fp4, long m, long n, int stages, bool pair, int cu_count)
+inline double line_tile_cost(const LineTileCost &t, int per_cu, long tiles, int stages, long cus)
+{
+    const long places = cus * per_cu, rounds = tiles / places, rest = tiles % places;
+    double stage = (double)rounds * per_cu * t.full;
+    if (rest) {
+        const double shared = (double)rest / cus * t.full;
+        stage += shared > t.few ? shared : t.few;
+    }
+    return stage * stages + t.fixed;
+}
+
+inline int quickest_tile(bool fp4, long m, long n, int stages, bool pair, int cu_count, double *its_cost = nullptr)
 {
     const long cus = cu_count > 0 ? cu_count : 256;
     int best = 0;
     double least = 0;
     for (int i = 0; i < 3 + !pair; ++i) {
         const LineTileCost &t = kLineTiles[i];
-        const int per_cu = line_tiles_per_cu(t, fp4);
         const long tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
-        const long places = cus * per_cu, rounds = tiles / places, rest = tiles % places;
-        double stage = (double)rounds * per_cu * t.full;
-        if (rest) {
-            const double shared = (double)rest / cus * t.full;
-            stage += shared > t.few ? shared : t.few;
-        }
-        const double cost = stage * stages + t.fixed;
+        const double cost = line_tile_cost(t, line_tiles_per_cu(t, fp4), tiles, stages, cus);
         if (i == 0 || cost < least) {
             best = i;
             least = cost;
         }
     }
+    if (its_cost)
+        *its_cost = least;
     return best;
+}
+
+// Slices of k that make a product of bfloat16 operands on 64 x 64 tiles quicker than the quickest tile does unsliced, by the same
+// costs; 1: none do.  At most `room` tile-slices; a slice is `least` stages long at least, and meeting costs as much as that.
+inline int quicker_slices(long m, long n, int stages, long room, int least, int cu_count)
+{
+    const long cus = cu_count > 0 ? cu_count : 256, tiles = ((m + 63) / 64) * ((n + 63) / 64);
+    const LineTileCost &t = kLineTiles[3];
+    double cost;
+    quickest_tile(false, m, n, stages, false, cu_count, &cost);
+    int best = 1;
+    for (int slices = 2; slices <= 16 && slices * tiles <= room && slices * least <= stages; ++slices) {
+        const double sliced = line_tile_cost(t, line_tiles_per_cu(t, false), tiles * slices, (stages + slices - 1) / slices + least, cus);
+        if (sliced < cost) {
+            cost = sliced;
+            best = slices;
+        }
+    }
+    return best;
+}
+
+// Slices of the products of one launch on 64 x 64 tiles, as short as `room` tile-slices allow but of `least` stages at least, and the
+// number of each product's first tile-slice.  If that leaves all of them whole, with `long_alone` those are sliced whose sums are
+// twice as long and more as what the device's `places` have on average. (us: 8192 x 512 x 512 73, so 61; with slices for ever longer sums, 1000 x 2000 x 2000 45, 50.)
+inline void group_slices(int count, const int *tiles, const int *stages, int least, int room, bool long_alone, long places, int *slices,
+                         int *first)
+{
+    long work = 0;
+    for (int i = 0; i < count; ++i)
+        work += (long)tiles[i] * stages[i];
+    bool only = false;
+    for (int shortest = least;;) {
+        int total = 0;
+        bool any = false;
+        for (int i = 0; i < count; ++i) {
+            const int most = only && stages[i] * places < 2 * work ? 1 : stages[i] / shortest;
+            slices[i] = most < 1 ? 1 : most > 16 ? 16 : most;
+            first[i] = total;
+            any = any || slices[i] > 1;
+            if (slices[i] > 1 || !only)  // (one slice has no one to meet)
+                total += tiles[i] * slices[i];
+        }
+        if (any ? total <= room : only || !long_alone)
+            return;
+        if (!any) {
+            only = true;
+            shortest = least;
+        } else {
+            shortest += shortest / 4;
+        }
+    }
 }
 
 }  // namespace int4linear

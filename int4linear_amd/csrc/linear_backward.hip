@@ -101,11 +101,11 @@ int linear_backward(const void *dy, const BackwardOperand &x, const BackwardOper
     }
     hipError_t e = launch_prepare(prepared, stream);
     const Bf16Product products[] = {
-        {p.dy_t, n, p.x_t, k, ld_sum, pieces > 1 && m > 0 ? (int)ld_sum : m, want_dw ? dw : nullptr, dw_type},
-        {ragged ? p.dy_padded : (const uint16_t *)dy, m, p.w_t, k, p.ld_n, n, want_dx ? dx : nullptr, kOutBF16}};
+        {p.dy_t, n, p.x_t, k, ld_sum, pieces > 1 && m > 0 ? (int)ld_sum : m, want_dw ? dw : nullptr, dw_type, m},
+        {ragged ? p.dy_padded : (const uint16_t *)dy, m, p.w_t, k, p.ld_n, n, want_dx ? dx : nullptr, kOutBF16, n}};
     const ColumnSums sums{want_sums ? dbias : nullptr, p.sums, (int)(p.ld_m / 64), n};
     if (e == hipSuccess)
-        e = launch_bf16_products(products, 2, sums, p.slices, info, stream);
+        e = launch_bf16_products(products, 2, int8, sums, p.slices, info, stream);
     return api_status(e);
 }
 

@@ -111,16 +111,19 @@ struct Bf16Product {
     int k;
     void *y;
     int out;
+    int terms;  // by which slices are chosen: k, but not three times as many where k holds a float's pieces, since the slices of the
+                // other products would depend on the type of this one, and with them their last bits
 };
-// Up to three of them, and the column sums.  Small ones are cut into slices of k, whose sums meet in `space`.  One whose
-// y is null is not wanted; results do not depend on which are.
+// Up to three of them, and the column sums.  Small ones are cut into slices of k, whose sums meet in `space`; with
+// `slices_alone` also one with a long sum that leaves the device idle beside the others, in one launch or
+// by itself.  One whose y is null is not wanted; results do not depend on which are.
 constexpr int kMostSlices = 1024;  // tiles of 64 x 64, times the slices of each
 struct SliceSpace {
     float *partial;      // kMostSlices * 64 * 64
     unsigned *arrivals;  // kMostSlices * 4, zeros
 };
-hipError_t launch_bf16_products(const Bf16Product *p, int count, const ColumnSums &sums, const SliceSpace &space, const DeviceInfo &dev,
-                                hipStream_t stream);
+hipError_t launch_bf16_products(const Bf16Product *p, int count, bool slices_alone, const ColumnSums &sums, const SliceSpace &space,
+                                const DeviceInfo &dev, hipStream_t stream);
 
 // Between the files of the C ABI (api.hip): the current device's record, set up for work on `stream`, and a
 // HIP error as the status of a call.  Both return an INT4LINEAR_* status.

@@ -283,6 +283,21 @@ def test_linear_backward(gpu, m, n, k, dw_type):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(1000, 1000, 1000), (1000, 2000, 1990), (200, 5000, 4000), (4000, 300, 500)])
+def test_input_gradients_do_not_depend_on_the_weights(gpu, m, n, k):
+    """dx has the same bits beside dw in either type and without it."""
+    (xq, _), (wq, _) = matrix(m, m, k), matrix(n, n, k, 1.0 / math.sqrt(k))
+    dy = torch.randn(m, n, generator=torch.Generator().manual_seed(m * n)).bfloat16().cuda()
+    results = []
+    for dw_type in ("bf16", "f32", None):
+        dw = torch.empty(n, k, dtype=ref.DTYPE[dw_type], device="cuda") if dw_type else None
+        work = torch.empty(lib.int8_linear_backward_bytes(m, n, k, dw_type or "bf16"), dtype=torch.uint8, device="cuda")
+        results.append(torch.empty(m, k, dtype=torch.bfloat16, device="cuda"))
+        lib.int8_linear_backward(dy, *xq, *wq, results[-1], dw, dw_type or "bf16", None, work, m, n, k)
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+
+
+@pytest.mark.gpu
 def test_gradients_as_floats_keep_the_values_bits(gpu):
     """One token with dy = 1: dw is X itself as a float, to the last bit."""
     k = 300
