@@ -98,7 +98,7 @@ hipError_t set_up_device(PerDevice &pd, int dev)
 }
 
 // Set-up for the device that is current on the calling thread; returns its record.  Set-up
-// queries the device, raises the dynamic-LDS limit of some 450 kernels and takes the address
+// queries the device, raises the dynamic-LDS limit of several hundred kernels and takes the address
 // of the scratch arrays (which loads the device image): none of that belongs inside a graph
 // capture, so a first call that arrives with `work_stream` capturing is refused
 // (`for_work`: the call is about to enqueue work on work_stream).

@@ -156,15 +156,15 @@ __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t co
 }
 
 // The same with a row in registers, read once: WAVES waves share it (1: LANES lanes of a wave have a row to themselves, a workgroup four
-// rows or more), a lane holds C times eight values, those of chunk i * 64 * WAVES + (its number in the group).  With a norm workgroups stay: gamma and beta
-// are read once, and the next row's values are on their way while this one's sums are made (16384 x 8192 bf16 145 us a row after the
-// other, so 102 us = 5.2 TB/s, what a copy of 1 GiB runs at).  Without, there is nothing to stay for (8192 x 14336 62 us = 5.7 TB/s; 71
-// where workgroups stay).
-template <int WAVES, int C>
+// rows or more), a lane holds C times eight values, those of chunk i * 64 * WAVES + (its number in the group).  With a norm workgroups
+// stay: gamma and beta are read once, and the next row's values are on their way while this one's sums are made (16384 x 8192 bf16
+// 145 us a row after the other, so 102 us = 5.2 TB/s, what a copy of 1 GiB runs at).  Without, there is nothing to stay for (8192 x
+// 14336 into 8 bits 62 us = 5.7 TB/s; 71 where workgroups stay).
+template <int C>
 constexpr int waves_per_simd = C <= 2 ? 4 : 3;
 
 template <int TYPE, int RESULT, bool NORM, int WAVES, int C, int LANES>
-__global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, (waves_per_simd<WAVES, C>)) void row_kernel(RowPass p, size_t code_stride, size_t scale_stride)
+__global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, waves_per_simd<C>) void row_kernel(RowPass p, size_t code_stride, size_t scale_stride)
 {
     static_assert(LANES == 64 || (WAVES == 1 && C == 1));
     constexpr int kAcross = WAVES * 64 * 8, kRows = WAVES == 1 ? kThreads / LANES : 1;
@@ -243,7 +243,7 @@ hipError_t launch(const RowPass &p, const DeviceInfo &dev, hipStream_t stream)
     const int cus = dev.cu_count > 0 ? dev.cu_count : 256;
     auto run = [&](auto waves, auto c, auto lanes) {
         constexpr int WAVES = decltype(waves)::value, C = decltype(c)::value, LANES = decltype(lanes)::value, kRows = WAVES == 1 ? kThreads / LANES : 1;
-        constexpr int kPlaces = 4 * waves_per_simd<WAVES, C> / (WAVES == 1 ? kThreads / 64 : WAVES);  // workgroups of a CU
+        constexpr int kPlaces = 4 * waves_per_simd<C> / (WAVES == 1 ? kThreads / 64 : WAVES);  // workgroups of a CU
         const int groups = min((p.rows + kRows - 1) / kRows, NORM ? cus * kPlaces : 1 << 20);
         row_kernel<TYPE, RESULT, NORM, WAVES, C, LANES><<<groups, WAVES == 1 ? kThreads : WAVES * 64, 0, stream>>>(p, codes, scales);
         return hipGetLastError();
