@@ -928,6 +928,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_group_kernel(LineGrou
 
 using Tile256 = LineTile<4, 2, 2, 4, 0, 2, 1, 2>;
 using Tile128 = LineTile<2, 2, 2, 2, 4, 2, 1, 4>;
+using Tile128Deep = LineTile<2, 2, 2, 2, 4, 4, 2, 2>;
 using Tile64x128 = LineTile<2, 2, 1, 2, 4, 3, 2, 4>;
 using Tile64 = LineTile<2, 2, 1, 1, 4, 4, 2, 4>;  // (too narrow for pairs of blocks)
 
@@ -952,12 +953,21 @@ constexpr bool described_by(const LineTileCost &t)
 }
 static_assert(described_by<Tile256>(kLineTiles[0]) && described_by<Tile128>(kLineTiles[1]) && described_by<Tile64x128>(kLineTiles[2]) &&
               described_by<Tile64>(kLineTiles[3]));
+static_assert(Tile128Deep::BM == kDeepTileCost.m && Tile128Deep::BN == kDeepTileCost.n && Tile128Deep::LDS<false> == kDeepTileCost.lds[0]);
 
 // n: columns of the product that have to be covered.
 template <int VALUES, class Ep>
 hipError_t launch(const LineOperands &o, int n, const Ep &ep, const DeviceInfo &dev, hipStream_t stream)
 {
-    switch (quickest_tile(VALUES == kFp4Values, o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev.cu_count)) {
+    int which;
+    if constexpr (VALUES == kFp4Values) {
+        which = quickest_tile(true, o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev.cu_count);
+    } else {
+        which = quickest_tile_without_scales(o.a_rows, n, o.stages, dev.cu_count);
+        if (which == kDeepTile)
+            return launch_tile<VALUES, Tile128Deep>(o, n, ep, dev, stream);
+    }
+    switch (which) {
     case 0:
         return launch_tile<VALUES, Tile256>(o, n, ep, dev, stream);
     case 1:
@@ -1016,6 +1026,8 @@ static hipError_t allow_lds()
     allow(Tile256{});
     allow(Tile128{});
     allow(Tile64x128{});
+    if constexpr (VALUES != kFp4Values)
+        allow(Tile128Deep{});
     if constexpr (!Ep::kPair)
         allow(Tile64{});
     return e;

@@ -56,6 +56,27 @@ inline int quickest_tile(bool fp4, long m, long n, int stages, bool pair, int cu
     return best;
 }
 
+// Operands without scales also go in tiles of 128 x 128 that have a CU to themselves and twice the stages on their way, where there are no
+// more of them than CUs (kDeepTile; else quickest_tile's).  us without it and with it, weights from HBM, 8-bit operands: 333 x 10880 x 4999 40.6,
+// 30.9; 256 x 11008 x 4999 42.8, 32.3; 1024 x 4096 x 4096 25.6, 19.8; 130 x 16384 x 2048 16.0, 12.6; 2048^3 15.3, 12.4; of bfloat16 ones, the
+// gradients of 2048^3 59.5, 49.2.
+constexpr LineTileCost kDeepTileCost = {128, 128, {131072, 0}, 46, 46, 740};
+constexpr int kDeepTile = 4;
+inline int quickest_tile_without_scales(long m, long n, int stages, int cu_count, double *its_cost = nullptr)
+{
+    const long cus = cu_count > 0 ? cu_count : 256, tiles = ((m + 127) / 128) * ((n + 127) / 128);
+    double cost;
+    int best = quickest_tile(false, m, n, stages, false, cu_count, &cost);
+    const double deep = line_tile_cost(kDeepTileCost, 1, tiles, stages, cus);
+    if (tiles <= cus && deep < cost) {
+        best = kDeepTile;
+        cost = deep;
+    }
+    if (its_cost)
+        *its_cost = cost;
+    return best;
+}
+
 // Slices of k that make a product of bfloat16 operands on 64 x 64 tiles quicker than the quickest tile does unsliced, by the same
 // costs; 1: none do.  At most `room` tile-slices; a slice is `least` stages long at least, and meeting costs as much as that.
 inline int quicker_slices(long m, long n, int stages, long room, int least, int cu_count)
@@ -63,7 +84,7 @@ inline int quicker_slices(long m, long n, int stages, long room, int least, int 
     const long cus = cu_count > 0 ? cu_count : 256, tiles = ((m + 63) / 64) * ((n + 63) / 64);
     const LineTileCost &t = kLineTiles[3];
     double cost;
-    quickest_tile(false, m, n, stages, false, cu_count, &cost);
+    quickest_tile_without_scales(m, n, stages, cu_count, &cost);
     int best = 1;
     for (int slices = 2; slices <= 16 && slices * tiles <= room && slices * least <= stages; ++slices) {
         const double sliced = line_tile_cost(t, line_tiles_per_cu(t, false), tiles * slices, (stages + slices - 1) / slices + least, cus);
