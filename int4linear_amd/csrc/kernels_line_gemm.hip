@@ -159,7 +159,7 @@ struct LineEpilogue {
     template <int FM, int FN>
     __device__ __forceinline__ void operator()(v16f (&acc)[FM][FN], int row, int col, int lane) const
     {
-        constexpr int kSide = FN > 2 ? 2 : 1;
+        constexpr int kSide = FN > 2 && FN % 2 == 0 ? 2 : 1;
 #pragma unroll
         for (int i = 0; i < FN; i += kSide)
 #pragma unroll
@@ -237,7 +237,7 @@ struct Int8Epilogue {
         } else {
             // (Two blocks side by side are a line of 16-bit results: its halves leave one after the other, where there are registers for it.  With a column of blocks after
             // the other 8192 x 8192 x 2048 takes 155 us, so 151.)
-            constexpr int kSide = FN > 2 ? 2 : 1;
+            constexpr int kSide = FN > 2 && FN % 2 == 0 ? 2 : 1;
             float xs[FM];
 #pragma unroll
             for (int j = 0; j < FM; ++j)
@@ -929,6 +929,9 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void line_group_kernel(LineGrou
 using Tile256 = LineTile<4, 2, 2, 4, 0, 2, 1, 2>;
 using Tile128 = LineTile<2, 2, 2, 2, 4, 2, 1, 4>;
 using Tile128Deep = LineTile<2, 2, 2, 2, 4, 4, 2, 2>;
+using Tile192x128 = LineTile<2, 2, 3, 2, 4, 3, 2, 2>;
+using Tile128x192 = LineTile<2, 2, 2, 3, 4, 3, 2, 2>;
+using Tile192 = LineTile<2, 2, 3, 3, 4, 3, 1, 2>;
 using Tile64x128 = LineTile<2, 2, 1, 2, 4, 3, 2, 4>;
 using Tile64 = LineTile<2, 2, 1, 1, 4, 4, 2, 4>;  // (too narrow for pairs of blocks)
 
@@ -953,7 +956,13 @@ constexpr bool described_by(const LineTileCost &t)
 }
 static_assert(described_by<Tile256>(kLineTiles[0]) && described_by<Tile128>(kLineTiles[1]) && described_by<Tile64x128>(kLineTiles[2]) &&
               described_by<Tile64>(kLineTiles[3]));
-static_assert(Tile128Deep::BM == kDeepTileCost.m && Tile128Deep::BN == kDeepTileCost.n && Tile128Deep::LDS<false> == kDeepTileCost.lds[0]);
+template <class C>
+constexpr bool deep_as(const LineTileCost &t)
+{
+    return t.m == C::BM && t.n == C::BN && t.lds[0] == C::template LDS<false>;
+}
+static_assert(deep_as<Tile128Deep>(kDeepTileCosts[0]) && deep_as<Tile192x128>(kDeepTileCosts[1]) && deep_as<Tile128x192>(kDeepTileCosts[2]) &&
+              deep_as<Tile192>(kDeepTileCosts[3]));
 
 // n: columns of the product that have to be covered.
 template <int VALUES, class Ep>
@@ -964,8 +973,16 @@ hipError_t launch(const LineOperands &o, int n, const Ep &ep, const DeviceInfo &
         which = quickest_tile(true, o.a_rows, (long)n * (Ep::kPair ? 2 : 1), o.stages, Ep::kPair, dev.cu_count);
     } else {
         which = quickest_tile_without_scales(o.a_rows, n, o.stages, dev.cu_count);
-        if (which == kDeepTile)
+        switch (which - kDeepTiles) {
+        case 0:
             return launch_tile<VALUES, Tile128Deep>(o, n, ep, dev, stream);
+        case 1:
+            return launch_tile<VALUES, Tile192x128>(o, n, ep, dev, stream);
+        case 2:
+            return launch_tile<VALUES, Tile128x192>(o, n, ep, dev, stream);
+        case 3:
+            return launch_tile<VALUES, Tile192>(o, n, ep, dev, stream);
+        }
     }
     switch (which) {
     case 0:
@@ -1026,8 +1043,12 @@ static hipError_t allow_lds()
     allow(Tile256{});
     allow(Tile128{});
     allow(Tile64x128{});
-    if constexpr (VALUES != kFp4Values)
+    if constexpr (VALUES != kFp4Values) {
         allow(Tile128Deep{});
+        allow(Tile192x128{});
+        allow(Tile128x192{});
+        allow(Tile192{});
+    }
     if constexpr (!Ep::kPair)
         allow(Tile64{});
     return e;

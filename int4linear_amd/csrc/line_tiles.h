@@ -56,21 +56,32 @@ inline int quickest_tile(bool fp4, long m, long n, int stages, bool pair, int cu
     return best;
 }
 
-// Operands without scales also go in tiles of 128 x 128 that have a CU to themselves and twice the stages on their way, where there are no
-// more of them than CUs (kDeepTile; else quickest_tile's).  us without it and with it, weights from HBM, 8-bit operands: 333 x 10880 x 4999 40.6,
-// 30.9; 256 x 11008 x 4999 42.8, 32.3; 1024 x 4096 x 4096 25.6, 19.8; 130 x 16384 x 2048 16.0, 12.6; 2048^3 15.3, 12.4; of bfloat16 ones, the
-// gradients of 2048^3 59.5, 49.2.
-constexpr LineTileCost kDeepTileCost = {128, 128, {131072, 0}, 46, 46, 740};
-constexpr int kDeepTile = 4;
+// Operands without scales also go in tiles that have a CU to themselves and more bytes on their way, where there are no more of
+// them than CUs: numbers kDeepTiles and up.  us without them and with them, weights from HBM, 8-bit operands:
+//   128 x 128   256 x 11008 x 4999 42.8, 32.3; 1024 x 4096 x 4096 25.6, 19.6; 130 x 16384 x 2048 16.0, 12.1; 2048^3 15.3, 12.2
+//   192 x 128   333 x 11008 x 4999 41.4, 35.1; 384 x 11008 x 4096 34.3, 27.7; 333 x 14336 x 2048 21.8, 15.8
+//   128 x 192   512 x 11008 x 4096 43.0, 30.9; 1024 x 5120 x 5120 39.5, 31.7
+//   192 x 192   3000 x 2900 x 4000 48.6, 39.8; 2048 x 4096 x 4096 39.0, 36.0; 2700^3 29.1, 29.5
+// and the gradients, with bfloat16 ones, of 2048^3 59.7, 49.3; 3000^3 152, 122.  Where there are few of them, smaller tiles bring more CUs'
+// loads: 512 x 4096 x 11008 42.7 on 64 x 128, 53.2 on 128 x 128 of this kind; 200 x 4096 x 14336 31.3 on 64 x 64, 57.4.
+constexpr int kDeepTiles = 4;
+constexpr LineTileCost kDeepTileCosts[] = {{128, 128, {131072, 0}, 46, 46, 740},
+                                           {192, 128, {122880, 0}, 58, 58, 950},
+                                           {128, 192, {122880, 0}, 58, 58, 950},
+                                           {192, 192, {147456, 0}, 85, 85, 1050}};
 inline int quickest_tile_without_scales(long m, long n, int stages, int cu_count, double *its_cost = nullptr)
 {
-    const long cus = cu_count > 0 ? cu_count : 256, tiles = ((m + 127) / 128) * ((n + 127) / 128);
+    const long cus = cu_count > 0 ? cu_count : 256;
     double cost;
     int best = quickest_tile(false, m, n, stages, false, cu_count, &cost);
-    const double deep = line_tile_cost(kDeepTileCost, 1, tiles, stages, cus);
-    if (tiles <= cus && deep < cost) {
-        best = kDeepTile;
-        cost = deep;
+    for (int i = 0; i < 4; ++i) {
+        const LineTileCost &t = kDeepTileCosts[i];
+        const long tiles = ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n);
+        const double deep = line_tile_cost(t, 1, tiles, stages, cus);
+        if (tiles <= cus && deep < cost) {
+            best = kDeepTiles + i;
+            cost = deep;
+        }
     }
     if (its_cost)
         *its_cost = cost;

@@ -200,7 +200,8 @@ LINEAR = [(1, 1, 1), (1, 100, 64), (2, 33, 257), (5, 64, 512), (16, 130, 1000), 
           (3, 8203, 2050), (16, 8200, 1300), (20, 8192, 5000), (48, 4100, 1000), (4250, 4504, 130), (2200, 4201, 400), (2, 5, 14336), (3, 130, 700),
           (4, 301, 1300), (4, 8195, 2050), (7, 50, 1025), (33, 8193, 515), (49, 5000, 700), (50, 8192, 300), (64, 8192, 1300), (64, 8193, 520), (64, 31, 4000), (65, 1, 1), (70, 3, 129),
           (66, 8, 128), (129, 12, 200), (65, 8193, 130), (100, 8200, 260),
-          (900, 3904, 2100), (897, 3901, 2050)]
+          (900, 3904, 2100), (897, 3901, 2050), (330, 14336, 2100), (331, 14330, 2100),
+          (500, 11008, 2100), (510, 10950, 2050), (2800, 2880, 2700), (2700, 2890, 2701)]
 
 
 def product(x, w, bias=None):
@@ -252,7 +253,7 @@ def test_linear_without_k_and_without_rows(gpu):
 
 
 BACKWARD = [(1, 1, 1), (2, 33, 65), (5, 7, 300), (16, 130, 1000), (64, 64, 64), (65, 129, 257), (130, 1001, 515), (300, 200, 333), (70, 900, 520),
-            (1000, 2000, 1990), (2816, 2050, 2800), (2000, 2040, 1904), (1990, 2033, 1901)]
+            (1000, 2000, 1990), (2816, 2050, 2800), (2000, 2040, 1904), (1990, 2033, 1901), (2800, 2760, 2808)]
 
 
 @pytest.mark.gpu

@@ -1,6 +1,6 @@
 """The rules by which products of a backward pass are cut into slices of their sums, compiled for the host from the library's own header:
 tile-slices never exceed the room that a workspace has, and slices are no shorter than they may be.  And the rule by which products of
-operands without scales take the tile with the most stages on their way."""
+operands without scales take a tile that has a CU to itself."""
 import ctypes
 import subprocess
 
@@ -12,7 +12,7 @@ SOURCE = """
 #include "line_tiles.h"
 using namespace int4linear;
 extern "C" int alone(long m, long n, int stages, long room, int least, int cus) { return quicker_slices(m, n, stages, room, least, cus); }
-extern "C" int deep(long m, long n, int stages, int cus) { return quickest_tile_without_scales(m, n, stages, cus) == kDeepTile; }
+extern "C" int tile(long m, long n, int stages, int cus) { return quickest_tile_without_scales(m, n, stages, cus); }
 extern "C" void group(int count, const int *tiles, const int *stages, int least, int room, int alone, int *slices, int *first)
 {
     group_slices(count, tiles, stages, least, room, alone, 512, slices, first);
@@ -28,7 +28,7 @@ def rules(tmp_path_factory):
     (tmp / "rule.cpp").write_text(SOURCE)
     subprocess.run(["g++", "-std=c++20", "-O1", "-shared", "-fPIC", f"-I{CSRC}", str(tmp / "rule.cpp"), "-o", str(tmp / "rule.so")], check=True)
     lib = ctypes.CDLL(str(tmp / "rule.so"))
-    lib.deep.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_int]
+    lib.tile.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_int]
     lib.alone.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_long, ctypes.c_int, ctypes.c_int]
     return lib
 
@@ -81,13 +81,25 @@ def test_a_long_sum_beside_short_ones(rules, m, n, k, want):
     assert slices[0] > 1 or not want
 
 
-def test_tiles_with_the_most_stages(rules):
+#: tiles that have a CU to themselves, from number 4 on
+DEEP = ((128, 128), (192, 128), (128, 192), (192, 192))
+
+
+def test_tiles_with_the_most_bytes_on_their_way(rules):
     for m in SIZES:
         for n in SIZES:
             for stages in (1, 8, 40, 200):
-                if rules.deep(m, n, stages, 256):
-                    assert -(-m // 128) * -(-n // 128) <= 256
-    # one to a CU, long enough a sum; not two rounds of them, nor few of them
-    assert rules.deep(333, 10880, 40, 256) and rules.deep(900, 3900, 17, 256) and rules.deep(2048, 2048, 32, 256)
-    assert not rules.deep(333, 11008, 40, 256) and not rules.deep(1100, 3500, 8, 256) and not rules.deep(128, 1024, 40, 256)
-    assert not rules.deep(900, 3900, 17, 200)
+                which = rules.tile(m, n, stages, 256)
+                if which >= 4:
+                    assert -(-m // DEEP[which - 4][0]) * -(-n // DEEP[which - 4][1]) <= 256
+
+
+@pytest.mark.parametrize("m, n, stages, want", [(333, 10880, 40, 4), (900, 3904, 17, 4), (333, 11008, 40, 5), (330, 14336, 17, 5), (331, 14330, 17, 5),
+                                                   (512, 11008, 32, 6), (500, 11008, 17, 6), (3000, 2900, 32, 7), (2800, 2880, 22, 7)])
+def test_one_tile_to_a_cu(rules, m, n, stages, want):
+    assert rules.tile(m, n, stages, 256) == want
+
+
+@pytest.mark.parametrize("m, n, stages", [(1100, 3500, 8), (128, 1024, 40), (2048, 3000, 8), (8192, 8192, 64), (200, 4096, 112), (512, 4096, 86)])
+def test_other_tiles(rules, m, n, stages):
+    assert rules.tile(m, n, stages, 256) < 4
