@@ -307,8 +307,9 @@ int int4linear_int8_linear_backward(const void *dy_d, const void *x_codes_d, con
  * The norm in front of such layers: y = (x - mean) / sqrt(variance + eps) * gamma + beta, mean and variance (of all n, not n - 1)
  * over a row.  (The reference has no counterpart.)  x_d is rows x n of `type`, `ld` >= n elements between rows, aligned to its element;
  * gamma_d and beta_d are n floats each or NULL (1 and 0); eps >= 0 and finite, else INT4LINEAR_ERR_UNSUPPORTED, as are more than 2^30
- * rows and n beyond 2^22.  Sums and statistics are held in float: a row whose squares (of x - mean) add up to more
- * than a float holds gives beta.  A row with an infinity or a NaN becomes NaN, and so does one without variance where eps is 0.
+ * rows and n beyond 2^22.  Sums and statistics are held in float: a row of finite values whose squares (of x - mean) add up to more
+ * than a float holds gives beta, a dx of 0 and nothing for dgamma.  A row with an infinity or a NaN becomes NaN, and so does one without
+ * variance where eps is 0.
  *   int4linear_layer_norm        y_d is rows x n of out_type, ld_y >= n elements between rows, aligned to its element; it may be x_d
  *                                where types and distances of rows are the same;
  *   int4linear_layer_norm_int8   y in 8 bits, quantised from its float value: the operand of int4linear_int8_linear;

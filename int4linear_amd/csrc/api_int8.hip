@@ -13,8 +13,6 @@ using namespace int4linear;
 
 // Sums of products of 8-bit numbers: k * 128 * 128 is below 2^31.
 constexpr int kMostSummands = (1 << 17) - 1;
-// Sums over a row are those of at most as many floats.
-constexpr int kMostNorm = 1 << 22;
 
 Int8Matrix matrix(const void *codes, const float *scales, int rows) { return {(const int8_t *)codes, scales, rows}; }
 

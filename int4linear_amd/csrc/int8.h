@@ -33,6 +33,9 @@ hipError_t launch_int8_skinny(const Int8Matrix &x, const Int8Matrix &w, const fl
 // y (rows x k of `type`, ld elements between rows) = what q stands for.
 hipError_t launch_int8_dequantize(const Int8Matrix &q, void *y, int type, size_t ld, int k, hipStream_t stream);
 
+// The longest row of a norm: sums over it are those of at most as many floats.
+constexpr int kMostNorm = 1 << 22;
+
 // One pass over rows of x (rows x n of `type`, an OutKind other than kOutS32; ld elements between rows): as they are, or
 // normalised, (x - mean) / sqrt(variance + eps) * gamma + beta (gamma and beta: n floats or null), into one of three forms.
 enum RowResult : int { kRowTyped, kRowInt8, kRowMx };

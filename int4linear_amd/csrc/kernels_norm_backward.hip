@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward 
             load8(x, c0, p.n, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                sum[0] += v[e];
+                add_part(sum[0], v[e]);
         }
         group_all<Add>(sum, room[0], wave, kWaves);
         const float shift = row_shift(sum[0], over_n);
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(NormBackward 
                 const float a = p.gamma ? g[e] * w[e] : g[e];
                 if (c0 + e < p.n) {
                     means[0] += a;
-                    means[1] = fmaf(a, s.normalised(v[e] - shift), means[1]);
+                    means[1] = fmaf(a, s.of(v[e]), means[1]);
                 }
             }
         }
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void norm_columns_kernel(NormBackward p, 
             widen8<D>(in_dy[u], c0, p.n, dy);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float h = s.of.normalised(x[e] - s.of.shift);
+                const float h = s.of.of(x[e]);
                 out[e] = fmaf(h, along, fmaf(dy[e] * gamma[e], s.of.r, less));
                 dgamma[e] = fmaf(dy[e], h, dgamma[e]);
                 dbeta[e] += dy[e];
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBack
         for (int i = 0; i < C; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                sum[0] += x[i][e];
+                add_part(sum[0], x[i][e]);
         group_all<Add, LANES>(sum, room, wave, WAVES);
         const float shift = row_shift(sum[0], over_n);
 #pragma unroll
@@ -258,6 +258,14 @@ __global__ __launch_bounds__(most_threads<C>) void norm_backward_kernel(NormBack
         }
         group_all<Add, LANES>(four, room + WAVES, wave, WAVES);
         const RowStatistics s = RowStatistics::from(shift, four[0], four[1], over_n, p.eps);
+        if (s.flat) {  // rare
+            four[3] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[i][e] = 0.0f;
+        }
         const float mean_g = four[2] * over_n, mean_gh = fmaf(s.r, four[3], s.c * four[2]) * over_n;
         const float less = -s.r * mean_g, along = -s.r * mean_gh;
         X *dx = (X *)p.dx + (size_t)row * p.ld_dx;

@@ -118,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t co
                     load_affine(p, c0, g, b);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        v[e] -= s.shift;
+                        v[e] = s.flat ? 0.0f : v[e] - s.shift;
                     normalise8(s, c0, p.n, g, b, v);
                 }
                 f(c0, v);
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t co
                 load8(x, c0, p.n, v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    sum[0] += v[e];
+                    add_part(sum[0], v[e]);
             }
             group_all<Add>(sum, room[0], wave, kWaves);
             const float shift = row_shift(sum[0], over_n);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, waves_per_simd<
             for (int i = 0; i < C; ++i)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    sum[0] += v[i][e];
+                    add_part(sum[0], v[i][e]);
             group_all<Add, LANES>(sum, room[turn][0], in_row, WAVES);
             const float shift = row_shift(sum[0], over_n);
 #pragma unroll
@@ -211,6 +211,13 @@ __global__ __launch_bounds__(WAVES == 1 ? kThreads : WAVES * 64, waves_per_simd<
                 centre8(shift, first + i * kAcross, p.n, v[i], two);
             group_all<Add, LANES>(two, room[turn][1], in_row, WAVES);
             const RowStatistics s = RowStatistics::from(shift, two[0], two[1], over_n, p.eps);
+            if (s.flat) {  // rare
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        v[i][e] = 0.0f;
+            }
 #pragma unroll
             for (int i = 0; i < C; ++i)
                 normalise8(s, first + i * kAcross, p.n, g[i], b[i], v[i]);

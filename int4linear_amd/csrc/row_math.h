@@ -181,29 +181,40 @@ __device__ __forceinline__ void group_all(T (&v)[N], T *room, int wave, int wave
     }
 }
 
-// What all values of a row are centred on.  It has to be one number: left in sight, the product would be merged with some of the
-// differences that take it and not with others, and so be rounded for these alone.
+// A row's sum as one of small parts of its values: that of as many as a row may have is a float, whatever finite floats they are, so that a
+// row whose sum is none has an infinity or a NaN.  (A power of two: the same bits as a sum of the values themselves.)
+constexpr float kPart = 0x1p-23f;
+static_assert(kMostNorm <= 1 << 22);
+__device__ __forceinline__ void add_part(float &sum, float v) { sum = fmaf(v, kPart, sum); }
+
+// What all values of a row are centred on, from the sum of their parts.  It has to be one number: left in sight, the product would be merged
+// with some of the differences that take it and not with others, and so be rounded for these alone.
 __device__ __forceinline__ float row_shift(float sum, float over_n)
 {
-    float shift = sum * over_n;
+    float shift = sum * (over_n * (1.0f / kPart));
     asm("" : "+v"(shift));
     return shift;
 }
 
 // A row's mean is `shift` + delta with shift a first sum's (rounded) mean, so that what is squared and summed next is centred: the
 // variance is the mean of (x - shift)^2 less delta^2, a correction of the first sum's rounding and no cancellation.
-// h = (x - mean) / sqrt(variance + eps) is d r + c with d = x - shift, one rounding.
+// h = (x - mean) / sqrt(variance + eps) is d r + c with d = x - shift, one rounding.  In a `flat` row h is 0, and d has to be: some of its d
+// may be infinite.
 struct RowStatistics {
     float shift, r, c;
+    bool flat;
     __device__ static RowStatistics from(float shift, float sum, float squares, float over_n, float eps)
     {
-        const float delta = sum * over_n;
-        const float variance = fmaxf(squares * over_n - delta * delta, 0.0f);
-        // (fmaxf takes a NaN away: rows with infinities or NaNs become NaN)
+        // Finite values that lie too far apart have an infinite sum of squares.  With an infinity or a NaN among them it is a NaN: shift is one
+        // too, or the same infinity, and so is what is left of that value.
+        const bool flat = squares == __builtin_inff();
+        const float delta = flat ? 0.0f : sum * over_n;
+        const float variance = fmaxf(fmaf(squares, over_n, -(delta * delta)), 0.0f);
         const float r = rsqrtf((squares == squares ? variance : squares) + eps);
-        return {shift, r, -delta * r};
+        return {shift, r, -delta * r, flat};
     }
     __device__ __forceinline__ float normalised(float d) const { return fmaf(d, r, c); }
+    __device__ __forceinline__ float of(float x) const { return normalised(flat ? 0.0f : x - shift); }
 };
 
 // The 8-bit format's scale of a row whose largest magnitude has the bits `big` (NaN above infinity above all numbers), and what

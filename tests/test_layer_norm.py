@@ -426,3 +426,62 @@ def test_the_example_runs_and_its_gradients(gpu):
         assert torch.equal(y, want[i])
         layer.forward(x)
         torch.cuda.synchronize()
+
+
+# ---- rows of very large values
+
+
+def work_of(rows, n):
+    return torch.empty(lib.layer_norm_backward_bytes(rows, n), dtype=torch.uint8, device="cuda")
+
+
+def large_rows(n, kind):
+    """Finite rows whose squares (of x - mean) add up to more than a float holds, and an ordinary one behind them: large values, one and two
+    of the type's lowest among ordinary ones, sums and differences that are no float either, and a constant row whose mean is not met exactly."""
+    gen = torch.Generator().manual_seed(n)
+    z = torch.randn(11, n, generator=gen)
+    top = torch.finfo(ref.DTYPE[kind]).max
+    z[0] *= 1e27
+    z[1] *= 1e29
+    z[2] *= 1e31
+    z[3] *= 1e37
+    z[4, n // 2] = -top
+    z[5, 0] = z[5, n - 1] = -top
+    z[6] = top * (1 - 2 * (torch.arange(n) % 2))
+    z[7] = top * torch.where(torch.arange(n) % 4 == 3, -1.0, 1.0)
+    z[8, 1] = top
+    z[9] = 0.97 * top
+    z[9, 0] = 0.9 * top
+    return z.to(ref.DTYPE[kind])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [8, 64, 100, 250, 500, 1000, 2000, 3001, 5000, 9000, 16000, 40000])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("copies", [1, 110])
+def test_finite_rows_without_a_variance_in_floats(gpu, n, kind, copies):
+    """They give beta, in every form; their dx is zero, and of what is summed over rows they have a share of dbeta alone."""
+    rows = 11 * copies
+    x = large_rows(n, kind).repeat(copies, 1).cuda()
+    gamma, beta = (t.cuda() for t in vectors(n, n))
+    y, z = torch.empty(2, rows, n, device="cuda")
+    lib.layer_norm(x, gamma, beta, y, rows, n, eps=EPS, in_type=kind, out_type="f32")
+    flat = torch.arange(rows, device="cuda") % 11 < 10
+    assert torch.equal(y[flat], beta.expand(10 * copies, n))
+    ref.check(y[~flat], *ref.norm(x[~flat], gamma, beta, EPS), "f32")
+    lib.layer_norm(x, None, None, z, rows, n, eps=EPS, in_type=kind, out_type="f32")
+    assert not z[flat].any()
+    for fused, apart, sizes in ((lib.layer_norm_int8, lib.int8_quantize, (lib.int8_code_bytes(rows, n), 4 * rows)),
+                                (lib.layer_norm_mxfp4, lib.mxfp4_quantize, (lib.mxfp4_code_bytes(rows, n), lib.mxfp4_scale_bytes(rows, n)))):
+        got, want = ([torch.empty(size, dtype=torch.uint8, device="cuda") for size in sizes] for _ in range(2))
+        fused(x, gamma, beta, *got, rows, n, eps=EPS, in_type=kind)
+        apart(y, *want, rows, n, in_type="f32")
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    dy = torch.randn(rows, n, generator=torch.Generator().manual_seed(1)).cuda()
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.layer_norm_backward(dy, x, gamma, dx, dgamma, dbeta, work_of(rows, n), rows, n, eps=EPS, dy_type="f32", in_type=kind)
+    (want_dx, e_dx), (want_dgamma, e_dgamma), _ = ref.norm_gradients(dy[~flat], x[~flat], gamma, EPS)
+    assert not dx[flat].any()
+    ref.check(dx[~flat], want_dx, e_dx, kind)
+    ref.check(dgamma, want_dgamma, e_dgamma, "f32")
+    ref.check(dbeta, dy.double().sum(0), (rows + 2) * ref.U * dy.double().abs().sum(0), "f32")
