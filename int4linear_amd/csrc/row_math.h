@@ -207,11 +207,15 @@ struct RowStatistics {
     {
         // Finite values that lie too far apart have an infinite sum of squares.  With an infinity or a NaN among them it is a NaN: shift is one
         // too, or the same infinity, and so is what is left of that value.
-        const bool flat = squares == __builtin_inff();
-        const float delta = flat ? 0.0f : sum * over_n;
-        const float variance = fmaxf(fmaf(squares, over_n, -(delta * delta)), 0.0f);
-        const float r = rsqrtf((squares == squares ? variance : squares) + eps);
-        return {shift, r, -delta * r, flat};
+        const bool far = squares == __builtin_inff();
+        const float delta = far ? 0.0f : sum * over_n, square = delta * delta;
+        // Of a constant row whose mean is not met exactly every d is the same but 0, and the difference of the two squares, which is nothing but
+        // their roundings, counts as nothing below 2^-22 of them: r would make values of 1e10 and more out of what delta is off.  (Floats that are
+        // not all the same deviate by more: by n^-1/2 of a unit in the mean's last place, of which delta is a few.)
+        const float spread = fmaf(squares, over_n, -square);
+        const bool constant = spread < square * 0x1p-22f;
+        const float r = rsqrtf((constant ? 0.0f : spread) + eps);
+        return {shift, r, (constant ? 0.0f : -delta) * r, far || constant};
     }
     __device__ __forceinline__ float normalised(float d) const { return fmaf(d, r, c); }
     __device__ __forceinline__ float of(float x) const { return normalised(flat ? 0.0f : x - shift); }

@@ -485,3 +485,26 @@ def test_finite_rows_without_a_variance_in_floats(gpu, n, kind, copies):
     ref.check(dx[~flat], want_dx, e_dx, kind)
     ref.check(dgamma, want_dgamma, e_dgamma, "f32")
     ref.check(dbeta, dy.double().sum(0), (rows + 2) * ref.U * dy.double().abs().sum(0), "f32")
+
+
+#: what a constant row's values are: from where a rounding of the mean begins to count to where squares of what it leaves are no float
+CONSTANTS = [1.1e7, 1.1e9, 1.3e10, 1.7e12, 1.1e15, 1.9e18, 1.3e20, 1.1e24, 1.7e27, 1.1e33]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [7, 100, 250, 500, 700, 1000, 1500, 3001, 5000, 9001, 16001, 40001, 100001])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_constant_rows_of_any_size(gpu, n, kind):
+    """Whatever a rounding of the mean leaves of x - mean, the same in every column, is no deviation: y is beta."""
+    x = torch.tensor(CONSTANTS)[:, None].expand(-1, n).to(ref.DTYPE[kind]).contiguous().cuda()
+    rows = len(CONSTANTS)
+    y = torch.empty(rows, n, device="cuda")
+    lib.layer_norm(x, None, None, y, rows, n, eps=EPS, in_type=kind, out_type="f32")
+    # With d what is left, the same in all columns, h = (d - mean(d)) r: a mean of `depth` additions and two more roundings, each U of itself.
+    # Either the row counts as one without deviations, or its variance is 2^-22 of mean(d)^2 at least and |mean(d)| r 2^11 at most.
+    depth = n / 64 + 24
+    assert y.abs().max().item() <= (depth + 4) * ref.U * 2.0**11
+    dy = torch.randn(rows, n, generator=torch.Generator().manual_seed(1)).cuda()
+    dx, dgamma = torch.empty(rows, n, device="cuda").to(ref.DTYPE[kind]), torch.empty(n, device="cuda")
+    lib.layer_norm_backward(dy, x, None, dx, dgamma, None, work_of(rows, n), rows, n, eps=EPS, dy_type="f32", in_type=kind)
+    assert bool(torch.isfinite(dx).all()) and bool((dgamma.abs() <= (depth + 4) * ref.U * 2.0**11 * dy.abs().sum(0)).all())
