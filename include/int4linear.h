@@ -296,7 +296,7 @@ int int4linear_int8_linear(const void *x_codes_d, const float *x_scales_d, const
  * likewise; its bytes depend on dw_type):
  *   dx (m x k, bfloat16) = dy W,  dw (n x k, dw_type) = dy^T X,  dbias (n floats) = column sums of dy.
  * A value has more bits than bfloat16, which the products take: dx and a bfloat16 dw are sums of terms with W and X rounded to
- * bfloat16, which adds as much to their errors as their own rounding does; where dw_type is INT4LINEAR_OUT_F32 X is taken as the sum
+ * bfloat16 (finite ones beyond its largest to that), which adds as much to their errors as their own rounding does; where dw_type is INT4LINEAR_OUT_F32 X is taken as the sum
  * of three bfloat16, which loses nothing of a float, and that product takes three times as long (and m beyond 2^21 is refused). */
 size_t int4linear_int8_linear_backward_bytes(int m, int n, int k, int dw_type);
 int int4linear_int8_linear_backward(const void *dy_d, const void *x_codes_d, const float *x_scales_d, const void *w_codes_d,

@@ -233,21 +233,43 @@ __device__ __forceinline__ void transpose_int8(const Transposed &t, int k, int d
 #pragma unroll
         for (int c = 0; c < 8; ++c)
             v[r][c] = (float)(int8_t)(codes[r][c / 4] >> 8 * (c % 4)) * scales[r];
+    // Between the largest bfloat16 and the largest float the nearest bfloat16 is an infinity: such a value becomes the former, or where it goes in
+    // pieces each of them is cut off, not rounded, so that no sum of them exceeds it.  (128 times such a scale gets there.)
+    bool large = false;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+        large = large || fabsf(scales[r]) >= 0x1p120f;
     uint16_t *dst = t.dst + (size_t)c0 * t.ld + r0;
     for (int pieces = t.apart ? 3 : 1;;) {
         v4u rows[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r)
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const v2bf two = {(__bf16)v[r][2 * p], (__bf16)v[r][2 * p + 1]};
-                v[r][2 * p] -= (float)two[0];
-                v[r][2 * p + 1] -= (float)two[1];
-                rows[r][p] = __builtin_bit_cast(unsigned, two);
-            }
+            for (int p = 0; p < 4; ++p)
+                rows[r][p] = __builtin_bit_cast(unsigned, (v2bf){(__bf16)v[r][2 * p], (__bf16)v[r][2 * p + 1]});
+        if (large) {  // rare
+            auto beyond = [](unsigned bits, float value) { return (bits & 0x7FFFu) == 0x7F80u && fabsf(value) < __builtin_inff(); };
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const float low = v[r][2 * p], high = v[r][2 * p + 1];
+                    if (t.apart)
+                        rows[r][p] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, high), __builtin_bit_cast(unsigned, low), 0x07060302u);
+                    else
+                        rows[r][p] -= (beyond(rows[r][p], low) ? 1u : 0u) + (beyond(rows[r][p] >> 16, high) ? 0x10000u : 0u);
+                }
+        }
         store_transposed(rows, dst, t.ld, k - c0);
         if (--pieces == 0)
             break;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                v[r][2 * p] -= __builtin_bit_cast(float, rows[r][p] << 16);
+                v[r][2 * p + 1] -= __builtin_bit_cast(float, rows[r][p] & 0xFFFF0000u);
+            }
         dst += t.apart;
     }
 }

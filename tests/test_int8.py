@@ -434,3 +434,40 @@ def test_results_do_not_change_from_stream_to_stream(gpu):
         torch.cuda.synchronize()
         first = first or (y, dx, dw)
         assert all(torch.equal(a, b) for a, b in zip(first, (y, dx, dw)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(3, 40, 70), (200, 130, 515)])
+@pytest.mark.parametrize("dw_type", ["bf16", "f32"])
+def test_gradients_at_the_largest_floats(gpu, m, n, k, dw_type):
+    """Values above the largest bfloat16, which is 2^-8 below the largest float."""
+    (xq, _), (wq, _) = matrix(m, m, k), matrix(n, n, k)
+    top = torch.finfo(torch.float32).max
+    for codes, scales in (xq, wq):
+        codes[:, :k][codes[:, :k] == -128] = 127
+        codes[:, 0], codes[:, k - 1] = 127, -127
+        scales[:2] = top / 127 * (1 - 2.0**-23)  # (127 times the rounded quotient is no float)
+    x, w = ref.decode(*xq, k), ref.decode(*wq, k)
+    assert (x.abs() > 3.39e38).any() and x.abs().max().item() <= top and w.abs().max().item() <= top
+    dy = (torch.randn(m, n, generator=torch.Generator().manual_seed(m * n)) * 2.0**-20).bfloat16().cuda()
+    dx, dw = torch.empty(m, k, dtype=torch.bfloat16, device="cuda"), torch.empty(n, k, dtype=ref.DTYPE[dw_type], device="cuda")
+    work = torch.empty(lib.int8_linear_backward_bytes(m, n, k, dw_type), dtype=torch.uint8, device="cuda")
+    lib.int8_linear_backward(dy, *xq, *wq, dx, dw, dw_type, None, work, m, n, k)
+    d = dy.double()
+    # as in test_linear_backward: a factor above the largest bfloat16 is taken as that, which is off by 2^-8 of it
+    ref.check(dx, d @ w, (2.0**-8 + n * 2.0**-23) * (d.abs() @ w.abs()), "bf16")
+    ref.check(dw, d.T @ x, ((2.0**-8 if dw_type == "bf16" else 2.0**-24) + 3 * m * 2.0**-23) * (d.abs().T @ x.abs()), dw_type)
+
+
+@pytest.mark.gpu
+def test_gradients_as_floats_keep_the_bits_of_the_largest_values(gpu):
+    """One token with dy = 1: dw is X itself, up to the largest float."""
+    k = 256
+    codes = torch.randint(-127, 128, (1, k), dtype=torch.int8, generator=torch.Generator().manual_seed(1)).cuda()
+    codes[0, 0], codes[0, 1] = 127, -127
+    dy, work = torch.ones(1, 8, dtype=torch.bfloat16, device="cuda"), torch.empty(1 << 25, dtype=torch.uint8, device="cuda")
+    s = torch.tensor([torch.finfo(torch.float32).max / 127 * (1 - 2.0**-23)], device="cuda")
+    dw = torch.empty(8, k, device="cuda")
+    lib.int8_linear_backward(dy, codes, s, None, None, None, dw, "f32", None, work, 1, 8, k)
+    want = codes.float() * s
+    assert bool(torch.isfinite(want).all()) and torch.equal(dw, want.expand(8, k))
