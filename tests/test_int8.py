@@ -471,3 +471,27 @@ def test_gradients_as_floats_keep_the_bits_of_the_largest_values(gpu):
     lib.int8_linear_backward(dy, codes, s, None, None, None, dw, "f32", None, work, 1, 8, k)
     want = codes.float() * s
     assert bool(torch.isfinite(want).all()) and torch.equal(dw, want.expand(8, k))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows, k", [(9000, 500), (5000, 1000), (1100, 2000), (1030, 4000), (1100, 4999), (1030, 8192), (1030, 12001), (1024, 16384)])
+def test_quantize_of_many_rows(gpu, rows, k, kind):
+    """The kernels that many rows choose, every code and scale against the formula."""
+    gen = torch.Generator().manual_seed(rows + k)
+    x = (torch.randn(rows, k, generator=gen) * torch.exp2(20 * torch.rand(rows, 1, generator=gen) - 10)).to(ref.DTYPE[kind])
+    assert same(quantize(x.cuda(), kind=kind), ref.encode(x.float()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2])
+def test_one_and_two_rows_against_weights_beyond_4_gib(gpu, m):
+    n, k = (1 << 16) + 5, (1 << 16) + 128
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    codes = torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda", generator=gen)
+    scales = torch.rand(n, device="cuda", generator=gen)
+    (xq, x) = matrix(4, m, k)
+    y = torch.empty(m, n, device="cuda")
+    lib.int8_linear(*xq, codes, scales, None, y, "f32", m, n, k)
+    at = torch.tensor([0, 1, n // 2, n - 6, n - 1], device="cuda")
+    ref.check(y[:, at], *product(x.cuda(), ref.decode(codes[at], scales[at], k)), "f32")

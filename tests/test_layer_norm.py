@@ -508,3 +508,61 @@ def test_constant_rows_of_any_size(gpu, n, kind):
     dx, dgamma = torch.empty(rows, n, device="cuda").to(ref.DTYPE[kind]), torch.empty(n, device="cuda")
     lib.layer_norm_backward(dy, x, None, dx, dgamma, None, work_of(rows, n), rows, n, eps=EPS, dy_type="f32", in_type=kind)
     assert bool(torch.isfinite(dx).all()) and bool((dgamma.abs() <= (depth + 4) * ref.U * 2.0**11 * dy.abs().sum(0)).all())
+
+
+# ---- kernels that stay for several rows, and those that many rows choose
+
+
+#: rows, n: for every way in which rows are dealt to waves, three turns of a workgroup and more
+TURNS = [(70000, 40), (70000, 64), (40000, 128), (20000, 250), (9000, 500), (9001, 1000), (7000, 2000), (2501, 4000), (1000, 3000), (2000, 8000),
+         (1030, 8192), (1300, 4999), (1100, 12001), (600, 16384), (601, 9001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, n", TURNS)
+@pytest.mark.parametrize("kind, out", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+def test_every_row_of_many(gpu, rows, n, kind, out):
+    x = rows_of(rows + n, rows, n, kind).cuda()
+    gamma, beta = (t.cuda() for t in vectors(n, n))
+    raw, y = guarded(rows * n * ref.DTYPE[out].itemsize)
+    lib.layer_norm(x, gamma, beta, y, rows, n, eps=EPS, in_type=kind, out_type=out)
+    torch.cuda.synchronize()
+    assert untouched(raw)
+    ref.check(y.view(ref.DTYPE[out]).view(rows, n), *ref.norm(x, gamma, beta, EPS), out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, n", TURNS)
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_every_quantised_row_of_many(gpu, rows, n, kind):
+    """Bit for bit what the norm as floats gives after its quantisation, which takes other kernels."""
+    x = rows_of(rows + n, rows, n, kind).cuda()
+    gamma, beta = (t.cuda() for t in vectors(n, n))
+    y = torch.empty(rows, n, device="cuda")
+    lib.layer_norm(x, gamma, beta, y, rows, n, in_type=kind, out_type="f32")
+    ref.check(y, *ref.norm(x, gamma, beta, EPS), "f32")
+    for fused, apart, sizes in ((lib.layer_norm_int8, lib.int8_quantize, (lib.int8_code_bytes(rows, n), 4 * rows)),
+                                (lib.layer_norm_mxfp4, lib.mxfp4_quantize, (lib.mxfp4_code_bytes(rows, n), lib.mxfp4_scale_bytes(rows, n)))):
+        (raw_c, codes), (raw_s, scales) = guarded(sizes[0]), guarded(sizes[1])
+        want = [torch.empty(size, dtype=torch.uint8, device="cuda") for size in sizes]
+        fused(x, gamma, beta, codes, scales, rows, n, in_type=kind)
+        apart(y, *want, rows, n, in_type="f32")
+        torch.cuda.synchronize()
+        assert untouched(raw_c) and untouched(raw_s) and torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, n", [(70000, 64), (40000, 128), (20000, 250), (9000, 500), (5001, 1000), (2500, 2000), (1100, 4000), (600, 8000),
+                                     (600, 16384), (900, 9001), (300, 20000)])
+@pytest.mark.parametrize("kind, dy_kind", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16"), ("bf16", "f32")])
+def test_gradients_of_many_rows(gpu, rows, n, kind, dy_kind):
+    x = rows_of(rows + n, rows, n, kind, spread=0.5).cuda()
+    dy = torch.randn(rows, n, generator=torch.Generator().manual_seed(rows)).to(ref.DTYPE[dy_kind]).cuda()
+    gamma = vectors(n, n)[0].cuda()
+    (raw_x, dx), (raw_g, dgamma), (raw_b, dbeta) = guarded(rows * n * ref.DTYPE[kind].itemsize), guarded(4 * n), guarded(4 * n)
+    lib.layer_norm_backward(dy, x, gamma, dx, dgamma, dbeta, work_of(rows, n), rows, n, dy_type=dy_kind, in_type=kind)
+    torch.cuda.synchronize()
+    assert untouched(raw_x) and untouched(raw_g) and untouched(raw_b)
+    got = dx.view(ref.DTYPE[kind]).view(rows, n), dgamma.view(torch.float32), dbeta.view(torch.float32)
+    for value, (want, error), out in zip(got, ref.norm_gradients(dy, x, gamma, EPS), (kind, "f32", "f32")):
+        ref.check(value, want, error, out)
