@@ -375,29 +375,31 @@ __device__ __forceinline__ void transpose_dy(const Prepared &p, int down, int ac
     }
 }
 
-// A workgroup takes DOWN x kTilesAcross tiles of one of the matrices, or of dy behind them: the first of each of these has number
-// first[i], and down[i] of them lie one below the other.  (A grid that is as long and as wide as the longest and the widest of them is mostly
-// empty workgroups where these differ.  Gradients of an 8-bit layer, us: 445 x 16320 x 2816 250, so 193; 64 x 8192 x 1024 57, 37; small ones
-// pay 0.4 for their number, 130 x 1001 x 515 14.1, 14.5.)
+// A workgroup takes DOWN x kTilesAcross tiles of one of the matrices, or of dy behind them.  LISTED: blockIdx.x numbers these workgroups, the first
+// of each operand has number first[i], and down[i] of them lie one below the other.  Else blockIdx.z is the operand, in a grid that is as long and as
+// wide as the longest and the widest of them, mostly empty where these differ.
 struct PrepareGrid {
     unsigned first[4], down[4], inverse[4];  // (first: of those that are not there, the number behind the last)
     // inverse: the whole part of 2^32 / down, or the largest number: a quotient by it is the true one or one less
 };
 
-template <int DOWN, bool INT8>
+template <int DOWN, bool INT8, bool LISTED>
 __global__ __launch_bounds__(DOWN *kTilesAcross * 64) void prepare_kernel(Prepared p, PrepareGrid grid, size_t code_stride, size_t scale_stride)
 {
-    if (blockIdx.x == 0)
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
         for (int i = threadIdx.x; i < p.zero_count; i += DOWN * kTilesAcross * 64)
             p.zeros[i] = 0;
-    int which = 0;
+    int which = (int)blockIdx.z, down = (int)blockIdx.x, across = (int)blockIdx.y;
+    if constexpr (LISTED) {
 #pragma unroll
-    for (int i = 1; i < 4; ++i)
-        which += blockIdx.x >= grid.first[i];
-    const unsigned mine = blockIdx.x - grid.first[which], its_down = grid.down[which];
-    unsigned quotient = __umulhi(mine, grid.inverse[which]);
-    quotient += mine - quotient * its_down >= its_down;
-    const int across = (int)quotient, down = (int)(mine - quotient * its_down);
+        for (int i = 1; i < 4; ++i)
+            which += blockIdx.x >= grid.first[i];
+        const unsigned mine = blockIdx.x - grid.first[which], its_down = grid.down[which];
+        unsigned quotient = __umulhi(mine, grid.inverse[which]);
+        quotient += mine - quotient * its_down >= its_down;
+        across = (int)quotient;
+        down = (int)(mine - quotient * its_down);
+    }
     if (which < p.matrices)
         if constexpr (INT8)
             transpose_int8<DOWN>(p.matrix[which], p.k, down, across);
@@ -485,6 +487,13 @@ hipError_t launch_mx_dequantize(const MxMatrix &q, void *y, int type, size_t ld,
 // 257 x 1400 x 1000 6.2, 9.2; 130 x 1001 x 515 6.7, 9.)
 constexpr long kLargeTranspose = 256l * 256 * 256;
 
+// How these are dealt to the device.  Workgroups of 16 waves are listed: gradients of an 8-bit layer, us, 445 x 16320 x 2816 250, so 193; of MXFP4
+// ones 64 x 8192 x 1024 52.8, 48.2.  Those of 4 as well, in columns of multiples of 8, so that what lies side by side comes to one XCD.  MXFP4, us, in a
+// box, listed as they come, in such columns: 130 x 1001 x 515 13.7, 14.0, 13.7; 16 x 2000 x 2000 22.6, 24.5, 22.6; 256 x 1024 x 4096 25.4, 26.2, 24.7;
+// 16 x 4000 x 1000 28.6, 28.5, 26.6; beyond four of them to a CU the box is quicker more often than not, 16 x 4000 x 4000 40.9, 43.5, 45.3; 64 x 4064 x
+// 4096 49.0, 47.2, 47.5, but not with 8-bit operands: 39.3, 39.0, 38.4 (64 rows) and 43.8, 40.4, 40.1.
+constexpr unsigned kMostListed = 1024, kXcds = 8;
+
 hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
 {
     int rows = p.dy ? p.rows : 0, cols = p.dy ? p.cols : 0;
@@ -503,15 +512,22 @@ hipError_t launch_prepare(const Prepared &p, hipStream_t stream)
             const bool is_dy = i == p.matrices && p.dy;
             if (i < p.matrices || is_dy) {
                 const int its_rows = is_dy ? p.rows : p.matrix[i].of.q.rows, its_cols = is_dy ? p.cols : p.k;
-                grid.down[i] = (unsigned)((its_rows + kSide - 1) / kSide);
+                constexpr unsigned kStep = DOWN == 1 ? kXcds : 1;
+                grid.down[i] = ((unsigned)((its_rows + kSide - 1) / kSide) + kStep - 1) / kStep * kStep;
                 grid.inverse[i] = grid.down[i] > 1 ? (unsigned)((1ull << 32) / grid.down[i]) : ~0u;
                 count += grid.down[i] * (unsigned)((its_cols + kWide - 1) / kWide);
             }
         }
+        const size_t code_stride = mx_code_stride(p.k), scale_stride = mx_scale_stride(p.k);
+        constexpr int kGroup = DOWN * kTilesAcross * 64;
         if (p.int8)
-            prepare_kernel<DOWN, true><<<count, DOWN * kTilesAcross * 64, 0, stream>>>(p, grid, 0, 0);
-        else
-            prepare_kernel<DOWN, false><<<count, DOWN * kTilesAcross * 64, 0, stream>>>(p, grid, mx_code_stride(p.k), mx_scale_stride(p.k));
+            prepare_kernel<DOWN, true, true><<<count, kGroup, 0, stream>>>(p, grid, 0, 0);
+        else if (DOWN > 1 || count <= kMostListed)
+            prepare_kernel<DOWN, false, true><<<count, kGroup, 0, stream>>>(p, grid, code_stride, scale_stride);
+        else if constexpr (DOWN == 1)
+            prepare_kernel<1, false, false><<<dim3((unsigned)((rows + kSide - 1) / kSide), (unsigned)((cols + kWide - 1) / kWide),
+                                                   (unsigned)(p.matrices + (p.dy != nullptr))),
+                                              kGroup, 0, stream>>>(p, grid, code_stride, scale_stride);
     };
     if ((long)rows * cols >= kLargeTranspose)
         run(std::integral_constant<int, 4>{});
