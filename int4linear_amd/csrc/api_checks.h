@@ -28,6 +28,11 @@ struct Checks {
         that(a >= 0 && b >= 0 && c >= 0, INT4LINEAR_ERR_SHAPE);
         return that(a <= kMostRows && b <= kMostRows && c <= kMostRows, INT4LINEAR_ERR_UNSUPPORTED);
     }
+    // Elements between rows of `columns`.  (A negative number given as size_t is beyond all memory: rows would lie in front of the array.)
+    Checks &apart(size_t ld, int columns)
+    {
+        return that(ld >= (size_t)(columns > 0 ? columns : 0) && ld <= (size_t)1 << 48, INT4LINEAR_ERR_SHAPE);
+    }
     // An array the call reads or writes; `used`: it has elements.
     Checks &array(const void *p, size_t alignment, bool used)
     {

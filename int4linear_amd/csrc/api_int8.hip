@@ -26,9 +26,9 @@ int layer_norm(RowPass p, void *stream)
 {
     const bool used = p.rows > 0 && p.n > 0;
     Checks ok;
-    ok.sizes(p.rows, p.n, 0).that(p.ld >= (size_t)(p.n > 0 ? p.n : 0), INT4LINEAR_ERR_SHAPE);
+    ok.sizes(p.rows, p.n, 0).apart(p.ld, p.n);
     if (p.result == kRowTyped)
-        ok.that(p.ld_y >= (size_t)(p.n > 0 ? p.n : 0), INT4LINEAR_ERR_SHAPE);
+        ok.apart(p.ld_y, p.n);
     ok.that(p.n <= kMostNorm && is_type(p.type) && p.eps >= 0.0f && std::isfinite(p.eps), INT4LINEAR_ERR_UNSUPPORTED);
     if (p.result == kRowTyped)
         ok.that(is_type(p.out), INT4LINEAR_ERR_UNSUPPORTED);
@@ -55,7 +55,7 @@ size_t int4linear_int8_code_bytes(int rows, int k) { return rows < 0 || k < 0 ? 
 int int4linear_int8_quantize(const void *x_d, int type, size_t ld, void *codes_d, float *scales_d, int rows, int k, void *stream)
 {
     Checks ok;
-    ok.sizes(rows, 0, k).that(ld >= (size_t)(k > 0 ? k : 0), INT4LINEAR_ERR_SHAPE).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(rows, 0, k).apart(ld, k).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
     if (!ok || rows == 0 || k == 0)
         return ok.status;
     ok.array(x_d, type_bytes(type), true);
@@ -81,7 +81,7 @@ int int4linear_int8_quantize(const void *x_d, int type, size_t ld, void *codes_d
 int int4linear_int8_dequantize(const void *codes_d, const float *scales_d, void *y_d, int type, size_t ld, int rows, int k, void *stream)
 {
     Checks ok;
-    ok.sizes(rows, 0, k).that(ld >= (size_t)(k > 0 ? k : 0), INT4LINEAR_ERR_SHAPE).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(rows, 0, k).apart(ld, k).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
     if (!ok || rows == 0 || k == 0)
         return ok.status;
     ok.array(y_d, type_bytes(type), true);
@@ -152,9 +152,10 @@ int int4linear_layer_norm_backward(const void *dy_d, int dy_type, size_t ld_dy, 
                                    float eps, void *dx_d, size_t ld_dx, float *dgamma_d, float *dbeta_d, void *work_d, size_t work_bytes,
                                    int rows, int n, void *stream)
 {
-    const size_t least = (size_t)(n > 0 ? n : 0);
     Checks ok;
-    ok.sizes(rows, n, 0).that(ld_dy >= least && ld >= least && (!dx_d || ld_dx >= least), INT4LINEAR_ERR_SHAPE);
+    ok.sizes(rows, n, 0).apart(ld_dy, n).apart(ld, n);
+    if (dx_d)
+        ok.apart(ld_dx, n);
     ok.that(n <= kMostNorm && is_type(dy_type) && is_type(type) && eps >= 0.0f && std::isfinite(eps), INT4LINEAR_ERR_UNSUPPORTED);
     const bool want_dx = dx_d && rows > 0;
     if (!ok || n == 0 || (!want_dx && !dgamma_d && !dbeta_d))

@@ -50,7 +50,7 @@ size_t int4linear_mxfp4_scale_bytes(int rows, int k) { return rows < 0 || k < 0 
 int int4linear_mxfp4_quantize(const void *x_d, int type, size_t ld, void *codes_d, void *scales_d, int rows, int k, void *stream)
 {
     Checks ok;
-    ok.sizes(rows, 0, k).that(ld >= (size_t)(k > 0 ? k : 0), INT4LINEAR_ERR_SHAPE).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(rows, 0, k).apart(ld, k).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
     ok.array(x_d, type_bytes(type), rows > 0 && k > 0).matrix(codes_d, scales_d, rows, k);
     if (!ok || rows == 0 || k == 0)
         return ok.status;
@@ -65,7 +65,7 @@ int int4linear_mxfp4_dequantize(const void *codes_d, const void *scales_d, void 
                                 void *stream)
 {
     Checks ok;
-    ok.sizes(rows, 0, k).that(ld >= (size_t)(k > 0 ? k : 0), INT4LINEAR_ERR_SHAPE).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
+    ok.sizes(rows, 0, k).apart(ld, k).that(is_type(type), INT4LINEAR_ERR_UNSUPPORTED);
     ok.array(y_d, type_bytes(type), rows > 0 && k > 0).matrix(codes_d, scales_d, rows, k);
     if (!ok || rows == 0 || k == 0)
         return ok.status;

@@ -77,6 +77,21 @@ def test_objects_without_an_address_are_refused(wrong):
         lib.layer_norm_backward(A, A, A, A, A, A, A, 1, 8, stream=0)
 
 
+def test_rows_a_negative_number_apart_are_refused():
+    """(ctypes makes a size_t of it; rows would lie in front of the array.)"""
+    A = 4096
+    for call in (lambda: lib.layer_norm(A, A, A, A, 3, 8, ld=-8, stream=0), lambda: lib.layer_norm(A, A, A, A, 3, 8, ld_y=-8, stream=0),
+                 lambda: lib.layer_norm_int8(A, A, A, A, A, 3, 8, ld=-8, stream=0), lambda: lib.layer_norm_mxfp4(A, A, A, A, A, 3, 8, ld=-1, stream=0),
+                 lambda: lib.layer_norm_backward(A, A, A, A, A, A, A, 3, 8, ld=-8, work_bytes=1 << 30, stream=0),
+                 lambda: lib.layer_norm_backward(A, A, A, A, A, A, A, 3, 8, ld_dy=-8, work_bytes=1 << 30, stream=0),
+                 lambda: lib.layer_norm_backward(A, A, A, A, A, A, A, 3, 8, ld_dx=-8, work_bytes=1 << 30, stream=0),
+                 lambda: lib.int8_quantize(A, A, A, 3, 8, ld=-8, stream=0), lambda: lib.int8_dequantize(A, A, A, 3, 8, ld=-8, stream=0),
+                 lambda: lib.mxfp4_quantize(A, A, A, 3, 8, ld=-8, stream=0), lambda: lib.mxfp4_dequantize(A, A, A, 3, 8, ld=-8, stream=0)):
+        with pytest.raises(lib.Int4LinearError) as refused:
+            call()
+        assert refused.value.status == SHAPE
+
+
 def test_the_reference_gradients_against_differences():
     """The formulas that the device's gradients are compared with, against central differences."""
     gen = torch.Generator().manual_seed(5)
