@@ -495,3 +495,23 @@ def test_one_and_two_rows_against_weights_beyond_4_gib(gpu, m):
     lib.int8_linear(*xq, codes, scales, None, y, "f32", m, n, k)
     at = torch.tensor([0, 1, n // 2, n - 6, n - 1], device="cuda")
     ref.check(y[:, at], *product(x.cuda(), ref.decode(codes[at], scales[at], k)), "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n", [(1, (1 << 22) + 5), (2, (1 << 22) + 4097), (5, (1 << 25) + 37)])
+def test_more_workgroups_than_one_axis_holds(gpu, m, n):
+    """Streamed weights of very many short rows."""
+    k = 20
+    (xq, x) = matrix(1, m, k)
+    gen = torch.Generator("cuda").manual_seed(n)
+    codes = torch.randint(-128, 128, (n, 128), dtype=torch.int8, device="cuda", generator=gen)
+    codes[:, k:] = 0
+    scales = torch.rand(n, device="cuda", generator=gen)
+    raw, y = guarded(m * n * 2)
+    lib.int8_linear(*xq, codes, scales, None, y, "bf16", m, n, k)
+    torch.cuda.synchronize()
+    assert untouched(raw)
+    y = y.view(torch.bfloat16).view(m, n)
+    for at in range(0, n, 1 << 22):
+        part = slice(at, min(n, at + (1 << 22)))
+        ref.check(y[:, part], *product(x.cuda(), ref.decode(codes[part], scales[part], k)), "bf16")

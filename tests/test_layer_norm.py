@@ -581,3 +581,50 @@ def test_gradients_of_many_rows(gpu, rows, n, kind, dy_kind):
     got = dx.view(ref.DTYPE[kind]).view(rows, n), dgamma.view(torch.float32), dbeta.view(torch.float32)
     for value, (want, error), out in zip(got, ref.norm_gradients(dy, x, gamma, EPS), (kind, "f32", "f32")):
         ref.check(value, want, error, out)
+
+
+# ---- the ends of the ranges
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_the_longest_rows(gpu, kind):
+    """2^22 columns, the last of them with the largest values: a plain sum of them would be 2^22 times what a float holds."""
+    rows, n = 3, 1 << 22
+    x = rows_of(5, rows, n, kind)
+    x[2] = torch.finfo(ref.DTYPE[kind]).max
+    x = x.cuda()
+    gamma, beta = (t.cuda() for t in vectors(1, n))
+    y = torch.empty(rows, n, device="cuda")
+    lib.layer_norm(x, gamma, beta, y, rows, n, eps=EPS, in_type=kind, out_type="f32")
+    ref.check(y[:2], *ref.norm(x[:2], gamma, beta, EPS), "f32")
+    assert torch.equal(y[2], beta)
+    dy = torch.randn(rows, n, generator=torch.Generator().manual_seed(2)).cuda()
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.layer_norm_backward(dy, x, gamma, dx, dgamma, dbeta, work_of(rows, n), rows, n, eps=EPS, dy_type="f32", in_type=kind)
+    (want_dx, e_dx), (want_dgamma, e_dgamma), _ = ref.norm_gradients(dy[:2], x[:2], gamma, EPS)
+    ref.check(dx[:2], want_dx, e_dx, kind)
+    assert bool(torch.isfinite(dx[2]).all())
+    ref.check(dgamma, want_dgamma, e_dgamma, "f32")
+    ref.check(dbeta, dy.double().sum(0), (rows + 2) * ref.U * dy.double().abs().sum(0), "f32")
+
+
+@pytest.mark.gpu
+def test_very_many_short_rows(gpu):
+    """2^25 rows and a few: beyond what one axis of a launch holds, in every form and back."""
+    rows, n = (1 << 25) + 5, 3
+    x = torch.randn(rows, n, generator=torch.Generator("cuda").manual_seed(1), device="cuda") + 2
+    gamma, beta = (t.cuda() for t in vectors(1, n))
+    y = torch.empty_like(x)
+    lib.layer_norm(x, gamma, beta, y, rows, n, eps=EPS, in_type="f32", out_type="f32")
+    ref.check(y, *ref.norm(x, gamma, beta, EPS), "f32")
+    codes, scales = torch.empty(rows, 128, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    want = torch.empty_like(codes), torch.empty_like(scales)
+    lib.layer_norm_int8(x, gamma, beta, codes, scales, rows, n, in_type="f32")
+    lib.int8_quantize(y, *want, rows, n, in_type="f32")
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+    del codes, scales, want
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.layer_norm_backward(x, x, gamma, dx, dgamma, dbeta, work_of(rows, n), rows, n, eps=EPS, dy_type="f32", in_type="f32")
+    for value, (want, error) in zip((dx, dgamma, dbeta), ref.norm_gradients(x, x, gamma, EPS)):
+        ref.check(value, want, error, "f32")
