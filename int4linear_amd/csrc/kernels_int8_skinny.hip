@@ -1,8 +1,9 @@
 // Few rows of x against 8-bit weights: every byte of w is read once, and the stream of w is what bounds it.
 //
-// Up to four rows: a wave takes whole rows of w, 16 bytes a lane, so that a load is 1 KB of one row, straight into registers; four
-// products to an instruction (v_dot4_i32_i8) are enough for what arrives, and the lanes' sums meet once at the end.  8192 x 8192, one
-// row, weights from HBM: 11.7 us = 5.7 TB/s; a kernel that does nothing but read as much takes 11.1.
+// One and two rows, three and four against fewer than 8192 of w: two waves share the k of two rows of w, 16 bytes a lane, so that a load is 1 KB of
+// one row, straight into registers; four products to an instruction (v_dot4_i32_i8) are enough for what arrives, and the lanes' sums meet
+// once at the end, then those of the two waves in LDS.  8192 x 8192, one row, weights from HBM: 11.6 us = 5.8 TB/s; a kernel that does nothing but
+// read as much takes 11.1.
 // More: a workgroup takes 16 R rows of w and all of k, its waves split k line by line.  A wave's lines of w and x go straight to LDS
 // (eight rows of 128 bytes an instruction), those of its next line while it multiplies this one's with v_mfma_i32_16x16x64_i8, and the
 // waves' sums meet in LDS.  Workgroups begin at different lines: rows lie a power of two apart as often as not, and where all begin
@@ -243,14 +244,16 @@ constexpr int kMostWaves = 8;
 
 }  // namespace
 
-// Where this kernel is quicker than tiles of 64 x 64 and more.  us here and on tiles, weights from HBM:
+// Where this kernel is quicker than tiles (of any size, those that have a CU to themselves among them).  us here and on tiles, weights from HBM:
 //   rows of x            3            16           32           48           64
-//   4096 x 4096          5.7, 8.3     6.4, 8.3     7.3, 8.4     8.2, 8.5     8.9, 8.5
-//   4096 x 14336         13.0, 29.9   13.6, 30.4   16.9, 31.4   20.6, 33.5   22.7, 36.5
-//   1024 x 8192          5.1, 13.4    7.9, 13.4    9.9, 13.5    11.8, 13.6   13.0, 13.6
-//   8192 x 8192          13.3, 20.0   13.8, 20.1   15.2, 20.5   17.4, 21.7   19.6, 23.2
-//   14336 x 4096         11.9, 15.2   12.8, 15.3   14.9, 15.4   18.2, 15.6   23.1, 16.0
-//   28672 x 8192         38.5, 54     41.0, 54.1   48.1, 54.7   56.0, 54.6   69.7, 54.9
+//   2048 x 2048          4.8, 5.5     5.1, 5.6     5.1, 5.7     5.7, 5.8     6.1, 5.8
+//   4096 x 4096          6.3, 8.3     6.2, 8.3     7.0, 8.4     8.1, 8.5     8.7, 8.5
+//   4096 x 14336         13.3, 29.9   13.5, 30.3   16.8, 31.4   20.4, 33.2   22.5, 36.3
+//   1024 x 8192          4.7, 13.4    7.7, 13.5    9.8, 13.6    11.6, 13.6   12.8, 13.7
+//   8192 x 8192          13.1, 19.9   13.5, 20.1   15.4, 20.7   17.5, 21.5   19.6, 23.1
+//   14336 x 4096         11.7, 14.8   12.6, 15.2   14.8, 15.4   18.2, 15.6   23.0, 16.0
+//   28672 x 8192         38.2, 51.0   40.6, 48.6   48.1, 51.8   55.3, 52.2   69.7, 52.6
+// (It does not look at k: against short rows of w the tiles are 3 to 5 % quicker from 56 rows of x on.)
 bool int8_skinny_preferred(int m, int n) { return m <= 32 || (m <= 64 && n <= kWide); }
 
 hipError_t int8_skinny_init()

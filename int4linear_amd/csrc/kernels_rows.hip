@@ -96,7 +96,8 @@ __device__ __forceinline__ void centre8(float shift, int c0, int n, float (&v)[8
     }
 }
 
-// Rows of any length: a workgroup takes a row at a time and reads it again in every pass, from the caches.
+// Rows of any length: a workgroup takes a row at a time and reads it again in every pass, from the caches: twice for its quantisation, three times
+// for a norm, four for a norm into 8 bits (4096 x 28672 bf16 101 us = 3.5 TB/s, 155 = 3.0, 186 = 1.9; into MXFP4 134).
 template <int TYPE, int RESULT, bool NORM>
 __global__ __launch_bounds__(kThreads) void row_loop_kernel(RowPass p, size_t code_stride, size_t scale_stride)
 {
