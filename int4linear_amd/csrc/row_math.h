@@ -209,12 +209,13 @@ struct RowStatistics {
         // too, or the same infinity, and so is what is left of that value.
         const bool far = squares == __builtin_inff();
         const float delta = far ? 0.0f : sum * over_n, square = delta * delta;
-        // Of a constant row whose mean is not met exactly every d is the same but 0, and the difference of the two squares, which is nothing but
-        // their roundings, counts as nothing below 2^-22 of them: r would make values of 1e10 and more out of what delta is off.  (Floats that are
-        // not all the same deviate by more: by n^-1/2 of a unit in the mean's last place, of which delta is a few.)
+        // Of a constant row whose mean is not met exactly every d is the same but 0, and the difference of the two squares is nothing but their
+        // roundings.  Where it and eps are below 2^-22 of them it counts as nothing: r would make values of 1e10 and more out of what delta is
+        // off.  (Floats that are not all the same deviate by more: by n^-1/2 of a unit in the mean's last place, of which delta is a few.)
         const float spread = fmaf(squares, over_n, -square);
-        const bool constant = spread < square * 0x1p-22f;
-        const float r = rsqrtf((constant ? 0.0f : spread) + eps);
+        const float variance = (spread < 0.0f ? 0.0f : spread) + eps;
+        const bool constant = variance < square * 0x1p-22f;
+        const float r = rsqrtf(constant ? eps : variance);
         return {shift, r, (constant ? 0.0f : -delta) * r, far || constant};
     }
     __device__ __forceinline__ float normalised(float d) const { return fmaf(d, r, c); }

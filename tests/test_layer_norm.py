@@ -525,6 +525,23 @@ def test_constant_rows_of_any_size(gpu, n, kind):
     assert bool(torch.isfinite(dx).all()) and bool((dgamma.abs() <= (depth + 4) * ref.U * 2.0**11 * dy.abs().sum(0)).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1000, 16001, 100001])
+def test_rows_that_are_constant_but_for_a_few_columns(gpu, n):
+    """Deviations of one unit in the last place, that eps is large beside: they stay, as small as they are."""
+    x = torch.tensor([1050.8, 1.3, 7777.7])[:, None].repeat(1, n)
+    x[:, [1, n // 2, n - 1]] *= 1 + 2.0**-23
+    x = x.cuda()
+    gamma, beta = (t.cuda() for t in vectors(n, n))
+    y, dx, dgamma = torch.empty(3, n, device="cuda"), torch.empty(3, n, device="cuda"), torch.empty(n, device="cuda")
+    lib.layer_norm(x, gamma, beta, y, 3, n, eps=EPS, in_type="f32", out_type="f32")
+    ref.check(y, *ref.norm(x, gamma, beta, EPS), "f32")
+    dy = torch.randn(3, n, generator=torch.Generator().manual_seed(1)).cuda()
+    lib.layer_norm_backward(dy, x, gamma, dx, dgamma, None, work_of(3, n), 3, n, eps=EPS, dy_type="f32", in_type="f32")
+    for value, (want, error) in zip((dx, dgamma), ref.norm_gradients(dy, x, gamma, EPS)):
+        ref.check(value, want, error, "f32")
+
+
 # ---- kernels that stay for several rows, and those that many rows choose
 
 
